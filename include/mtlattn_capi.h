@@ -315,6 +315,94 @@ int mtlattn_paged_decode(const mtlattn_problem* p,
                          void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/*
+ * A paged KV cache held in 8 bits. No counterpart in the reference. Pages,
+ * token rows and the block table as for mtlattn_paged_decode; an element is a
+ * code, and a value is its code times the scale of its block of tokens and kv
+ * head. Codes: e4m3 (sign, 4 exponent and 3 mantissa bits, +-448 at most, one
+ * NaN) or int8 (-127 .. 127).
+ *   k, v            : codes [num_pages, page_size, Hkv, D], token row strides
+ *                     k_row_stride / v_row_stride (elements), rows and strides
+ *                     16-byte aligned (8-byte for writing and reading back)
+ *   k_scale, v_scale: fp32 [num_pages, page_size / block, Hkv], contiguous
+ *   block           : tokens that share a scale: 16, 32, 64, 128 or 256, and a
+ *                     divisor of page_size
+ * Writing and reading back take D a multiple of 8 in [16, 256] and
+ * Hkv * D <= 65536; attention D in {64, 128}.
+ */
+enum {
+    MTLATTN_CODE_E4M3 = 3,
+    MTLATTN_CODE_INT8 = 4
+};
+
+typedef struct mtlattn_cache8 {
+    int32_t code;             /* MTLATTN_CODE_* */
+    int32_t page_size;
+    int32_t block;
+    int32_t num_heads_kv;
+    int32_t head_dim;
+    int64_t num_pages;
+    void* k;
+    int64_t k_row_stride;
+    void* v;
+    int64_t v_row_stride;
+    float* k_scale;
+    float* v_scale;
+    const int32_t* block_table;    /* device int32 [num_seqs, block_table_stride] */
+    int64_t block_table_stride;
+} mtlattn_cache8;
+
+/*
+ * Writes rows k, v [total, Hkv, D] (dtype fp32 / fp16 / bf16, row strides in
+ * elements, 16-byte aligned rows) into the cache: sequence s's rows
+ * cu_seqlens[s] .. cu_seqlens[s + 1] become its last logical tokens, whose count
+ * cu_seqlens_kv (prefix sums, with the new tokens) gives -- the offsets that the
+ * attention over the cache then takes for its queries and keys.
+ * For each block and kv head that gets rows, with a = the largest magnitude
+ * among their finite values (at least 2^-92): need = the smallest power of two
+ * with a <= 448 need (e4m3), a / 127 (int8). A block that already holds tokens of
+ * the sequence keeps a larger scale; a smaller one grows to `need`, and the
+ * earlier tokens' codes are rounded to it. Codes are the nearest to value /
+ * scale, ties to even; infinities take the largest code, NaN stays NaN in e4m3
+ * and is 0 in int8. Nothing else of the cache changes.
+ * Rows whose logical position is negative (more rows than tokens), or whose
+ * table column or page does not exist, are not written. Blocks that get rows
+ * must belong to one sequence each. No workspace; deterministic.
+ */
+int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype,
+                         const void* k, int64_t k_row_stride,
+                         const void* v, int64_t v_row_stride,
+                         int64_t total, int32_t num_seqs,
+                         const int32_t* cu_seqlens, const int32_t* cu_seqlens_kv,
+                         void* stream);
+
+/*
+ * Reads the last tokens of each sequence back: rows cu_seqlens[s] ..
+ * cu_seqlens[s + 1] of k and v (contiguous [total, Hkv, D], 16-byte aligned, of
+ * type dtype) are its last logical tokens, code * scale rounded once. With
+ * cu_seqlens = cu_seqlens_kv: all of them. Table columns and pages are clamped
+ * as in the attention; rows of no sequence and of negative positions are 0.
+ */
+int mtlattn_cache8_read(const mtlattn_cache8* c, int32_t dtype,
+                        void* k, void* v,
+                        int64_t total, int32_t num_seqs,
+                        const int32_t* cu_seqlens, const int32_t* cu_seqlens_kv,
+                        void* stream);
+
+/*
+ * mtlattn_paged_decode over an 8-bit cache: same computation, options and
+ * limits (p->dtype is the type of q and out), on values code * scale. Query rows
+ * past the 16 / (heads per group) that p->max_seqlen_q promised come back NaN.
+ * Workspace: mtlattn_decode8_workspace_size(p, max_seqlen_kv) bytes.
+ */
+size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv);
+int mtlattn_decode8(const mtlattn_problem* p,
+                    const void* q, int64_t q_row_stride,
+                    const mtlattn_cache8* c, int64_t max_seqlen_kv,
+                    void* out, float* lse,
+                    void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 /* Number of split-KV work-item slots per (kv head, head group) the forward's
  * decode routing would use for `p` (0 = the call is not routed to split-KV).
  * The automatic path cuts each sequence's KV into fixed-length chunks (about

@@ -190,7 +190,8 @@ def flash_attn_varlen_kvpacked_func(q, kv, cu_seqlens_q, cu_seqlens_k, max_seqle
 
 
 def paged_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_table, max_seqlen_q,
-                 max_seqlen_kv, scale=None, causal=False, window=0, attn_bias=None, lse_out=None):
+                 max_seqlen_kv, scale=None, causal=False, window=0, attn_bias=None, lse_out=None,
+                 k_scale=None, v_scale=None):
     """Decode (max_seqlen_q <= 16 query rows per sequence) over a paged KV
     cache; the reference has no paged KV, the layout is FlashAttention's
     varlen call with a block table.
@@ -201,12 +202,61 @@ def paged_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_table, 
     int [B+1] prefix sums of the logical KV lengths; max_seqlen_kv bounds
     them. causal / window / attn_bias as in varlen_attention; lse_out: an
     optional fp32 [Mq, Hq] tensor receiving the natural-log LSE. Forward
-    only (fp16/bf16, D in {64, 128}). Returns [Mq, Hq, D]."""
+    only (fp16/bf16, D in {64, 128}). Returns [Mq, Hq, D].
+
+    With k_scale and v_scale the cache is one of 8-bit codes (see
+    paged_cache_write): float8_e4m3fn or int8 for any q type, values code *
+    scale."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("mtlattn: k_scale and v_scale go together")
+    if k_scale is not None:
+        return _C.paged_decode8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q.int(), cu_seqlens_kv.int(),
+                                block_table.int(), int(max_seqlen_q), int(max_seqlen_kv), float(scale), bool(causal),
+                                int(window), lse_out, _prep_bias(attn_bias))
     return _C.paged_decode(q, k_cache, v_cache, cu_seqlens_q.int(), cu_seqlens_kv.int(), block_table.int(),
                            int(max_seqlen_q), int(max_seqlen_kv), float(scale), bool(causal), int(window),
                            lse_out, _prep_bias(attn_bias))
+
+
+def paged_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_seqlens_kv, block_table):
+    """Write new K/V rows into a paged cache of 8-bit codes, in place (no
+    reference counterpart).
+
+    k, v: [M, Hkv, D] (fp32/fp16/bf16, row-strided views allowed), rows
+    cu_seqlens[s]..cu_seqlens[s+1] being the last logical tokens of sequence
+    s, of cu_seqlens_kv[s+1] - cu_seqlens_kv[s] in all: the offsets that
+    paged_decode then takes for its queries and keys. k_cache, v_cache:
+    [num_pages, page_size, Hkv, D] float8_e4m3fn or int8, block_table as for
+    paged_decode. k_scale, v_scale: fp32 [num_pages, page_size // block, Hkv],
+    one scale for each block of 16, 32, 64, 128 or 256 tokens and kv head.
+
+    A block's scale fits the largest finite magnitude of its rows: the
+    smallest power of two with magnitude <= 448 * scale (e4m3), magnitude /
+    127 (int8). Tokens appended to a block that holds earlier ones raise its
+    scale where they need it, and the earlier codes are rounded to the new
+    scale. Infinities take the largest code; NaN stays NaN in e4m3 and is 0
+    in int8. Rows without a place (a table column or page that does not
+    exist, more rows than tokens) are not written, so a page of -1 drops its
+    rows. A block that gets rows must belong to one sequence: copy shared
+    pages first. D: a multiple of 8 in [16, 256]."""
+    _C.paged_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, cu_seqlens.int(), cu_seqlens_kv.int(),
+                         block_table.int())
+
+
+def paged_cache_read(k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_seqlens_kv, block_table, total,
+                     dtype=torch.bfloat16):
+    """Read the last tokens of each sequence back from a paged cache of 8-bit
+    codes (no reference counterpart): (k, v), each [total, Hkv, D] in dtype
+    (fp32/fp16/bf16), rows cu_seqlens[s]..cu_seqlens[s+1] being sequence s's
+    last logical tokens, code * scale rounded once. With cu_seqlens_kv for
+    both offsets these are all tokens: the packed K/V that varlen_attention
+    takes, for prompts' chunks against the cache. total: the rows, at least
+    cu_seqlens[-1] (rows past it are 0). Other arguments as for
+    paged_cache_write."""
+    return _C.paged_cache_read(k_cache, v_cache, k_scale, v_scale, cu_seqlens.int(), cu_seqlens_kv.int(),
+                               block_table.int(), int(total), dtype)
 
 
 # ---- dense scaled_dot_product_attention adapter ----

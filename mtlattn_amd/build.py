@@ -26,7 +26,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmtlattn_hip.so")
 EXT = os.path.join(HERE, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 CALIB = os.path.join(HERE, "libmtlattn_calib.so")
-HIP_SOURCES = ["fwd.hip", "bwd.hip", "bwd_wide.hip", "decode.hip", "generic.hip", "f32mfma.hip", "pad.hip", "capi.hip"]
+HIP_SOURCES = ["fwd.hip", "bwd.hip", "bwd_wide.hip", "decode.hip", "decode8.hip", "cache8.hip", "generic.hip", "f32mfma.hip", "pad.hip", "capi.hip"]
 # Per-source flags. bwd_wide.hip pins its accumulators to the AGPRs by inline
 # asm and needs the compiler's own MFMA results in VGPRs, where the VALU reads
 # them.

@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(_HERE, "libmtlattn_hip.so")
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_LAUNCH = 0, -1, -2, -3, -4
+CODE_E4M3, CODE_INT8 = 3, 4
 ABI_VERSION = 2
 
 
@@ -36,13 +37,25 @@ class Problem(ctypes.Structure):
     ]
 
 
+class Cache8(ctypes.Structure):
+    """struct mtlattn_cache8 (field order and widths as in the header)."""
+    _fields_ = [
+        ("code", ctypes.c_int32), ("page_size", ctypes.c_int32), ("block", ctypes.c_int32),
+        ("num_heads_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("num_pages", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_row_stride", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_row_stride", ctypes.c_int64),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64),
+    ]
+
+
 class MtlattnError(RuntimeError):
     def __init__(self, fn, rc, msg):
         super().__init__(f"{fn} failed ({rc}): {msg}")
         self.rc = rc
 
 
-_P = ctypes.POINTER(Problem)
+_P, _C8 = ctypes.POINTER(Problem), ctypes.POINTER(Cache8)
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
 
 # name -> (restype, argtypes); checked against the header by the CPU tests
@@ -70,6 +83,10 @@ SIGNATURES = {
     "mtlattn_paged_decode_workspace_size": (_sz, [_P, _i64]),
     "mtlattn_paged_decode": (ctypes.c_int, [_P, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _i64, _i64, _vp,
                                             _vp, _vp, _sz, _vp]),
+    "mtlattn_cache8_write": (ctypes.c_int, [_C8, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "mtlattn_cache8_read": (ctypes.c_int, [_C8, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp]),
+    "mtlattn_decode8_workspace_size": (_sz, [_P, _i64]),
+    "mtlattn_decode8": (ctypes.c_int, [_P, _vp, _i64, _C8, _i64, _vp, _vp, _vp, _sz, _vp]),
     "mtlattn_pack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "mtlattn_unpack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                              _vp]),

@@ -172,7 +172,7 @@ size_t plan_bytes(const mtlattn_problem* p, const DecodePlan& plan) {
 
 int run_splitkv(const mtlattn_problem* p, const void* q, int64_t qrs, const void* k, int64_t krs, const void* v,
                 int64_t vrs, void* out, float* lse, const DecodePlan& plan, void* ws, size_t ws_bytes, hipStream_t st,
-                const PagedKV* paged = nullptr) {
+                const PagedKV* paged = nullptr, const mtlattn_cache8* c8 = nullptr) {
     const int ns = plan.ns, chunk = plan.chunk;
     const size_t need = plan_bytes(p, plan);
     if (ws_bytes < need || (ws == nullptr && need > 0))
@@ -194,6 +194,12 @@ int run_splitkv(const mtlattn_problem* p, const void* q, int64_t qrs, const void
         a.bt_stride = paged->bt_stride;
         a.page_size = paged->page_size;
         a.num_pages = (int)paged->num_pages;
+    }
+    if (c8 != nullptr) {
+        a.k_scale = c8->k_scale;
+        a.v_scale = c8->v_scale;
+        a.block = c8->block;
+        return launch_status(launch_decode8(p->dtype, c8->code, a, st), "8-bit decode");
     }
     return launch_status(launch_decode(p->dtype, a, st), "split-KV decode");
 }
@@ -325,6 +331,69 @@ DecodePlan paged_plan(const mtlattn_problem* p, int64_t max_seqlen_kv) {
     const int64_t c = plan_chunk(p, span * p->num_seqs);
     plan.ns = (int)((span + c - 1) / c);
     return plan;
+}
+
+// The same over an 8-bit cache.
+DecodePlan plan8(const mtlattn_problem* p, int64_t max_seqlen_kv) { return paged_plan(p, max_seqlen_kv); }
+
+// An 8-bit cache as every entry takes it (pointers apart).
+int check_cache8(const mtlattn_cache8* c, const char* what) {
+    if (c == nullptr) return fail(MTLATTN_ERR_INVALID, "%s: null cache descriptor", what);
+    if (c->code != MTLATTN_CODE_E4M3 && c->code != MTLATTN_CODE_INT8)
+        return fail(MTLATTN_ERR_INVALID, "%s: unknown cache code %d", what, c->code);
+    if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128 && c->block != 256)
+        return fail(MTLATTN_ERR_INVALID, "%s: tokens per scale must be 16, 32, 64, 128 or 256 (got %d)", what, c->block);
+    if (c->page_size < 1 || c->page_size % c->block != 0)
+        return fail(MTLATTN_ERR_INVALID, "%s: page_size (%d) must be a multiple of the tokens per scale (%d)", what,
+                    c->page_size, c->block);
+    if (c->num_pages < 1 || c->num_pages > 0x7fffffffLL || c->num_pages * (int64_t)c->page_size > 0x7fffffffLL)
+        return fail(MTLATTN_ERR_INVALID, "%s: num_pages * page_size must be in [1, 2^31)", what);
+    if (c->block_table_stride < 1) return fail(MTLATTN_ERR_INVALID, "%s: block_table_stride must be >= 1", what);
+    if (c->num_heads_kv < 1 || c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 8 != 0 ||
+        (int64_t)c->num_heads_kv * c->head_dim > 65536)
+        return fail(MTLATTN_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [16, 256] and Hkv * D at most 65536",
+                    what);
+    const int64_t row = (int64_t)c->num_heads_kv * c->head_dim;
+    if (c->k_row_stride < row || c->v_row_stride < row)
+        return fail(MTLATTN_ERR_INVALID, "%s: cache row strides must cover a row", what);
+    if (!tile_stride_ok(c->k_row_stride) || !tile_stride_ok(c->v_row_stride))
+        return fail(MTLATTN_ERR_UNSUPPORTED, "%s: cache row strides must be below 2^24", what);
+    return MTLATTN_OK;
+}
+
+bool cache8_pointers(const mtlattn_cache8* c) {
+    return c->k != nullptr && c->v != nullptr && c->k_scale != nullptr && c->v_scale != nullptr && c->block_table != nullptr;
+}
+
+bool cache8_aligned(const mtlattn_cache8* c, int64_t to) {
+    return (uintptr_t)c->k % to == 0 && (uintptr_t)c->v % to == 0 && c->k_row_stride % to == 0 && c->v_row_stride % to == 0 &&
+           (uintptr_t)c->k_scale % 4 == 0 && (uintptr_t)c->v_scale % 4 == 0;
+}
+
+// The rows of a write or a read (pointers apart).
+int check_cache8_rows(int32_t dtype, int64_t total, int32_t num_seqs, const int32_t* cu, const int32_t* cu_kv,
+                      const char* what) {
+    if (dtype != MTLATTN_DTYPE_F32 && dtype != MTLATTN_DTYPE_F16 && dtype != MTLATTN_DTYPE_BF16)
+        return fail(MTLATTN_ERR_INVALID, "%s: unsupported dtype code %d", what, dtype);
+    if (total < 0 || total > 0x7fffffffLL) return fail(MTLATTN_ERR_INVALID, "%s: bad row count", what);
+    if (num_seqs < 1 || cu == nullptr || cu_kv == nullptr)
+        return fail(MTLATTN_ERR_INVALID, "%s: cu_seqlens and cu_seqlens_kv must both be [B+1]", what);
+    return MTLATTN_OK;
+}
+
+Cache8Args cache8_args(const mtlattn_cache8* c, int64_t total, int32_t num_seqs, const int32_t* cu, const int32_t* cu_kv) {
+    Cache8Args a{};
+    a.code = c->code;
+    a.k_cache = (uint8_t*)c->k; a.v_cache = (uint8_t*)c->v;
+    a.kc_rs = c->k_row_stride; a.vc_rs = c->v_row_stride;
+    a.k_scale = c->k_scale; a.v_scale = c->v_scale;
+    a.page_size = c->page_size; a.block = c->block; a.num_pages = (int)c->num_pages;
+    a.hkv = c->num_heads_kv; a.d = c->head_dim;
+    a.block_table = c->block_table; a.bt_stride = c->block_table_stride;
+    a.cu = cu; a.cu_kv = cu_kv;
+    a.num_seqs = num_seqs;
+    a.total = total;
+    return a;
 }
 
 constexpr int kMaxDevices = 64;
@@ -930,6 +999,69 @@ int mtlattn_paged_decode(const mtlattn_problem* p, const void* q, int64_t q_row_
                        workspace_bytes, (hipStream_t)stream, &pk);
 }
 
+int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype, const void* k, int64_t k_row_stride, const void* v,
+                         int64_t v_row_stride, int64_t total, int32_t num_seqs, const int32_t* cu_seqlens,
+                         const int32_t* cu_seqlens_kv, void* stream) {
+    int rc = check_cache8(c, "cache8_write");
+    if (rc == MTLATTN_OK) rc = check_cache8_rows(dtype, total, num_seqs, cu_seqlens, cu_seqlens_kv, "cache8_write");
+    if (rc != MTLATTN_OK) return rc;
+    if (total == 0) return ok();
+    if (k == nullptr || v == nullptr || !cache8_pointers(c))
+        return fail(MTLATTN_ERR_INVALID, "cache8_write: null k/v/cache/scale/block_table pointer");
+    const int64_t row = (int64_t)c->num_heads_kv * c->head_dim;
+    if (total > 1 && (k_row_stride < row || v_row_stride < row))
+        return fail(MTLATTN_ERR_INVALID, "cache8_write: row strides must cover a row");
+    if (!aligned16(k, k_row_stride, dtype) || !aligned16(v, v_row_stride, dtype) || !cache8_aligned(c, 8))
+        return fail(MTLATTN_ERR_UNSUPPORTED, "cache8_write: k/v rows must be 16-byte aligned, cache rows 8-byte aligned");
+    Cache8Args a = cache8_args(c, total, num_seqs, cu_seqlens, cu_seqlens_kv);
+    a.k = const_cast<void*>(k); a.v = const_cast<void*>(v);
+    a.k_rs = k_row_stride; a.v_rs = v_row_stride;
+    return launch_status(launch_cache8_write(dtype, a, (hipStream_t)stream), "8-bit cache write");
+}
+
+int mtlattn_cache8_read(const mtlattn_cache8* c, int32_t dtype, void* k, void* v, int64_t total, int32_t num_seqs,
+                        const int32_t* cu_seqlens, const int32_t* cu_seqlens_kv, void* stream) {
+    int rc = check_cache8(c, "cache8_read");
+    if (rc == MTLATTN_OK) rc = check_cache8_rows(dtype, total, num_seqs, cu_seqlens, cu_seqlens_kv, "cache8_read");
+    if (rc != MTLATTN_OK) return rc;
+    if (total == 0) return ok();
+    if (k == nullptr || v == nullptr || !cache8_pointers(c))
+        return fail(MTLATTN_ERR_INVALID, "cache8_read: null k/v/cache/scale/block_table pointer");
+    if (((uintptr_t)k & 15u) != 0 || ((uintptr_t)v & 15u) != 0 || !cache8_aligned(c, 8))
+        return fail(MTLATTN_ERR_UNSUPPORTED, "cache8_read: k/v must be 16-byte aligned, cache rows 8-byte aligned");
+    Cache8Args a = cache8_args(c, total, num_seqs, cu_seqlens, cu_seqlens_kv);
+    a.k = k; a.v = v;
+    return launch_status(launch_cache8_read(dtype, a, (hipStream_t)stream), "8-bit cache read");
+}
+
+size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv) {
+    if (check_problem(p) != MTLATTN_OK || !splitkv_supported(p)) return 0;
+    return plan_bytes(p, plan8(p, max_seqlen_kv));
+}
+
+int mtlattn_decode8(const mtlattn_problem* p, const void* q, int64_t q_row_stride, const mtlattn_cache8* c,
+                    int64_t max_seqlen_kv, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+    int rc = check_problem(p);
+    if (rc == MTLATTN_OK) rc = check_cache8(c, "decode8");
+    if (rc != MTLATTN_OK) return rc;
+    if (!is16(p->dtype)) return fail(MTLATTN_ERR_UNSUPPORTED, "decode8: half/bf16");
+    if (!decode_head_dim(p->head_dim)) return fail(MTLATTN_ERR_UNSUPPORTED, "decode8: D in {64,128}");
+    if (p->max_seqlen_q < 1 || p->max_seqlen_q > 16)
+        return fail(MTLATTN_ERR_UNSUPPORTED, "decode8: max_seqlen_q must be in [1, 16]");
+    if (c->num_heads_kv != p->num_heads_kv || c->head_dim != p->head_dim)
+        return fail(MTLATTN_ERR_INVALID, "decode8: the cache's heads (%d x %d) are not the problem's (%d x %d)",
+                    c->num_heads_kv, c->head_dim, p->num_heads_kv, p->head_dim);
+    if (max_seqlen_kv < 0) return fail(MTLATTN_ERR_INVALID, "decode8: negative max_seqlen_kv");
+    if (p->total_q == 0) return ok();
+    if (q == nullptr || out == nullptr || !cache8_pointers(c))
+        return fail(MTLATTN_ERR_INVALID, "decode8: null q/cache/scale/block_table/out pointer");
+    if (!aligned16(q, q_row_stride, p->dtype) || !cache8_aligned(c, 16) || ((uintptr_t)out & 15u) != 0)
+        return fail(MTLATTN_ERR_UNSUPPORTED, "decode8: q and cache rows must be 16-byte aligned");
+    const PagedKV pk{c->block_table, c->block_table_stride, c->num_pages, c->page_size};
+    return run_splitkv(p, q, q_row_stride, c->k, c->k_row_stride, c->v, c->v_row_stride, out, lse,
+                       plan8(p, max_seqlen_kv), workspace, workspace_bytes, (hipStream_t)stream, &pk, c);
+}
 
 int mtlattn_pack_padded(int32_t dtype, int32_t B, int32_t N, int32_t H, int32_t D, const void* src, int64_t sb,
                         int64_t sh, int64_t sn, const int32_t* lens, int32_t* cu_out, void* dst, void* stream) {

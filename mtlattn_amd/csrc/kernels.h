@@ -168,6 +168,29 @@ struct DecodeArgs {
     const int* block_table = nullptr;
     int64_t bt_stride = 0;
     int page_size = 0, num_pages = 0;
+    // 8-bit caches (launch_decode8): fp32 scales [num_pages, page_size / block, hkv]
+    const float* k_scale = nullptr;
+    const float* v_scale = nullptr;
+    int block = 0;
+};
+
+// An 8-bit paged cache and the rows written to it or read from it
+// (launch_cache8_write / _read): rows [total, hkv, d] of type dtype with row
+// strides k_rs / v_rs, sequence s's rows cu[s] .. cu[s + 1] being its last
+// logical tokens, whose count cu_kv gives.
+struct Cache8Args {
+    int code;                                  // MTLATTN_CODE_*
+    uint8_t* k_cache; uint8_t* v_cache;        // token strides kc_rs / vc_rs (bytes)
+    int64_t kc_rs, vc_rs;
+    float* k_scale; float* v_scale;
+    int page_size, block, num_pages, hkv, d;
+    const int* block_table;
+    int64_t bt_stride;
+    const int* cu; const int* cu_kv;
+    int num_seqs;
+    int64_t total;
+    void* k; void* v;                          // rows: the input of a write, the output of a read
+    int64_t k_rs, v_rs;
 };
 
 // Launchers return hipSuccess or the launch error. `dtype` is MTLATTN_DTYPE_*.
@@ -207,6 +230,9 @@ struct ZeroFill {
 // Zeroes those rows of up to three tensors in one launch.
 hipError_t launch_zero_outside(const ZeroFill* fills, int n, int num_seqs, hipStream_t st);
 hipError_t launch_decode(int dtype, const DecodeArgs& a, hipStream_t st);
+hipError_t launch_decode8(int dtype, int code, const DecodeArgs& a, hipStream_t st);
+hipError_t launch_cache8_write(int dtype, const Cache8Args& a, hipStream_t st);
+hipError_t launch_cache8_read(int dtype, const Cache8Args& a, hipStream_t st);
 hipError_t launch_pad_pack(int esize, int B, int N, int H, int D, const void* src, int64_t sb, int64_t sh,
                            int64_t sn, const int* lens, int* cu, void* dst, hipStream_t st);
 hipError_t launch_pad_unpack(int esize, int B, int N, int H, int D, const void* src, const int* lens, const int* cu,

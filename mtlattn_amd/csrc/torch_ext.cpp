@@ -403,6 +403,158 @@ at::Tensor paged_decode(const at::Tensor& q, const at::Tensor& k_cache, const at
     return out;
 }
 
+// An 8-bit paged cache (no reference counterpart): codes
+// [num_pages, page_size, Hkv, D] of float8_e4m3fn or int8, laid out as for
+// paged_decode, and contiguous fp32 scales [num_pages, page_size / block, Hkv].
+// The descriptor points into `table`, which the caller keeps.
+mtlattn_cache8 make_cache8(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scale,
+                           const at::Tensor& v_scale, const at::Tensor& block_table, int64_t num_seqs,
+                           at::Tensor& table) {
+    TORCH_CHECK(k_cache.is_cuda(), "mtlattn: k_cache/v_cache must be GPU tensors");
+    TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes(),
+                "mtlattn: k_cache/v_cache must both be [num_pages, page_size, Hkv, D]");
+    TORCH_CHECK(k_cache.scalar_type() == v_cache.scalar_type() &&
+                    (k_cache.scalar_type() == at::kFloat8_e4m3fn || k_cache.scalar_type() == at::kChar),
+                "mtlattn: an 8-bit cache must be float8_e4m3fn or int8, keys and values alike");
+    const int64_t pages = k_cache.size(0), page_size = k_cache.size(1), Hkv = k_cache.size(2), D = k_cache.size(3);
+    TORCH_CHECK(pages > 0 && page_size > 0 && Hkv > 0 && D > 0, "mtlattn: empty cache");
+    for (const auto& c : {k_cache, v_cache}) {
+        TORCH_CHECK(c.stride(3) == 1 && (Hkv == 1 || c.stride(2) == D),
+                    "mtlattn: cache inner dims [Hkv, D] must be contiguous");
+        TORCH_CHECK(c.size(0) <= 1 || c.stride(0) == page_size * c.stride(1),
+                    "mtlattn: cache pages must be page_size consecutive token rows");
+    }
+    for (const auto& t : {k_scale, v_scale})
+        TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 3 && t.is_contiguous() && t.size(0) == pages &&
+                        t.size(1) == k_scale.size(1) && t.size(1) > 0 && page_size % t.size(1) == 0 && t.size(2) == Hkv,
+                    "mtlattn: k_scale/v_scale must be contiguous fp32 [num_pages, page_size / block, Hkv]");
+    TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == num_seqs &&
+                    block_table.size(1) > 0,
+                "mtlattn: block_table must be an int32 [B, max_pages] GPU tensor");
+    for (const auto& t : {v_cache, k_scale, v_scale, block_table})
+        TORCH_CHECK(t.is_cuda() && t.get_device() == k_cache.get_device(),
+                    "mtlattn: the cache, its scales and the block table must be on the same device");
+    table = block_table.contiguous();
+    mtlattn_cache8 c;
+    std::memset(&c, 0, sizeof(c));
+    c.code = k_cache.scalar_type() == at::kChar ? MTLATTN_CODE_INT8 : MTLATTN_CODE_E4M3;
+    c.page_size = (int32_t)std::min<int64_t>(page_size, 0x7fffffff);
+    c.block = (int32_t)std::min<int64_t>(page_size / k_scale.size(1), 0x7fffffff);
+    c.num_heads_kv = (int32_t)std::min<int64_t>(Hkv, 0x7fffffff);
+    c.head_dim = (int32_t)std::min<int64_t>(D, 0x7fffffff);
+    c.num_pages = pages;
+    c.k = k_cache.data_ptr();
+    c.k_row_stride = page_size > 1 ? k_cache.stride(1) : Hkv * D;
+    c.v = v_cache.data_ptr();
+    c.v_row_stride = page_size > 1 ? v_cache.stride(1) : Hkv * D;
+    c.k_scale = k_scale.data_ptr<float>();
+    c.v_scale = v_scale.data_ptr<float>();
+    c.block_table = table.data_ptr<int32_t>();
+    c.block_table_stride = table.size(1);
+    return c;
+}
+
+// _C.paged_cache_write: rows k, v [M, Hkv, D] into an 8-bit cache, as the last
+// logical tokens of their sequences.
+void paged_cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                       const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& cu_seqlens,
+                       const at::Tensor& cu_seqlens_kv, const at::Tensor& block_table) {
+    check_qkv(k, k, v);
+    check_cu(cu_seqlens, cu_seqlens_kv, k);
+    at::Tensor table;
+    const mtlattn_cache8 c =
+        make_cache8(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens.numel() - 1, table);
+    TORCH_CHECK(k_cache.get_device() == k.get_device(), "mtlattn: k/v and the cache must be on the same device");
+    TORCH_CHECK(k.size(1) == k_cache.size(2) && k.size(2) == k_cache.size(3),
+                "mtlattn: k/v heads and head dim must be the cache's");
+    const c10::OptionalDeviceGuard guard(k.device());
+    auto cu = cu_seqlens.contiguous(), cu_kv = cu_seqlens_kv.contiguous();
+    check_rc(mtlattn_cache8_write(&c, dtype_code(k.scalar_type()), k.data_ptr(), row_stride(k), v.data_ptr(),
+                                  row_stride(v), k.size(0), (int32_t)(cu.numel() - 1), cu.data_ptr<int32_t>(),
+                                  cu_kv.data_ptr<int32_t>(), current_stream(k)));
+}
+
+// _C.paged_cache_read: the last logical tokens of each sequence as rows
+// [total, Hkv, D] of `dtype`.
+std::tuple<at::Tensor, at::Tensor> paged_cache_read(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                    const at::Tensor& k_scale, const at::Tensor& v_scale,
+                                                    const at::Tensor& cu_seqlens, const at::Tensor& cu_seqlens_kv,
+                                                    const at::Tensor& block_table, int64_t total,
+                                                    at::ScalarType dtype) {
+    const int code = dtype_code(dtype);
+    check_cu(cu_seqlens, cu_seqlens_kv, k_cache);
+    at::Tensor table;
+    const mtlattn_cache8 c =
+        make_cache8(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens.numel() - 1, table);
+    TORCH_CHECK(total >= 0, "mtlattn: total must not be negative");
+    const c10::OptionalDeviceGuard guard(k_cache.device());
+    auto cu = cu_seqlens.contiguous(), cu_kv = cu_seqlens_kv.contiguous();
+    auto k = at::empty({total, k_cache.size(2), k_cache.size(3)}, k_cache.options().dtype(dtype));
+    auto v = at::empty_like(k);
+    if (total > 0)
+        check_rc(mtlattn_cache8_read(&c, code, k.data_ptr(), v.data_ptr(), total, (int32_t)(cu.numel() - 1),
+                                     cu.data_ptr<int32_t>(), cu_kv.data_ptr<int32_t>(), current_stream(k_cache)));
+    return {k, v};
+}
+
+// _C.paged_decode8: paged_decode over an 8-bit cache.
+at::Tensor paged_decode8(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& cu_seqlens_q,
+                         const at::Tensor& cu_seqlens_kv, const at::Tensor& block_table, int64_t max_seqlen_q,
+                         int64_t max_seqlen_kv, double scale, bool causal, int64_t window,
+                         c10::optional<at::Tensor> lse_out, c10::optional<at::Tensor> attn_bias) {
+    TORCH_CHECK(q.is_cuda(), "mtlattn: q must be a GPU tensor");
+    TORCH_CHECK(q.dim() == 3, "mtlattn: q must be [M, H, D]");
+    check_cu(cu_seqlens_q, cu_seqlens_kv, q);
+    at::Tensor table;
+    const mtlattn_cache8 c =
+        make_cache8(k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens_q.numel() - 1, table);
+    const int64_t D = q.size(2), Hkv = k_cache.size(2), page_size = k_cache.size(1);
+    TORCH_CHECK(k_cache.size(3) == D, "mtlattn: k_cache head dim must match q");
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) % Hkv == 0, "mtlattn: query heads must be a multiple of kv heads");
+    TORCH_CHECK((q.size(2) == 1 || q.stride(2) == 1) && (q.size(1) == 1 || q.stride(1) == D),
+                "mtlattn: q inner dims must be contiguous");
+    TORCH_CHECK(k_cache.get_device() == q.get_device(), "mtlattn: q and the caches must be on the same device");
+    const c10::OptionalDeviceGuard guard(q.device());
+    auto cu_q = cu_seqlens_q.contiguous(), cu_kv = cu_seqlens_kv.contiguous();
+    TORCH_CHECK(max_seqlen_kv >= 0 && block_table.size(1) * page_size >= max_seqlen_kv,
+                "mtlattn: block_table has ", block_table.size(1), " pages of ", page_size,
+                " tokens per sequence, fewer than max_seqlen_kv (", max_seqlen_kv, ")");
+    auto out = at::empty({q.size(0), q.size(1), D}, q.options());
+    float* lse = nullptr;
+    if (defined(lse_out)) {
+        const at::Tensor& l = *lse_out;
+        TORCH_CHECK(l.is_cuda() && l.get_device() == q.get_device() && l.scalar_type() == at::kFloat &&
+                        l.is_contiguous() && l.dim() == 2 && l.size(0) == q.size(0) && l.size(1) == q.size(1),
+                    "mtlattn: lse_out must be a contiguous fp32 [total_q, H] GPU tensor");
+        lse = l.data_ptr<float>();
+    }
+    mtlattn_problem p;
+    std::memset(&p, 0, sizeof(p));
+    p.dtype = dtype_code(q.scalar_type());
+    if (q.size(0) == 0) return out;
+    p.num_seqs = (int32_t)(cu_q.numel() - 1);
+    p.total_q = q.size(0);
+    // (a bound on the logical KV total: sequences may share pages)
+    p.total_kv = std::min<int64_t>((int64_t)p.num_seqs * max_seqlen_kv, 0x7fffffff);
+    p.num_heads_q = (int32_t)q.size(1);
+    p.num_heads_kv = (int32_t)Hkv;
+    p.head_dim = (int32_t)D;
+    p.max_seqlen_q = (int32_t)std::min<int64_t>(max_seqlen_q, 0x7fffffff);
+    p.scale = (float)scale;
+    p.causal = causal ? 1 : 0;
+    p.window = window > 0 ? (int32_t)std::min<int64_t>(window, 0x7fffffff) : 0;
+    p.cu_seqlens_q = cu_q.data_ptr<int32_t>();
+    p.cu_seqlens_kv = cu_kv.data_ptr<int32_t>();
+    at::Tensor bias_keep;
+    fill_bias(p, attn_bias, q, bias_keep);
+    const size_t ws_bytes = mtlattn_decode8_workspace_size(&p, max_seqlen_kv);
+    at::Tensor ws = workspace((int64_t)ws_bytes, q);
+    check_rc(mtlattn_decode8(&p, q.data_ptr(), row_stride(q), &c, max_seqlen_kv, out.data_ptr(), lse, ws.data_ptr(),
+                             ws_bytes, current_stream(q)));
+    return out;
+}
+
 // _C.mpp_bwd_dq (src/ext.mm:656-711): fp32 dQ.
 at::Tensor mpp_bwd_dq(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& dO,
                       const at::Tensor& lse, const at::Tensor& delta, const at::Tensor& cu_q_in,
@@ -538,6 +690,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("k_cache"), py::arg("v_cache"), py::arg("cu_seqlens_q"), py::arg("cu_seqlens_kv"),
           py::arg("block_table"), py::arg("max_seqlen_q"), py::arg("max_seqlen_kv"), py::arg("scale"),
           py::arg("causal") = false, py::arg("window") = 0, py::arg("lse_out") = c10::nullopt,
+          py::arg("attn_bias") = c10::nullopt);
+    m.def("paged_cache_write", &paged_cache_write, "rows into a paged KV cache of 8-bit codes", py::arg("k"),
+          py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"),
+          py::arg("cu_seqlens"), py::arg("cu_seqlens_kv"), py::arg("block_table"));
+    m.def("paged_cache_read", &paged_cache_read, "the last tokens of each sequence out of an 8-bit cache",
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seqlens"),
+          py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("total"), py::arg("dtype"));
+    m.def("paged_decode8", &paged_decode8, "paged_decode over an 8-bit cache", py::arg("q"), py::arg("k_cache"),
+          py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seqlens_q"),
+          py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("max_seqlen_q"), py::arg("max_seqlen_kv"),
+          py::arg("scale"), py::arg("causal") = false, py::arg("window") = 0, py::arg("lse_out") = c10::nullopt,
           py::arg("attn_bias") = c10::nullopt);
     m.def("mpp_bwd_dkv", &mpp_bwd_dkv, "dK/dV backward kernel, fp32 outputs (test entry)", py::arg("q"), py::arg("k"),
           py::arg("v"), py::arg("dO"), py::arg("lse"), py::arg("delta"), py::arg("cu_q"), py::arg("cu_kv"),
