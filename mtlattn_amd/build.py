@@ -29,8 +29,9 @@ CALIB = os.path.join(HERE, "libmtlattn_calib.so")
 HIP_SOURCES = ["fwd.hip", "bwd.hip", "bwd_wide.hip", "decode.hip", "decode8.hip", "cache8.hip", "generic.hip", "f32mfma.hip", "pad.hip", "capi.hip"]
 # Per-source flags. bwd_wide.hip pins its accumulators to the AGPRs by inline
 # asm and needs the compiler's own MFMA results in VGPRs, where the VALU reads
-# them.
-SOURCE_FLAGS = {"bwd_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# them; decode8.hip's accumulators are rescaled by the VALU.
+SOURCE_FLAGS = {"bwd_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+                "decode8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = os.environ.get("MTLATTN_ARCH", "gfx950")

@@ -172,7 +172,7 @@ size_t plan_bytes(const mtlattn_problem* p, const DecodePlan& plan) {
 
 int run_splitkv(const mtlattn_problem* p, const void* q, int64_t qrs, const void* k, int64_t krs, const void* v,
                 int64_t vrs, void* out, float* lse, const DecodePlan& plan, void* ws, size_t ws_bytes, hipStream_t st,
-                const PagedKV* paged = nullptr, const mtlattn_cache8* c8 = nullptr) {
+                const PagedKV* paged = nullptr) {
     const int ns = plan.ns, chunk = plan.chunk;
     const size_t need = plan_bytes(p, plan);
     if (ws_bytes < need || (ws == nullptr && need > 0))
@@ -194,12 +194,6 @@ int run_splitkv(const mtlattn_problem* p, const void* q, int64_t qrs, const void
         a.bt_stride = paged->bt_stride;
         a.page_size = paged->page_size;
         a.num_pages = (int)paged->num_pages;
-    }
-    if (c8 != nullptr) {
-        a.k_scale = c8->k_scale;
-        a.v_scale = c8->v_scale;
-        a.block = c8->block;
-        return launch_status(launch_decode8(p->dtype, c8->code, a, st), "8-bit decode");
     }
     return launch_status(launch_decode(p->dtype, a, st), "split-KV decode");
 }
@@ -333,8 +327,17 @@ DecodePlan paged_plan(const mtlattn_problem* p, int64_t max_seqlen_kv) {
     return plan;
 }
 
-// The same over an 8-bit cache.
-DecodePlan plan8(const mtlattn_problem* p, int64_t max_seqlen_kv) { return paged_plan(p, max_seqlen_kv); }
+Dec8Plan plan8(const mtlattn_problem* p, int64_t max_seqlen_kv) {
+    return make_dec8_plan(make_geo(p), p->max_seqlen_q, max_seqlen_kv, device_cus());
+}
+
+// Workspace of a decode over an 8-bit cache: its partial rows, then their LSEs.
+size_t plan8_o_bytes(const mtlattn_problem* p, const Dec8Plan& plan) {
+    return ((size_t)plan.rows * (size_t)p->head_dim * sizeof(float) + 255) & ~(size_t)255;
+}
+size_t plan8_bytes(const mtlattn_problem* p, const Dec8Plan& plan) {
+    return plan8_o_bytes(p, plan) + (size_t)plan.rows * sizeof(float);
+}
 
 // An 8-bit cache as every entry takes it (pointers apart).
 int check_cache8(const mtlattn_cache8* c, const char* what) {
@@ -1036,7 +1039,7 @@ int mtlattn_cache8_read(const mtlattn_cache8* c, int32_t dtype, void* k, void* v
 
 size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv) {
     if (check_problem(p) != MTLATTN_OK || !splitkv_supported(p)) return 0;
-    return plan_bytes(p, plan8(p, max_seqlen_kv));
+    return plan8_bytes(p, plan8(p, max_seqlen_kv));
 }
 
 int mtlattn_decode8(const mtlattn_problem* p, const void* q, int64_t q_row_stride, const mtlattn_cache8* c,
@@ -1058,9 +1061,24 @@ int mtlattn_decode8(const mtlattn_problem* p, const void* q, int64_t q_row_strid
         return fail(MTLATTN_ERR_INVALID, "decode8: null q/cache/scale/block_table/out pointer");
     if (!aligned16(q, q_row_stride, p->dtype) || !cache8_aligned(c, 16) || ((uintptr_t)out & 15u) != 0)
         return fail(MTLATTN_ERR_UNSUPPORTED, "decode8: q and cache rows must be 16-byte aligned");
-    const PagedKV pk{c->block_table, c->block_table_stride, c->num_pages, c->page_size};
-    return run_splitkv(p, q, q_row_stride, c->k, c->k_row_stride, c->v, c->v_row_stride, out, lse,
-                       plan8(p, max_seqlen_kv), workspace, workspace_bytes, (hipStream_t)stream, &pk, c);
+    Dec8Args a{};
+    a.plan = plan8(p, max_seqlen_kv);
+    const size_t need = plan8_bytes(p, a.plan);
+    if (workspace_bytes < need || (workspace == nullptr && need > 0))
+        return fail(MTLATTN_ERR_WORKSPACE, "decode8: workspace too small (%zu < %zu bytes)", workspace_bytes, need);
+    if (need > 0 && ((uintptr_t)workspace & 15u) != 0)
+        return fail(MTLATTN_ERR_WORKSPACE, "decode8: the workspace must be 16-byte aligned");
+    a.geo = make_geo(p);
+    a.q = q; a.q_rs = q_row_stride;
+    a.k = (const uint8_t*)c->k; a.k_rs = c->k_row_stride;
+    a.v = (const uint8_t*)c->v; a.v_rs = c->v_row_stride;
+    a.k_scale = c->k_scale; a.v_scale = c->v_scale;
+    a.page_size = c->page_size; a.block = c->block; a.num_pages = (int)c->num_pages;
+    a.block_table = c->block_table; a.bt_stride = c->block_table_stride;
+    a.o = out; a.lse = lse;
+    a.o_part = (float*)workspace;
+    a.lse_part = (float*)((char*)workspace + plan8_o_bytes(p, a.plan));
+    return launch_status(launch_decode8(p->dtype, c->code, a, (hipStream_t)stream), "8-bit decode");
 }
 
 int mtlattn_pack_padded(int32_t dtype, int32_t B, int32_t N, int32_t H, int32_t D, const void* src, int64_t sb,

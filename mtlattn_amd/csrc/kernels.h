@@ -168,10 +168,31 @@ struct DecodeArgs {
     const int* block_table = nullptr;
     int64_t bt_stride = 0;
     int page_size = 0, num_pages = 0;
-    // 8-bit caches (launch_decode8): fp32 scales [num_pages, page_size / block, hkv]
-    const float* k_scale = nullptr;
-    const float* v_scale = nullptr;
-    int block = 0;
+};
+
+// How a decode over an 8-bit cache is laid out (make_dec8_plan): `waves` per
+// workgroup, `hw` kv heads of a workgroup, `hpb` query heads of a 16-row group;
+// pieces > 0: the work in that many pieces, with `rows` partial rows (d values
+// and an LSE each) in the workspace; 0: a workgroup per sequence.
+struct Dec8Plan {
+    int waves = 8, hw = 1, hpb = 1, pieces = 0;
+    int64_t rows = 0;
+};
+Dec8Plan make_dec8_plan(const Geometry& g, int max_q, int64_t max_kv, int cus);
+
+// Decode over an 8-bit paged cache (layout as Cache8Args).
+struct Dec8Args {
+    Geometry geo;
+    const void* q; int64_t q_rs;
+    const uint8_t* k; int64_t k_rs;
+    const uint8_t* v; int64_t v_rs;
+    const float* k_scale; const float* v_scale;
+    int page_size, block, num_pages;
+    const int* block_table; int64_t bt_stride;
+    void* o;                      // contiguous [total_q, hq, d]
+    float* lse;                   // nullable
+    Dec8Plan plan;
+    float* o_part; float* lse_part;
 };
 
 // An 8-bit paged cache and the rows written to it or read from it
@@ -230,7 +251,7 @@ struct ZeroFill {
 // Zeroes those rows of up to three tensors in one launch.
 hipError_t launch_zero_outside(const ZeroFill* fills, int n, int num_seqs, hipStream_t st);
 hipError_t launch_decode(int dtype, const DecodeArgs& a, hipStream_t st);
-hipError_t launch_decode8(int dtype, int code, const DecodeArgs& a, hipStream_t st);
+hipError_t launch_decode8(int dtype, int code, const Dec8Args& a, hipStream_t st);
 hipError_t launch_cache8_write(int dtype, const Cache8Args& a, hipStream_t st);
 hipError_t launch_cache8_read(int dtype, const Cache8Args& a, hipStream_t st);
 hipError_t launch_pad_pack(int esize, int B, int N, int H, int D, const void* src, int64_t sb, int64_t sh,
