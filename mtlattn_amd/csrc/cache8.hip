@@ -25,6 +25,8 @@ namespace mtlattn {
 
 namespace {
 
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
 struct Cache8KParams {
     const void* in[2]; int64_t in_rs[2];       // rows of K and V (write)
     void* out[2];                              // rows of K and V (read; contiguous)
@@ -34,7 +36,7 @@ struct Cache8KParams {
     const int* cu; const int* cu_kv;
     int64_t total;
     int num_seqs, hkv, d, page_size, block, num_pages;
-    uint32_t div_row;                          // read: ceil(2^32 / units of a row)
+    uint32_t div_row, div_unit;                // read: ceil(2^32 / units (8 values) of a row, of a head)
     uint32_t div_head;                         // ceil(2^16 / (d / 8))
 };
 
@@ -44,25 +46,54 @@ __device__ inline int kv_length(const int* __restrict__ cu_kv, int s) {
     return (int)min(max(n, (int64_t)0), (int64_t)0x7ffffff0);
 }
 
-// Eight values of a row as fp32.
+// Eight values of a row, as they are stored, and as fp32.
 template <typename T>
-__device__ inline void load8(const typename T::raw* p, float* f) {
-    const u32x4_t x = ld16(p);
+struct Raw8 {
+    u32x4_t x;
+    __device__ inline void load(const typename T::raw* p) { x = ld16(p); }
+    __device__ inline void values(float* f) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = lo16<T>(x[i]);
-        f[2 * i + 1] = hi16<T>(x[i]);
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = lo16<T>(x[i]);
+            f[2 * i + 1] = hi16<T>(x[i]);
+        }
     }
-}
+    // The larger magnitudes' bits, in either half: patterns order as magnitudes do.
+    static constexpr uint32_t kInf = T::code == BF16::code ? 0x7f80u : 0x7c00u;
+    __device__ inline uint32_t max_bits(uint32_t m) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u16x2_t a = __builtin_bit_cast(u16x2_t, x[i] & 0x7fff7fffu), b = __builtin_bit_cast(u16x2_t, m);
+            m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, b));
+        }
+        return m;
+    }
+    __device__ static inline uint32_t fold(uint32_t m) { return max(m & 0xffffu, m >> 16); }
+    __device__ static inline float magnitude(uint32_t m) { return T::to_float((uint16_t)m); }
+};
 template <>
-__device__ inline void load8<F32>(const float* p, float* f) {
-    const u32x4_t x = ld16(p), y = ld16(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[i] = __uint_as_float(x[i]);
-        f[4 + i] = __uint_as_float(y[i]);
+struct Raw8<F32> {
+    u32x4_t x, y;
+    __device__ inline void load(const float* p) {
+        x = ld16(p);
+        y = ld16(p + 4);
     }
-}
+    __device__ inline void values(float* f) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[i] = __uint_as_float(x[i]);
+            f[4 + i] = __uint_as_float(y[i]);
+        }
+    }
+    static constexpr uint32_t kInf = 0x7f800000u;
+    __device__ inline uint32_t max_bits(uint32_t m) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, max(x[i] & 0x7fffffffu, y[i] & 0x7fffffffu));
+        return m;
+    }
+    __device__ static inline uint32_t fold(uint32_t m) { return m; }
+    __device__ static inline float magnitude(uint32_t m) { return __uint_as_float(m); }
+};
 template <typename T>
 __device__ inline void store8(typename T::raw* p, const float* f) {
     st16(p, u32x4_t{T::pack2(f[0], f[1]), T::pack2(f[2], f[3]), T::pack2(f[4], f[5]), T::pack2(f[6], f[7])});
@@ -84,37 +115,49 @@ __device__ inline float scale_for(float a) {
     return ldexpf(1.f, e - 9 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));
 }
 
-// Four values as codes of this scale (pow2: the scale is a power of two).
+// Four values as codes of this scale (pow2: the scale is a power of two; odd: there
+// may be values that are not finite or too large for the scale).
 template <typename C>
-__device__ inline uint32_t encode4(const float* x, float scale, float inv, bool pow2);
+__device__ inline uint32_t encode4(const float* x, float scale, float inv, bool pow2, bool odd);
 template <>
-__device__ inline uint32_t encode4<E4M3>(const float* x, float scale, float inv, bool pow2) {
+__device__ inline uint32_t encode4<E4M3>(const float* x, float scale, float inv, bool pow2, bool odd) {
     float y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float v = pow2 ? x[i] * inv : x[i] / scale;
-        const float u = v > 448.f ? 448.f : v;                  // (a NaN stays)
-        y[i] = u < -448.f ? -448.f : u;
+    for (int i = 0; i < 4; ++i) y[i] = pow2 ? x[i] * inv : x[i] / scale;
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[i] = y[i] > 448.f ? 448.f : y[i];                 // (a NaN stays)
+            y[i] = y[i] < -448.f ? -448.f : y[i];
+        }
     }
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
 }
 template <>
-__device__ inline uint32_t encode4<I8>(const float* x, float scale, float inv, bool) {
-    uint32_t w = 0;
+__device__ inline uint32_t encode4<I8>(const float* x, float scale, float inv, bool, bool odd) {
     const float half = 0.5f * scale, lim = 127.f * scale;
+    float n[4], r[4];
+    bool tie = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float v = fminf(fmaxf(x[i], -lim), lim);
-        // n is nearest(v / scale) or, next to a tie, the other neighbour: v - n scale
-        // is exact, and tells
-        float n = __builtin_rintf(v * inv);
-        const float r = fmaf(-n, scale, v);
-        const bool odd = ((int)n & 1) != 0;
-        if (r > half || (r == half && odd)) n += 1.f;
-        if (r < -half || (r == -half && odd)) n -= 1.f;
-        n = fminf(fmaxf(n, -127.f), 127.f);
-        const int c = x[i] == x[i] ? (int)n : 0;
+        const float v = odd ? fminf(fmaxf(x[i], -lim), lim) : x[i];
+        // n is nearest(v / scale) or, next to a tie, the other neighbour: the
+        // remainder v - n scale is exact, and tells
+        n[i] = __builtin_rintf(v * inv);
+        r[i] = fmaf(-n[i], scale, v);
+        tie = tie || fabsf(r[i]) >= half;
+    }
+    if (tie) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (fabsf(r[i]) > half || (fabsf(r[i]) == half && ((int)n[i] & 1) != 0)) n[i] += r[i] > 0.f ? 1.f : -1.f;
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int c = (int)n[i];
+        if (odd) c = x[i] == x[i] ? min(max(c, -127), 127) : 0;
         w |= ((uint32_t)c & 0xffu) << (8 * i);
     }
     return w;
@@ -132,85 +175,119 @@ __device__ inline uint32_t recode4(uint32_t w, double scale, double now) {
         const double x = (double)f[i] * scale / now;
         f[i] = (float)(C::code == I8::code ? __builtin_rint(x) : x);
     }
-    if (C::code == E4M3::code) return encode4<E4M3>(f, 1.f, 1.f, true);
-    return encode4<I8>(f, 1.f, 1.f, true);
+    if (C::code == E4M3::code) return encode4<E4M3>(f, 1.f, 1.f, true, true);
+    return encode4<I8>(f, 1.f, 1.f, true, true);
 }
 
 // One wave per 16 tokens of a block and kv head; the block / 16 waves of a
 // (block, head) meet in LDS for its largest magnitude. A workgroup holds W waves:
-// W / (block / 16) heads of one block. ITER * 64 lanes hold 8 values each,
-// 16 d values in all, in registers between the two uses of them. Blocks that a
-// sequence's new rows touch: slots cu[s] / block + 2 s + i, at least as many as
-// there can be, found without the host.
+// W / (block / 16) heads of one block, K or V; the other heads, then the other side,
+// of the block come next in the grid. ITER * 64 lanes hold 8 values each, 16 d
+// values in all, in registers between the two uses of them.
+// The blocks that a sequence's new rows touch are numbered over the sequences, 64 of
+// them at a time, one lane each (total / block + 2 num_seqs bounds them); a wave's
+// rows do not need the page table, so that their loads and its lookup go out
+// together: offsets, then rows, then stores (a binary search, the ranges, the page
+// and the rows one after the other took 132 us for 64800 tokens of 8 heads, D = 128,
+// bf16, against 91 now, 402 MB).
 template <typename T, typename C, int ITER, int W>
 __global__ __launch_bounds__(W * 64) void cache8_write_kernel(Cache8KParams p) {
-    __shared__ float s_max[W], s_old[W];
+    __shared__ uint32_t s_max[W];
+    __shared__ float s_old[W];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int sub = p.block / 16, team = w / sub, part = w - team * sub;
-    const int side = blockIdx.z, slot = blockIdx.x;
+    const int sub = p.block / 16, team = w / sub, part = w - team * sub, heads = W / sub;
+    const int groups = (p.hkv + heads - 1) / heads;
+    const int head = (int)(blockIdx.x % groups) * heads + team, side = blockIdx.x / groups % 2;
+    const int slot = blockIdx.x / groups / 2;
 
-    int lo = 0, hi = p.num_seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        const int c = min(max(p.cu[mid], 0), (int)p.total);
-        if (c / p.block + 2 * mid <= slot) lo = mid; else hi = mid - 1;
+    int s = -1, blk = 0, start = 0, p0 = 0, p1 = 0, base = 0;
+    for (int g0 = 0; g0 < p.num_seqs && s < 0; g0 += 64) {
+        const int i = min(g0 + lane, p.num_seqs - 1);
+        const SeqRange r = seq_range(p.cu, i, p.total);
+        const int kv = kv_length(p.cu_kv, i), n = r.end - r.start, from = max(kv - n, 0) / p.block;
+        const int mine = g0 + lane < p.num_seqs && n > 0 && kv > 0 ? (kv - 1) / p.block - from + 1 : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(sum, o);
+            if (lane >= o) sum += y;
+        }
+        const uint64_t past = __ballot(base + sum > slot);
+        if (past != 0) {
+            const int l = __builtin_ctzll(past);
+            s = g0 + l;
+            blk = __builtin_amdgcn_readlane(from, l) + slot - base - __builtin_amdgcn_readlane(sum - mine, l);
+            start = __builtin_amdgcn_readlane(r.start, l);
+            p1 = __builtin_amdgcn_readlane(kv, l);
+            p0 = p1 - __builtin_amdgcn_readlane(n, l);
+        }
+        base += __builtin_amdgcn_readlane(sum, 63);
     }
-    const int s = lo;
-    const SeqRange nr = seq_range(p.cu, s, p.total);
-    const int n_new = nr.end - nr.start, p1 = kv_length(p.cu_kv, s), p0 = p1 - n_new;
-    const int64_t blk = max(p0, 0) / p.block + (slot - (nr.start / p.block + 2 * s));
-    const int64_t b0 = blk * p.block;                           // first token of the block
-    if (n_new == 0 || b0 >= p1) return;
+    if (s < 0) return;
+    const int b0 = blk * p.block;                               // first token of the block
+    const bool active = head < p.hkv, held = b0 < p0;           // earlier tokens in the block
     const int64_t col = b0 / p.page_size;
-    if (col >= p.bt_stride) return;
-    const int pg = p.block_table[(int64_t)s * p.bt_stride + col];
-    if (pg < 0 || pg >= p.num_pages) return;
-    const int64_t row0 = (int64_t)pg * p.page_size + (b0 - col * p.page_size);
+    const int pg = col < p.bt_stride ? p.block_table[(int64_t)s * p.bt_stride + col] : -1;
 
-    const int head = blockIdx.y * (W / sub) + team;
-    const bool active = head < p.hkv;
-    const int du = p.d / 8;
-    float* scale_at = p.scale[side] + (row0 / p.block) * p.hkv + head;
-    const bool held = b0 < p0;                                  // earlier tokens in the block
-    float old = 0.f;
-    if (active && held && part == 0) old = *scale_at;
-
-    float x[ITER][8];
-    u32x2_t code[ITER];
+    Raw8<T> x[ITER];
     int kind[ITER];                                             // 1: new, 2: earlier
-    float amax = 0.f;
+    const int du = p.d / 8;
     const typename T::raw* in = (const typename T::raw*)p.in[side] + (int64_t)head * p.d;
-    uint8_t* codes = p.codes[side] + (row0 + 16 * part) * p.c_rs[side] + (int64_t)head * p.d;
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
         const int e = lane + 64 * it, t = (int)(((uint32_t)e * p.div_head) >> 16), c = e - t * du;
-        const int64_t pos = b0 + 16 * part + t;
+        const int pos = b0 + 16 * part + t;
         kind[it] = !active || t >= 16 || pos >= p1 ? 0 : pos >= p0 ? 1 : 2;
-        if (kind[it] == 1) load8<T>(in + (nr.start + (pos - p0)) * p.in_rs[side] + 8 * c, x[it]);
-        if (kind[it] == 2) code[it] = ld8(codes + t * p.c_rs[side] + 8 * c);
+        if (kind[it] == 1) x[it].load(in + (start + (pos - p0)) * p.in_rs[side] + 8 * c);
     }
+    if (pg < 0 || pg >= p.num_pages) return;                    // (the whole workgroup)
+    const int64_t row0 = (int64_t)pg * p.page_size + (b0 - (int)col * p.page_size);
+    float* scale_at = p.scale[side] + (row0 / p.block) * p.hkv + head;
+    uint8_t* codes = p.codes[side] + (row0 + 16 * part) * p.c_rs[side] + (int64_t)head * p.d;
+    float old = 0.f;
+    u32x2_t code[ITER];
+    if (held && active) {
+        if (part == 0) old = *scale_at;
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-        if (kind[it] != 1) continue;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float m = fabsf(x[it][i]);
-            amax = m < kPosInf ? fmaxf(amax, m) : amax;         // (finite values)
+        for (int it = 0; it < ITER; ++it) {
+            const int e = lane + 64 * it, t = (int)(((uint32_t)e * p.div_head) >> 16), c = e - t * du;
+            if (kind[it] == 2) code[it] = ld8(codes + t * p.c_rs[side] + 8 * c);
         }
     }
-    amax = wave_max(amax);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int it = 0; it < ITER; ++it)
+        if (kind[it] == 1) bits = x[it].max_bits(bits);
+    bits = Raw8<T>::fold(bits);
+    bool odd = __any(bits >= Raw8<T>::kInf);                    // something is not finite
+    if (odd) {
+        float a = 0.f;
+#pragma unroll
+        for (int it = 0; it < ITER; ++it) {
+            if (kind[it] != 1) continue;
+            float f[8];
+            x[it].values(f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a = fabsf(f[i]) < kPosInf ? fmaxf(a, fabsf(f[i])) : a;
+        }
+        bits = __float_as_uint(a);
+    } else {
+        bits = __float_as_uint(Raw8<T>::magnitude(bits));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, o));
     if (sub > 1) {
         if (lane == 0) {
-            s_max[w] = amax;
+            s_max[w] = bits;
             if (part == 0) s_old[team] = old;
         }
         __syncthreads();
-        for (int i = 0; i < sub; ++i) amax = fmaxf(amax, s_max[team * sub + i]);
+        for (int i = 0; i < sub; ++i) bits = max(bits, s_max[team * sub + i]);
         old = s_old[team];
     }
     if (!active) return;
     old = __shfl(old, 0);
-    const float need = scale_for<C>(amax);
+    const float need = scale_for<C>(__uint_as_float(bits));
     const float now = held && old > need ? old : need;
     const float inv = 1.f / now;
     const bool pow2 = (__float_as_uint(now) & 0x7fffffu) == 0;
@@ -218,11 +295,14 @@ __global__ __launch_bounds__(W * 64) void cache8_write_kernel(Cache8KParams p) {
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
         const int e = lane + 64 * it, t = (int)(((uint32_t)e * p.div_head) >> 16), c = e - t * du;
-        if (kind[it] == 1)
+        if (kind[it] == 1) {
+            float f[8];
+            x[it].values(f);
             st8(codes + t * p.c_rs[side] + 8 * c,
-                u32x2_t{encode4<C>(x[it], now, inv, pow2), encode4<C>(x[it] + 4, now, inv, pow2)});
-        else if (kind[it] == 2 && grew)
+                u32x2_t{encode4<C>(f, now, inv, pow2, odd), encode4<C>(f + 4, now, inv, pow2, odd)});
+        } else if (kind[it] == 2 && grew) {
             st8(codes + t * p.c_rs[side] + 8 * c, u32x2_t{recode4<C>(code[it][0], old, now), recode4<C>(code[it][1], old, now)});
+        }
     }
     if (part == 0 && lane == 0 && (!held || grew)) *scale_at = now;
 }
@@ -233,45 +313,79 @@ constexpr int kReadRows = 16;
 // them stream 8 values at a time. Rows of no sequence are written as 0.
 template <typename T, typename C>
 __global__ __launch_bounds__(256) void cache8_read_kernel(Cache8KParams p) {
-    __shared__ int64_t s_row[kReadRows];
-    const int side = blockIdx.y;
+    __shared__ int s_row[kReadRows], s_srow[kReadRows];         // cache row (-1: none), row of scales
+    const int side = blockIdx.y, tid = threadIdx.x;
     const int64_t r0 = (int64_t)blockIdx.x * kReadRows;
-    if (threadIdx.x < kReadRows) {
-        const int64_t r = r0 + threadIdx.x;
-        int lo = 0, hi = p.num_seqs - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (p.cu[mid] <= r) lo = mid; else hi = mid - 1;
-        }
-        const SeqRange nr = seq_range(p.cu, lo, p.total);
-        int64_t row = -1;
-        if (r >= nr.start && r < nr.end) {
-            const int64_t pos = (int64_t)kv_length(p.cu_kv, lo) - (nr.end - r);
-            if (pos >= 0) {
-                const int64_t col = min(pos / p.page_size, p.bt_stride - 1);
-                const int pg = min(max(p.block_table[(int64_t)lo * p.bt_stride + col], 0), p.num_pages - 1);
-                row = (int64_t)pg * p.page_size + pos % p.page_size;
+    if (tid < 64) {
+        // lane t: row r0 + t. Among 64 sequences by one load of all lanes, among more by a search
+        const int r = (int)min(r0 + min(tid, kReadRows - 1), (int64_t)0x7fffffff);
+        int lo = 0;
+        SeqRange nr;
+        int kv;
+        if (p.num_seqs <= 64) {
+            const int i = min(tid, p.num_seqs - 1), first = p.cu[i];
+            const SeqRange mine = seq_range(p.cu, i, p.total);
+            const int len = kv_length(p.cu_kv, i);
+            for (int t = 0; t < kReadRows; ++t) {
+                const uint64_t le = __ballot(tid < p.num_seqs && first <= r0 + t);
+                if (tid == t) lo = 63 - __builtin_clzll(le | 1);
             }
+            nr.start = __shfl(mine.start, lo);
+            nr.end = __shfl(mine.end, lo);
+            kv = __shfl(len, lo);
+        } else {
+            int hi = p.num_seqs - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (p.cu[mid] <= r) lo = mid; else hi = mid - 1;
+            }
+            nr = seq_range(p.cu, lo, p.total);
+            kv = kv_length(p.cu_kv, lo);
         }
-        s_row[threadIdx.x] = row;
+        if (tid < kReadRows) {
+            const int pos = r < nr.end ? kv - (nr.end - r) : -1;
+            int row = -1;
+            if (r >= nr.start && pos >= 0) {
+                const int page = pos / p.page_size;
+                const int64_t col = min((int64_t)page, p.bt_stride - 1);
+                const int pg = min(max(p.block_table[(int64_t)lo * p.bt_stride + col], 0), p.num_pages - 1);
+                row = pg * p.page_size + (pos - page * p.page_size);
+            }
+            s_row[tid] = row;
+            s_srow[tid] = row / p.block;
+        }
     }
     __syncthreads();
-    const int rows = (int)min((int64_t)kReadRows, p.total - r0), du = p.d / 8, upr = p.hkv * du;
+    const int rows = (int)min((int64_t)kReadRows, p.total - r0), upr = p.hkv * (p.d / 8);
     typename T::raw* out = (typename T::raw*)p.out[side] + r0 * p.hkv * p.d;
-    for (int u = threadIdx.x; u < rows * upr; u += 256) {
-        const int t = (int)__umulhi((uint32_t)u, p.div_row), i = u - t * upr;
-        const int64_t row = s_row[t];
-        float f[8] = {};
-        if (row >= 0) {
-            const int head = i / du;
-            const u32x2_t w = ld8(p.codes[side] + row * p.c_rs[side] + 8 * i);
-            const float sc = p.scale[side][(row / p.block) * p.hkv + head];
-            C::to_float4(w[0], f);
-            C::to_float4(w[1], f + 4);
+    // four units' loads in flight (one at a time: 500 rows of 8 heads 6.6 us against 5.8)
+    constexpr int U = 4;
+    for (int u0 = tid; u0 < rows * upr; u0 += 256 * U) {
+        u32x2_t w[U];
+        float sc[U];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] *= sc;
+        for (int k = 0; k < U; ++k) {
+            const int u = u0 + 256 * k, t = (int)__umulhi((uint32_t)u, p.div_row), i = u - t * upr;
+            const int row = u < rows * upr ? s_row[t] : -1;
+            w[k] = u32x2_t{0u, 0u};
+            sc[k] = 0.f;
+            if (row >= 0) {
+                const int head = (int)__umulhi((uint32_t)i, p.div_unit);
+                w[k] = ld8(p.codes[side] + row * p.c_rs[side] + 8 * i);
+                sc[k] = p.scale[side][(int64_t)s_srow[t] * p.hkv + head];
+            }
         }
-        store8<T>(out + (int64_t)u * 8, f);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int u = u0 + 256 * k;
+            if (u >= rows * upr) break;
+            float f[8];
+            C::to_float4(w[k][0], f);
+            C::to_float4(w[k][1], f + 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= sc[k];
+            store8<T>(out + (int64_t)u * 8, f);
+        }
     }
 }
 
@@ -290,6 +404,7 @@ Cache8KParams params(const Cache8Args& a) {
     p.page_size = a.page_size; p.block = a.block; p.num_pages = a.num_pages;
     const uint64_t upr = (uint64_t)a.hkv * (a.d / 8);
     p.div_row = (uint32_t)(((1ull << 32) + upr - 1) / upr);
+    p.div_unit = (uint32_t)(((1ull << 32) + a.d / 8 - 1) / (a.d / 8));
     p.div_head = (65536u + a.d / 8 - 1) / (a.d / 8);
     return p;
 }
@@ -299,8 +414,9 @@ hipError_t write_iter(const Cache8KParams& p, hipStream_t st) {
     const int sub = p.block / 16, W = sub <= 8 ? 8 : 16;
     const int64_t slots = p.total / p.block + 2 * (int64_t)p.num_seqs;
     const int heads = W / sub;
-    const dim3 grid((unsigned)slots, (unsigned)((p.hkv + heads - 1) / heads), 2);
-    if (slots > 0x7fffffff || grid.y > 65535) return hipErrorInvalidValue;
+    const int64_t wgs = slots * ((p.hkv + heads - 1) / heads) * 2;
+    if (wgs > 0x7fffffff) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)wgs);
     if (W == 8) hipLaunchKernelGGL((cache8_write_kernel<T, C, ITER, 8>), grid, dim3(512), 0, st, p);
     else hipLaunchKernelGGL((cache8_write_kernel<T, C, ITER, 16>), grid, dim3(1024), 0, st, p);
     return hipGetLastError();
