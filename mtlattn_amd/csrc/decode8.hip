@@ -41,19 +41,31 @@ struct Dec8Params {
     const uint8_t* k; const uint8_t* v; int64_t k_rs, v_rs;
     const float* k_scale; const float* v_scale;
     const int* block_table; int64_t bt_stride;
-    int page_size, block, num_pages;
+    int page_size, page_log2, block_log2, num_pages;   // page_log2: -1 where the page is no power of two
     const int* cu_q; const int* cu_kv;
     const float* bias; int64_t bias_qs, bias_hs, bias_cols, bias_ss, bias_rows;
     int64_t total_q, total_kv;
     int num_seqs, hq, hkv, g, hpb, n_hg;
-    int hw;             // kv heads of a workgroup
+    int hw_log2;        // kv heads of a workgroup
     int pieces;         // pieces of the work (0: a sequence each)
-    int unit_keys;      // 32 * waves that share a head
+    int unit_log2;      // keys of a unit: 32 * waves that share a head
     int rpw;            // heads of a row that a workgroup of the combine takes
     float scale_log2;
     int causal, window, bias_v4;
     float* o_part; float* lse_part;     // [hkv][n_hg][pieces + num_seqs][16] rows
+    uint16_t* out; float* lse_out;
 };
+
+// The kernels read their parameters where they lie. A fresh pointer (params) keeps
+// the compiler from holding a loop's worth of them, and of what follows from them, in
+// registers: it spilled up to 86 scalars before the first load (32 sequences of up to
+// 16384 keys, window 2048, 16 heads, D = 64: 34.8 us, 31.7 without).
+typedef const __attribute__((address_space(4))) Dec8Params CParams;
+__device__ inline CParams* params() {
+    uint64_t a = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return (CParams*)a;
+}
 
 constexpr int kKT = 32;                 // keys per tile
 
@@ -69,18 +81,27 @@ __device__ inline const uint8_t* lane_pointer(uint64_t p, int l) {
 // sees (rounded down to a tile), and units of work, with their sum up to and with
 // each lane. Sequences without queries have no work.
 struct SeqGroup {
+    int k0, k1, q0, q1;                 // offsets, as they are read
     int len, q_start, q_len, lo, n, sum;
-    __device__ inline void load_one(const Dec8Params& p, int s) {
-        const SeqRange kr = seq_range(p.cu_kv, s, p.total_kv), qr = seq_range(p.cu_q, s, p.total_q);
-        len = kr.end - kr.start;
-        q_start = qr.start;
-        q_len = qr.end - qr.start;
-        lo = p.window > 0 ? max(0, len - q_len - p.window + 1) & ~(kKT - 1) : 0;
-        sum = n = q_len > 0 ? (len - lo + p.unit_keys - 1) / p.unit_keys : 0;
+    __device__ inline void fetch(CParams* p, int s) {
+        s = min(s, p->num_seqs - 1);
+        k0 = p->cu_kv[s];
+        k1 = p->cu_kv[s + 1];
+        q0 = p->cu_q[s];
+        q1 = p->cu_q[s + 1];
     }
-    __device__ inline void load(const Dec8Params& p, int g0, int lane) {
-        load_one(p, min(g0 + lane, p.num_seqs - 1));
-        if (g0 + lane >= p.num_seqs) n = 0;
+    __device__ inline void finish(CParams* p) {
+        const int tk = (int)p->total_kv, tq = (int)p->total_q;
+        k0 = min(max(k0, 0), tk);
+        q_start = min(max(q0, 0), tq);
+        len = min(max(k1, k0), tk) - k0;
+        q_len = min(max(q1, q_start), tq) - q_start;
+        lo = p->window > 0 ? max(0, len - q_len - p->window + 1) & ~(kKT - 1) : 0;
+        sum = n = q_len > 0 ? (len - lo + (1 << p->unit_log2) - 1) >> p->unit_log2 : 0;
+    }
+    __device__ inline void scan(CParams* p, int g0, int lane) {
+        finish(p);
+        if (g0 + lane >= p->num_seqs) n = 0;
         sum = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -88,18 +109,22 @@ struct SeqGroup {
             if (lane >= o) sum += y;
         }
     }
+    __device__ inline void load(CParams* p, int g0, int lane) {
+        fetch(p, g0 + lane);
+        scan(p, g0, lane);
+    }
     __device__ inline int total() const { return __builtin_amdgcn_readlane(sum, 63); }
 };
 
-// Units of a piece: all work in p.pieces equal ones. `grp` holds the first group.
-__device__ inline int piece_units(const Dec8Params& p, const SeqGroup& grp, int lane, int& work) {
+// Units of a piece: all work in p->pieces equal ones. `grp` holds the first group.
+__device__ inline int piece_units(CParams* p, const SeqGroup& grp, int lane, int& work) {
     work = grp.total();
-    for (int g0 = 64; g0 < p.num_seqs; g0 += 64) {
+    for (int g0 = 64; g0 < p->num_seqs; g0 += 64) {
         SeqGroup more;
         more.load(p, g0, lane);
         work += more.total();
     }
-    return max((work + p.pieces - 1) / p.pieces, 1);
+    return max((work + p->pieces - 1) / p->pieces, 1);
 }
 
 // Waits until at most N of this wave's vector memory operations are pending; LDS
@@ -154,8 +179,8 @@ struct Tile8 {
 
 template <typename T, typename C, int D, bool BIAS, int NW>
 // (D = 64, 8 waves: two workgroups on a CU)
-__global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_kernel(Dec8Params p, typename T::raw* __restrict__ out,
-                                                          float* __restrict__ lse_out) {
+__global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_kernel(Dec8Params) {
+    CParams* p = params();
     using Tile = Tile8<D>;
     constexpr int KB = 2, NC = D / 64, DB = D / 16;
     constexpr int TPV = 64 / KB;                     // tiles whose lookups are fetched at once
@@ -171,42 +196,20 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
     const int n16 = lane & 15, lg = lane >> 4;
 
     // 8 neighbouring pieces on the 8 XCDs, the heads of a piece one after the other on its own
-    const int hw = p.hw, TW = NW / hw, per = p.hkv / hw * p.n_hg;
-    const int oct = blockIdx.x / (8 * per), in_oct = blockIdx.x - oct * 8 * per;
-    const int piece = 8 * oct + (in_oct & 7), hgk = in_oct >> 3;
-    const int hk0 = hgk % (p.hkv / hw) * hw, hgi = hgk / (p.hkv / hw);
-    const int hk = hk0 + w % hw, tw = w / hw;        // this wave's head, and tiles tw, tw + TW, ..
+    const int piece = 8 * blockIdx.z + blockIdx.x;
+    if (piece >= (p->pieces > 0 ? p->pieces : p->num_seqs)) return;
+    SeqGroup grp;                                    // (offsets under way, lane constants meanwhile)
+    grp.fetch(p, p->pieces > 0 ? lane : piece);
+    const int hw_log2 = p->hw_log2, hw = 1 << hw_log2, TW = NW >> hw_log2, hkgs = p->hkv >> hw_log2;
+    const int hgi = p->n_hg == 1 ? 0 : blockIdx.y / hkgs;
+    const int hk = ((int)blockIdx.y - hgi * hkgs) * hw + (w & (hw - 1)), tw = w >> hw_log2;   // head; tiles tw, tw + TW, ..
 
-    // units [u, u_end) of the work, from sequence group g0 on (`before` units before it)
-    SeqGroup grp;
-    int g0 = 0, before = 0, u, u_end;
-    if (p.pieces > 0) {
-        if (piece >= p.pieces) return;
-        grp.load(p, 0, lane);
-        int work;
-        const int units = piece_units(p, grp, lane, work);
-        if ((int64_t)piece * units >= work) return;
-        u = piece * units;
-        u_end = min(work - u, units) + u;
-        while (before + grp.total() <= u && g0 + 64 < p.num_seqs) {
-            before += grp.total();
-            g0 += 64;
-            grp.load(p, g0, lane);
-        }
-    } else {
-        if (piece >= p.num_seqs) return;
-        g0 = piece;                                  // (every lane holds the sequence)
-        grp.load_one(p, g0);
-        u = 0;
-        u_end = max(1, grp.n);
-    }
-
-    const uint8_t* kbase = p.k + (int64_t)hk * D;
-    const uint8_t* vbase = p.v + (int64_t)hk * D;
-    const int bt_last = (int)min(p.bt_stride, (int64_t)0x7fffffff) - 1;
+    const uint8_t* kbase = p->k + (int64_t)hk * D;
+    const uint8_t* vbase = p->v + (int64_t)hk * D;
+    const int bt_last = (int)min(p->bt_stride, (int64_t)0x7fffffff) - 1;
     // direct loads: lane l fills chunk position l % (D / 16) of row l / (D / 16)
-    const uint32_t k_rs = (uint32_t)p.k_rs, v_rs = (uint32_t)p.v_rs;
-    const int64_t k_half = Tile::kLoadRows * p.k_rs, v_half = Tile::kLoadRows * p.v_rs;
+    const uint32_t k_rs = (uint32_t)p->k_rs, v_rs = (uint32_t)p->v_rs;
+    const int64_t k_half = Tile::kLoadRows * p->k_rs, v_half = Tile::kLoadRows * p->v_rs;
     const int lrow = lane / (D / 16), lpos = lane % (D / 16);
     uint32_t koff[Tile::kPerBlock], voff[KB];
 #pragma unroll
@@ -221,12 +224,34 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
     const int ve = (lane & 15) >> 1, vkey = ve < 4 ? 4 * lg + ve : 12 + 4 * lg + ve;
     const int vread = Tile::kV + vkey * D + 16 * Tile::swz_v(vkey) + 8 * (lane & 1);   // chunk 0; db is this ^ 16 db
 
+    // units [u, u_end) of the work, from sequence group g0 on (`before` units before it)
+    int g0 = 0, before = 0, u, u_end;
+    if (p->pieces > 0) {
+        grp.scan(p, 0, lane);
+        int work;
+        const int units = piece_units(p, grp, lane, work);
+        if ((int64_t)piece * units >= work) return;
+        u = piece * units;
+        u_end = min(work - u, units) + u;
+        while (before + grp.total() <= u && g0 + 64 < p->num_seqs) {
+            before += grp.total();
+            g0 += 64;
+            grp.load(p, g0, lane);
+        }
+    } else {
+        g0 = piece;                                  // (every lane holds the sequence)
+        grp.finish(p);
+        u = 0;
+        u_end = max(1, uniform(grp.n));
+    }
+
     while (u < u_end) {
+        p = params();
         // the sequence of unit u
         int l = 0;
-        if (p.pieces > 0) {
+        if (p->pieces > 0) {
             uint64_t past = __ballot(before + grp.sum > u);
-            while (past == 0 && g0 + 64 < p.num_seqs) {
+            while (past == 0 && g0 + 64 < p->num_seqs) {
                 before += grp.total();
                 g0 += 64;
                 grp.load(p, g0, lane);
@@ -238,41 +263,41 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         const int s = g0 + l, kv_len = __builtin_amdgcn_readlane(grp.len, l), n_units = __builtin_amdgcn_readlane(grp.n, l);
         const int q_len = __builtin_amdgcn_readlane(grp.q_len, l), q_start = __builtin_amdgcn_readlane(grp.q_start, l);
         const int lo = __builtin_amdgcn_readlane(grp.lo, l);
-        const int t0 = p.pieces > 0 ? before + __builtin_amdgcn_readlane(grp.sum, l) - n_units : 0;
-        const bool whole = p.pieces == 0 || (u == t0 && t0 + n_units <= u_end);
-        const int ks = lo + (u - t0) * p.unit_keys;
-        const int ke = min(kv_len, lo + min(n_units, u_end - t0) * p.unit_keys);
-        u = p.pieces > 0 ? t0 + n_units : u_end;
+        const int t0 = p->pieces > 0 ? before + __builtin_amdgcn_readlane(grp.sum, l) - n_units : 0;
+        const bool whole = p->pieces == 0 || (u == t0 && t0 + n_units <= u_end);
+        const int ks = lo + ((u - t0) << p->unit_log2);
+        const int ke = min(kv_len, lo + (min(n_units, u_end - t0) << p->unit_log2));
+        u = p->pieces > 0 ? t0 + n_units : u_end;
         if (q_len == 0) continue;
         const int coff = kv_len - q_len;
 
         // Row n of the 16 columns: head hh = n / q_len of this group, query n % q_len.
         // (columns past the rows repeat row 0; nothing reads them)
-        const int rows = min(p.hpb * q_len, 16);
+        const int rows = min(p->hpb * q_len, 16);
         const bool row_ok = n16 < rows;
-        const int hh = row_ok ? n16 / q_len : 0;
+        const int hh = row_ok ? (q_len == 1 ? n16 : n16 / q_len) : 0;
         const int qi = row_ok ? n16 - hh * q_len : 0;
-        const int head = hk * p.g + hgi * p.hpb + hh;
+        const int head = hk * p->g + hgi * p->hpb + hh;
         const int64_t grow = q_start + qi;
         // keys [first, first + width) are the row's
-        const int first = p.window > 0 ? max(ks, qi + coff - p.window + 1) : ks;
-        const uint32_t width = (uint32_t)max(0, (p.causal ? min(ke, qi + coff + 1) : ke) - first);
+        const int first = p->window > 0 ? max(ks, qi + coff - p->window + 1) : ks;
+        const uint32_t width = (uint32_t)max(0, (p->causal ? min(ke, qi + coff + 1) : ke) - first);
 
         // operand kc = 2 c + h: codes 64 c + 16 lg + 8 h .. + 7 of a row
         u32x4_t qf[2 * NC];
         {
-            const uint16_t* qp = p.q + grow * p.q_rs + (int64_t)head * D + 16 * lg;
+            const uint16_t* qp = p->q + grow * p->q_rs + (int64_t)head * D + 16 * lg;
 #pragma unroll
             for (int kc = 0; kc < 2 * NC; ++kc) qf[kc] = ld16(qp + 64 * (kc >> 1) + 8 * (kc & 1));
         }
         const float* brow = nullptr;
         if (BIAS)
-            brow = p.bias + bias_row_offset(grow, s, q_start, p.bias_qs, p.bias_ss, p.bias_rows) +
-                   (int64_t)head * p.bias_hs;
+            brow = p->bias + bias_row_offset(grow, s, q_start, p->bias_qs, p->bias_ss, p->bias_rows) +
+                   (int64_t)head * p->bias_hs;
 
         const int n_tiles = ke > ks ? (ke - ks + kKT - 1) / kKT : 0;
-        const int n_my = n_tiles > tw ? (n_tiles - tw + TW - 1) / TW : 0;
-        const int* bt = p.block_table + (int64_t)s * p.bt_stride;
+        const int n_my = n_tiles > tw ? (n_tiles - tw + TW - 1) >> (NW == 8 ? 3 - hw_log2 : 2 - hw_log2) : 0;
+        const int* bt = p->block_table + (int64_t)s * p->bt_stride;
 
         // Lookups of tiles [i0, i0 + TPV): lane l has block l % KB of tile i0 + l / KB
         // (blocks past the item's end: its last block). Addresses of the block's first
@@ -280,14 +305,16 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         uint64_t vkp = 0, vvp = 0;
         float vks = 0.f, vvs = 0.f;
         auto lookup_key = [&](int i0) { return min(ks + (tw + (i0 + lane / KB) * TW) * kKT + 16 * (lane % KB), ke - 1) & ~15; };
-        auto table_entry = [&](int i0) { return bt + min(lookup_key(i0) / p.page_size, bt_last); };
+        auto page_of = [&](int key) { return p->page_log2 >= 0 ? key >> p->page_log2 : key / p->page_size; };
+        auto table_entry = [&](int i0) { return bt + min(page_of(lookup_key(i0)), bt_last); };
         auto find_rows = [&](int i0, int page) {
-            const int row = min(max(page, 0), p.num_pages - 1) * p.page_size + lookup_key(i0) % p.page_size;
-            vkp = (uint64_t)(kbase + (int64_t)row * p.k_rs);
-            vvp = (uint64_t)(vbase + (int64_t)row * p.v_rs);
-            const int64_t sc = (int64_t)(row / p.block) * p.hkv + hk;
-            lds_dma4(p.k_scale + sc, look + 256);
-            lds_dma4(p.v_scale + sc, look + 512);
+            const int key = lookup_key(i0);
+            const int row = (min(max(page, 0), p->num_pages - 1) - page_of(key)) * p->page_size + key;
+            vkp = (uint64_t)(kbase + (int64_t)row * p->k_rs);
+            vvp = (uint64_t)(vbase + (int64_t)row * p->v_rs);
+            const int64_t sc = (int64_t)(row >> p->block_log2) * p->hkv + hk;
+            lds_dma4(p->k_scale + sc, look + 256);
+            lds_dma4(p->v_scale + sc, look + 512);
         };
         // starts the loads of tile i of this wave into buf
         auto load = [&](int i, char* buf) __attribute__((always_inline)) {
@@ -316,7 +343,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 }
                 // the lane's 4 keys of the block, where the tile lies within the columns
                 if (BIAS)
-                    lds_dma16(p.bias_v4 && kt + kKT <= p.bias_cols ? (const void*)(brow + kt + 16 * b + 4 * lg) : (const void*)kp,
+                    lds_dma16(p->bias_v4 && kt + kKT <= p->bias_cols ? (const void*)(brow + kt + 16 * b + 4 * lg) : (const void*)kp,
                               buf + Tile::kBytes + b * 1024);
             }
         };
@@ -362,11 +389,11 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 for (int r = 0; r < 4; ++r) sc[b][r] *= k_sc;
                 if (BIAS) {
                     f32x4_t bb = *reinterpret_cast<const f32x4_t*>(buf + Tile::kBytes + b * 1024 + 16 * lane);
-                    if (!(p.bias_v4 && kt + kKT <= p.bias_cols)) {
+                    if (!(p->bias_v4 && kt + kKT <= p->bias_cols)) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const int64_t key = kt + 16 * b + 4 * lg + r;
-                            bb[r] = key < p.bias_cols ? brow[key] : 0.f;
+                            bb[r] = key < p->bias_cols ? brow[key] : 0.f;
                         }
                     }
 #pragma unroll
@@ -374,7 +401,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 }
             }
             // (rows' window bands start at qi + coff - W + 1 <= coff + q_len - W)
-            if ((kt + kKT > ke) || (p.causal && kt + kKT - 1 > coff) || (p.window > 0 && kt < coff + q_len - p.window)) {
+            if ((kt + kKT > ke) || (p->causal && kt + kKT - 1 > coff) || (p->window > 0 && kt < coff + q_len - p->window)) {
 #pragma unroll
                 for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -422,15 +449,14 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         // the loop would wait for the direct loads too, which it does not count
         wait_vmcnt<0>();
         // Two tiles of LDS in turn: tile i is computed while tile i + 1 is in flight, then
-        // its place is loaded with tile i + 2. (Lookups between them are waited for early.
-        // One copy of each part: a workgroup's start is mostly instruction fetches.)
+        // its place is loaded with tile i + 2. (Lookups between them are waited for early.)
 #pragma clang loop unroll(disable)
         for (int i = -2; i < n_my; ++i) {
             char* buf = tiles + (i & 1) * TB;
             if (i >= 0) {
                 if (i + 1 < n_my) wait_loads<LOADS>(); else wait_loads<0>();
                 if (i % TPV == 0) {
-                    vks = *reinterpret_cast<const float*>(look + 256 + 4 * lane) * p.scale_log2;
+                    vks = *reinterpret_cast<const float*>(look + 256 + 4 * lane) * p->scale_log2;
                     vvs = *reinterpret_cast<const float*>(look + 512 + 4 * lane);
                 }
                 step(i, buf);
@@ -449,32 +475,33 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
             }
         }
 
+        p = params();
         const float lt = quad_sum(l_run);
         // where row n of this wave's head goes: the output, or a partial
         auto out_row = [&](int n) {
-            const int h2 = n / q_len;
-            return (int64_t)(q_start + n - h2 * q_len) * p.hq + hk * p.g + hgi * p.hpb + h2;
+            const int h2 = q_len == 1 ? n : n / q_len;
+            return (int64_t)(q_start + n - h2 * q_len) * p->hq + hk * p->g + hgi * p->hpb + h2;
         };
         auto part_row = [&](int n) {
-            return ((int64_t)(hk * p.n_hg + hgi) * (p.pieces + p.num_seqs) + s + piece) * 16 + n;
+            return ((int64_t)(hk * p->n_hg + hgi) * (p->pieces + p->num_seqs) + s + piece) * 16 + n;
         };
         auto put_lse = [&](int n, float m, float lsum) {
             const float lse = !(lsum <= 0.f) ? m * kLn2 + logf(lsum) : kNegInf;
-            if (!whole) p.lse_part[part_row(n)] = lse;
-            else if (lse_out != nullptr) lse_out[out_row(n)] = lse;
+            if (!whole) p->lse_part[part_row(n)] = lse;
+            else if (p->lse_out != nullptr) p->lse_out[out_row(n)] = lse;
         };
         if (TW == 1) {
             if (row_ok) {
                 const float inv = !(lt <= 0.f) ? 1.f / lt : 0.f;
                 if (whole) {
-                    typename T::raw* o = out + out_row(n16) * D + 4 * lg;
+                    uint16_t* o = p->out + out_row(n16) * D + 4 * lg;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) {
                         const f32x4_t x = oacc[db] * inv;
                         st8(o + 16 * db, u32x2_t{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])});
                     }
                 } else {
-                    float* o = p.o_part + part_row(n16) * D + 4 * lg;
+                    float* o = p->o_part + part_row(n16) * D + 4 * lg;
 #pragma unroll
                     for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(o + 16 * db) = oacc[db] * inv;
                 }
@@ -499,7 +526,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 f32x4_t ow[NW], o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < NW; ++i) {
-                    const int v = w % hw + (i < TW ? i : 0) * hw;
+                    const int v = (w & (hw - 1)) + (i < TW ? i : 0) * hw;
                     mw[i] = ml[v * 16 + n];
                     lw[i] = ml[(NW + v) * 16 + n];
                     ow[i] = *reinterpret_cast<const f32x4_t*>(smem + v * WB + n * OROW + d * 4);
@@ -516,47 +543,47 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                     }
                 }
                 o *= !(lsum <= 0.f) ? 1.f / lsum : 0.f;
-                if (whole) st8(out + out_row(n) * D + d, u32x2_t{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])});
-                else *reinterpret_cast<f32x4_t*>(p.o_part + part_row(n) * D + d) = o;
+                if (whole) st8(p->out + out_row(n) * D + d, u32x2_t{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])});
+                else *reinterpret_cast<f32x4_t*>(p->o_part + part_row(n) * D + d) = o;
                 if (d == 0) put_lse(n, m, lsum);
             }
             if (u < u_end) __syncthreads();
         }
         // rows past the 16 that max_seqlen_q promised: NaN (the combine's, of pieces)
-        if (p.pieces == 0) {
-            const int more = p.hpb * q_len - 16;
+        if (p->pieces == 0) {
+            const int more = p->hpb * q_len - 16;
             for (int64_t t = threadIdx.x; t < (int64_t)more * hw * D; t += NW * 64) {
                 const int64_t r = t / D;
                 const int hs = (int)(r % hw), n = 16 + (int)(r / hw), d = (int)(t % D), h2 = n / q_len;
-                const int64_t rh = (int64_t)(q_start + n - h2 * q_len) * p.hq + (hk0 + hs) * p.g + hgi * p.hpb + h2;
-                out[rh * D + d] = T::from_float(__builtin_nanf(""));
-                if (lse_out != nullptr && d == 0) lse_out[rh] = __builtin_nanf("");
+                const int64_t rh = (int64_t)(q_start + n - h2 * q_len) * p->hq + (hk - (w & (hw - 1)) + hs) * p->g + hgi * p->hpb + h2;
+                p->out[rh * D + d] = T::from_float(__builtin_nanf(""));
+                if (p->lse_out != nullptr && d == 0) p->lse_out[rh] = __builtin_nanf("");
             }
         }
     }
 }
 
 // Merges the partials of the pieces of a row's sequence with their LSEs: D / 4 lanes
-// to a partial, the 1024 / D such groups of a workgroup on p.rpw heads of one row,
+// to a partial, the 1024 / D such groups of a workgroup on p->rpw heads of one row,
 // the groups of a head taking its partials in turn with four loads of each in
 // flight. Many rows have few pieces each (one head to a group: 4096 rows of about 5
 // pieces 13 -> 8 us), few rows many (one wave that walked the 256 of a sequence of
 // 131071 keys took 30 us). Rows of a sequence inside one piece are there already;
 // rows of no sequence are left as they were.
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params p, typename T::raw* __restrict__ out,
-                                                       float* __restrict__ lse_out) {
+__global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params) {
+    CParams* p = params();
     constexpr int TPR = D / 4, G = NT / TPR, U = 4;
     __shared__ __attribute__((aligned(16))) float so[G][D];
     __shared__ float sm[G], sl[G];
-    const int tid = threadIdx.x, lane = tid & 63, split = G / p.rpw, per = p.hq / p.rpw;
-    const int row = blockIdx.x / per, head = (blockIdx.x - row * per) * p.rpw + tid / (TPR * split);
+    const int tid = threadIdx.x, lane = tid & 63, split = G / p->rpw, per = p->hq / p->rpw;
+    const int row = blockIdx.x / per, head = (blockIdx.x - row * per) * p->rpw + tid / (TPR * split);
     // the row's sequence, the units before it, and all work
     SeqGroup grp;
     int s = -1, q_len = 0, q_start = 0, n_units = 0, t0 = 0, work = 0;
-    for (int g0 = 0; g0 < p.num_seqs; g0 += 64) {
+    for (int g0 = 0; g0 < p->num_seqs; g0 += 64) {
         grp.load(p, g0, lane);
-        const uint64_t in = __ballot(g0 + lane < p.num_seqs && row >= grp.q_start && row < grp.q_start + grp.q_len);
+        const uint64_t in = __ballot(g0 + lane < p->num_seqs && row >= grp.q_start && row < grp.q_start + grp.q_len);
         if (in != 0) {
             const int l = __builtin_ctzll(in);
             s = g0 + l;
@@ -568,11 +595,11 @@ __global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params p, typename T::
         work += grp.total();
     }
     if (s < 0) return;
-    const int units = max((work + p.pieces - 1) / p.pieces, 1);
+    const int units = max((work + p->pieces - 1) / p->pieces, 1);
     const int first = t0 / units, count = n_units > 0 ? (t0 + n_units - 1) / units - first + 1 : 0;
-    const int qi = row - q_start, hk = head / p.g, hh_full = head - hk * p.g;
-    const int hgi = hh_full / p.hpb, n = (hh_full - hgi * p.hpb) * q_len + qi;
-    const int64_t base = ((int64_t)(hk * p.n_hg + hgi) * (p.pieces + p.num_seqs) + s + first) * 16 + n;
+    const int qi = row - q_start, hk = head / p->g, hh_full = head - hk * p->g;
+    const int hgi = hh_full / p->hpb, n = (hh_full - hgi * p->hpb) * q_len + qi;
+    const int64_t base = ((int64_t)(hk * p->n_hg + hgi) * (p->pieces + p->num_seqs) + s + first) * 16 + n;
     const int g = tid / TPR, d = 4 * (tid % TPR);
     float m = kNegInf, l = 0.f;
     f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -582,8 +609,8 @@ __global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params p, typename T::
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t at = base + (int64_t)min(i0 + u * split, count - 1) * 16;
-            li[u] = p.lse_part[at];
-            oi[u] = *reinterpret_cast<const f32x4_t*>(p.o_part + at * D + d);
+            li[u] = p->lse_part[at];
+            oi[u] = *reinterpret_cast<const f32x4_t*>(p->o_part + at * D + d);
         }
         float m_new = m;
 #pragma unroll
@@ -610,7 +637,7 @@ __global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params p, typename T::
     }
     __syncthreads();
     if (g % split != 0 || (count == 1 && n < 16)) return;
-    const int64_t rh = (int64_t)row * p.hq + head;
+    const int64_t rh = (int64_t)row * p->hq + head;
     float mt = kNegInf;
 #pragma unroll
     for (int i = 0; i < G; ++i) mt = i < split ? nan_max(sm[(g + i) % G], mt) : mt;
@@ -630,36 +657,35 @@ __global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params p, typename T::
         lse = __builtin_nanf("");
         o = f32x4_t{lse, lse, lse, lse};
     }
-    st8(out + rh * D + d, u32x2_t{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])});
-    if (lse_out != nullptr && d == 0) lse_out[rh] = lse;
+    st8(p->out + rh * D + d, u32x2_t{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])});
+    if (p->lse_out != nullptr && d == 0) p->lse_out[rh] = lse;
 }
 
 template <typename T, typename C, int D>
-hipError_t launch_typed(Dec8Params p, void* o, float* lse, hipStream_t st) {
+hipError_t launch_typed(Dec8Params p, hipStream_t st) {
     // the combine: groups of D / 4 lanes for a head's pieces (on average), eight each
     const int groups = 1024 / D;
     const bool many = p.pieces > 8 * groups * (int64_t)p.num_seqs;
     p.rpw = many ? 1 : groups;
     while (p.rpw > 1 && (p.hq % p.rpw != 0 || (int64_t)groups / p.rpw * 8 * p.num_seqs < p.pieces)) p.rpw /= 2;
-    typename T::raw* out = (typename T::raw*)o;
     const int64_t octs = ((p.pieces > 0 ? p.pieces : p.num_seqs) + 7) / 8;
-    const int64_t wgs = octs * 8 * (p.hkv / p.hw) * p.n_hg, rh = p.total_q * p.hq;
-    if (wgs > 0x7fffffff || rh > 0x7fffffff) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)wgs);
-    if (p.bias != nullptr) hipLaunchKernelGGL((decode8_kernel<T, C, D, true, 4>), grid, dim3(256), 0, st, p, out, lse);
-    else hipLaunchKernelGGL((decode8_kernel<T, C, D, false, 8>), grid, dim3(512), 0, st, p, out, lse);
+    const int64_t per = (int64_t)(p.hkv >> p.hw_log2) * p.n_hg, rh = p.total_q * p.hq;
+    if (octs > 65535 || per > 65535 || rh > 0x7fffffff) return hipErrorInvalidValue;
+    const dim3 grid(8, (unsigned)per, (unsigned)octs);
+    if (p.bias != nullptr) hipLaunchKernelGGL((decode8_kernel<T, C, D, true, 4>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((decode8_kernel<T, C, D, false, 8>), grid, dim3(512), 0, st, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.pieces == 0) return e;
     const dim3 cgrid((unsigned)(rh / p.rpw));
-    if (many) hipLaunchKernelGGL((combine8_kernel<T, D, 1024>), cgrid, dim3(1024), 0, st, p, out, lse);
-    else hipLaunchKernelGGL((combine8_kernel<T, D, 256>), cgrid, dim3(256), 0, st, p, out, lse);
+    if (many) hipLaunchKernelGGL((combine8_kernel<T, D, 1024>), cgrid, dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL((combine8_kernel<T, D, 256>), cgrid, dim3(256), 0, st, p);
     return hipGetLastError();
 }
 
 template <typename T, typename C>
-hipError_t launch_dim(const Dec8Params& p, int d, void* o, float* lse, hipStream_t st) {
-    if (d == 128) return launch_typed<T, C, 128>(p, o, lse, st);
-    if (d == 64) return launch_typed<T, C, 64>(p, o, lse, st);
+hipError_t launch_dim(const Dec8Params& p, int d, hipStream_t st) {
+    if (d == 128) return launch_typed<T, C, 128>(p, st);
+    if (d == 64) return launch_typed<T, C, 64>(p, st);
     return hipErrorInvalidValue;
 }
 
@@ -682,7 +708,7 @@ Dec8Plan make_dec8_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
         return hw;
     };
     const int64_t seq_heads = (int64_t)g.num_seqs * g.hkv * n_hg;
-    if (max_kv <= 1024 || (max_kv <= 2048 && seq_heads > 32)) {
+    if ((max_kv <= 1024 || (max_kv <= 2048 && seq_heads > 32)) && g.num_seqs <= 8 * 65535) {
         // One workgroup per sequence, no second launch; as many of its waves on a head as
         // the CUs have room for: a wave takes about 1 us per tile, which a bandwidth-bound
         // stream hides. bf16, D = 128, 32/8 heads, up to 1024 keys: 16 sequences 13.4 us
@@ -716,7 +742,9 @@ hipError_t launch_decode8(int dtype, int code, const Dec8Args& a, hipStream_t st
     p.k = a.k; p.v = a.v; p.k_rs = a.k_rs; p.v_rs = a.v_rs;
     p.k_scale = a.k_scale; p.v_scale = a.v_scale;
     p.block_table = a.block_table; p.bt_stride = a.bt_stride;
-    p.page_size = a.page_size; p.block = a.block; p.num_pages = a.num_pages;
+    p.page_size = a.page_size; p.num_pages = a.num_pages;
+    p.page_log2 = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctz(a.page_size) : -1;
+    p.block_log2 = __builtin_ctz(a.block);
     p.cu_q = g.cu_q; p.cu_kv = g.cu_kv;
     p.bias = g.bias; p.bias_qs = g.bias_qs; p.bias_hs = g.bias_hs; p.bias_cols = g.bias_cols;
     p.bias_ss = g.bias_ss; p.bias_rows = g.bias_rows;
@@ -724,9 +752,9 @@ hipError_t launch_decode8(int dtype, int code, const Dec8Args& a, hipStream_t st
     p.num_seqs = g.num_seqs; p.hq = g.hq; p.hkv = g.hkv; p.g = g.g;
     p.hpb = a.plan.hpb;
     p.n_hg = g.g / p.hpb;
-    p.hw = a.plan.hw;
+    p.hw_log2 = __builtin_ctz(a.plan.hw);
     p.pieces = a.plan.pieces;
-    p.unit_keys = kKT * (a.plan.waves / p.hw);
+    p.unit_log2 = __builtin_ctz(kKT * (a.plan.waves / a.plan.hw));
     p.scale_log2 = g.scale * kLog2e;
     p.causal = g.causal;
     p.window = g.window;
@@ -734,13 +762,15 @@ hipError_t launch_decode8(int dtype, int code, const Dec8Args& a, hipStream_t st
                 (g.bias_ss < 0 || g.bias_ss % 4 == 0);
     p.o_part = a.o_part;
     p.lse_part = a.lse_part;
+    p.out = (uint16_t*)a.o;
+    p.lse_out = a.lse;
     const bool e4m3 = code == MTLATTN_CODE_E4M3;
     if (dtype == MTLATTN_DTYPE_BF16)
-        return e4m3 ? launch_dim<BF16, E4M3>(p, g.d, a.o, a.lse, st)
-                    : launch_dim<BF16, I8>(p, g.d, a.o, a.lse, st);
+        return e4m3 ? launch_dim<BF16, E4M3>(p, g.d, st)
+                    : launch_dim<BF16, I8>(p, g.d, st);
     if (dtype == MTLATTN_DTYPE_F16)
-        return e4m3 ? launch_dim<F16, E4M3>(p, g.d, a.o, a.lse, st)
-                    : launch_dim<F16, I8>(p, g.d, a.o, a.lse, st);
+        return e4m3 ? launch_dim<F16, E4M3>(p, g.d, st)
+                    : launch_dim<F16, I8>(p, g.d, st);
     return hipErrorInvalidValue;
 }
 
