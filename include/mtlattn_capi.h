@@ -379,7 +379,7 @@ int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype,
 /*
  * Reads the last tokens of each sequence back: rows cu_seqlens[s] ..
  * cu_seqlens[s + 1] of k and v (contiguous [total, Hkv, D], 16-byte aligned, of
- * type dtype) are its last logical tokens, code * scale rounded once. With
+ * type dtype) are its last logical tokens, code * scale in fp32, rounded to it. With
  * cu_seqlens = cu_seqlens_kv: all of them. Table columns and pages are clamped
  * as in the attention; rows of no sequence and of negative positions are 0.
  */

@@ -250,7 +250,7 @@ def paged_cache_read(k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_seqlens_
     """Read the last tokens of each sequence back from a paged cache of 8-bit
     codes (no reference counterpart): (k, v), each [total, Hkv, D] in dtype
     (fp32/fp16/bf16), rows cu_seqlens[s]..cu_seqlens[s+1] being sequence s's
-    last logical tokens, code * scale rounded once. With cu_seqlens_kv for
+    last logical tokens, code * scale in fp32, rounded to dtype. With cu_seqlens_kv for
     both offsets these are all tokens: the packed K/V that varlen_attention
     takes, for prompts' chunks against the cache. total: the rows, at least
     cu_seqlens[-1] (rows past it are 0). Other arguments as for

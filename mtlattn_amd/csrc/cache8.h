@@ -16,9 +16,10 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 // exponent of 1024 and subtracting 1152, one instruction each per pair.
 struct E4M3 {
     static constexpr int code = 3;
-    static constexpr float kMax = 448.f;
     template <typename T>
     __device__ static inline u32x2_t unpack4(uint32_t w);
+    // 1 in each byte whose code is a NaN
+    __device__ static inline uint32_t nans(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u; }
     __device__ static inline void to_float4(uint32_t w, float* f) {
         const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
         f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
@@ -37,7 +38,6 @@ __device__ inline u32x2_t E4M3::unpack4<F16>(uint32_t w) {
 
 struct I8 {
     static constexpr int code = 4;
-    static constexpr float kMax = 127.f;
     template <typename T>
     __device__ static inline u32x2_t unpack4(uint32_t w);
     __device__ static inline void to_float4(uint32_t w, float* f) {
@@ -60,16 +60,6 @@ __device__ inline u32x2_t I8::unpack4<F16>(uint32_t w) {
     const f16x2_t a = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
     const f16x2_t b = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
     return u32x2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
-}
-
-// 4 x 4 bytes transposed: out[c] = {r0[c], r1[c], r2[c], r3[c]}.
-__device__ inline void transpose4x4b(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t out[4]) {
-    const uint32_t t0 = __builtin_amdgcn_perm(r1, r0, 0x05010400u), t1 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
-    const uint32_t u0 = __builtin_amdgcn_perm(r3, r2, 0x05010400u), u1 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
-    out[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100u);
-    out[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302u);
-    out[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100u);
-    out[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
 }
 
 }  // namespace mtlattn

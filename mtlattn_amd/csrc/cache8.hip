@@ -13,7 +13,8 @@
 // The powers of two cost a floating code nothing and make the recoding exact but
 // for the smallest values; an int8 code would lose up to a bit by them.
 //
-// Read. value = code * scale, rounded once to the output's type.
+// Read. value = code * scale in fp32, rounded to the output's type (an int8 code's
+// product takes up to 31 bits: two roundings where the scale is no power of two).
 //
 // Both are bound by HBM: 3 bytes per value for 16-bit rows.
 #include "cache8.h"
@@ -43,7 +44,7 @@ struct Cache8KParams {
 // Logical length of sequence s (the offsets are not bounded by a tensor).
 __device__ inline int kv_length(const int* __restrict__ cu_kv, int s) {
     const int64_t n = (int64_t)cu_kv[s + 1] - cu_kv[s];
-    return (int)min(max(n, (int64_t)0), (int64_t)0x7ffffff0);
+    return (int)min(max(n, (int64_t)0), (int64_t)0x7fff0000);      // (room for a block in an int)
 }
 
 // Eight values of a row, as they are stored, and as fp32.

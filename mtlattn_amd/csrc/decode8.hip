@@ -94,7 +94,7 @@ struct SeqGroup {
         const int tk = (int)p->total_kv, tq = (int)p->total_q;
         k0 = min(max(k0, 0), tk);
         q_start = min(max(q0, 0), tq);
-        len = min(max(k1, k0), tk) - k0;
+        len = min(min(max(k1, k0), tk) - k0, 0x7fff0000);    // (room for a few tiles in an int)
         q_len = min(max(q1, q_start), tq) - q_start;
         lo = p->window > 0 ? max(0, len - q_len - p->window + 1) & ~(kKT - 1) : 0;
         sum = n = q_len > 0 ? (len - lo + (1 << p->unit_log2) - 1) >> p->unit_log2 : 0;
@@ -407,6 +407,31 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         sc[b][r] = (uint32_t)(kt + 16 * b + 4 * lg + r - first) < width ? sc[b][r] : kNegInf;
+                // (0 * NaN: the keys before a window may lie in pages of another use by now)
+                if (C::code == E4M3::code) {
+                    uint32_t nan = 0;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) nan |= E4M3::nans(vc[db][0]) | E4M3::nans(vc[db][1]);
+                    if (__any(nan != 0)) {
+                        // Rows that see a NaN become one, by the count of those they see in each
+                        // column; the codes themselves become 0.
+                        u32x4_t see;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = kt + 16 * (e >> 1) + 4 * lg + 2 * (e & 1) - first;
+                            see[e] = ((uint32_t)key < width ? 0x3f80u : 0u) | ((uint32_t)key + 1 < width ? 0x3f800000u : 0u);
+                        }
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) {
+                            const uint32_t x = E4M3::nans(vc[db][0]), y = E4M3::nans(vc[db][1]);
+                            const u32x2_t a = E4M3::unpack4<BF16>(x * 0x38u), b = E4M3::unpack4<BF16>(y * 0x38u);
+                            const f32x4_t count = mfma16<BF16>(u32x4_t{a[0], a[1], b[0], b[1]}, see, f32x4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) oacc[db][r] = count[r] > 0.f ? __builtin_nanf("") : oacc[db][r];
+                            vc[db] &= ~u32x2_t{x * 0xffu, y * 0xffu};
+                        }
+                    }
+                }
             }
             float mx = kNegInf;
 #pragma unroll
@@ -430,7 +455,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 const int b = e >> 1, r = 2 * (e & 1);
                 const float e0 = __builtin_amdgcn_exp2f(sc[b][r] - m_use), e1 = __builtin_amdgcn_exp2f(sc[b][r + 1] - m_use);
                 l_run += e0 + e1;
-                const float p0 = e0 * vs[b], p1 = e1 * vs[b];
+                // (no weight, no value: the scale of a block that is masked may be anything)
+                const float p0 = e0 == 0.f ? 0.f : e0 * vs[b], p1 = e1 == 0.f ? 0.f : e1 * vs[b];
                 const uint32_t h = BF16::pack2(p0, p1);
                 hi[e] = h;
                 lw[e] = BF16::pack2(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));

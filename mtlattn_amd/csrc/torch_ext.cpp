@@ -535,8 +535,9 @@ at::Tensor paged_decode8(const at::Tensor& q, const at::Tensor& k_cache, const a
     if (q.size(0) == 0) return out;
     p.num_seqs = (int32_t)(cu_q.numel() - 1);
     p.total_q = q.size(0);
-    // (a bound on the logical KV total: sequences may share pages)
-    p.total_kv = std::min<int64_t>((int64_t)p.num_seqs * max_seqlen_kv, 0x7fffffff);
+    // What the tables hold bounds the logical KV total: a max_seqlen_kv that is too
+    // small (a captured graph's, of lengths that grew) shapes the launch, no more.
+    p.total_kv = std::min<int64_t>((int64_t)p.num_seqs * block_table.size(1), 0x7fffffff / page_size) * page_size;
     p.num_heads_q = (int32_t)q.size(1);
     p.num_heads_kv = (int32_t)Hkv;
     p.head_dim = (int32_t)D;

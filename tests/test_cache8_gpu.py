@@ -195,7 +195,7 @@ READS = [
 
 @pytest.mark.parametrize("kind,dt,hkv,d,page,block,rows,kv", READS)
 def test_read(mt, kind, dt, hkv, d, page, block, rows, kv):
-    """code * scale rounded once, bit for bit; rows past the last sequence 0."""
+    """code * scale in fp32, rounded to the type, bit for bit; rows past the last sequence 0."""
     g = torch.Generator().manual_seed(d + page)
     cache, table = _cache(kind, kv, page, hkv, d, block, g)
     cu = cu_of(kv if rows is None else rows)
@@ -307,6 +307,102 @@ def test_decode_nan_reaches_its_rows(mt):
                           table.cuda(), 1, 300, lse_out=lse, k_scale=cache[2].cuda(), v_scale=cache[3].cuda()).cpu()
     assert bool(torch.isnan(out[0, 4:]).all()) and bool(torch.isnan(lse[0, 4:]).all())
     assert bool(torch.isfinite(out[0, :4]).all()) and bool(torch.isfinite(out[1]).all())
+
+
+@pytest.mark.parametrize("kind,d,block,page,ql,kv,causal,window,max_kv", [
+    ("e4m3", 128, 16, 16, [1, 3, 4], [100, 203, 77], True, 40, 203),
+    ("e4m3", 64, 32, 96, [4, 1, 2], [333, 640, 65], True, 50, 640),
+    ("e4m3", 128, 16, 64, [2, 4, 4, 1], [2500, 4097, 2, 900], True, 70, 4097),
+    ("e4m3", 64, 16, 16, [3, 4], [2100, 61], True, 0, 2100),
+    ("int8", 128, 16, 32, [1, 4, 2], [500, 130, 2300], True, 33, 2300),
+    ("int8", 64, 64, 64, [1, 1], [700, 2900], False, 128, 2900),
+])
+def test_decode_masked_garbage(mt, kind, d, block, page, ql, kv, causal, window, max_kv):
+    """What a row does not see is not in its result, whatever lies there: NaN codes
+    and scales that are no numbers before a window (pages given to other uses), a
+    NaN in V at keys that only some rows see."""
+    gen = torch.Generator().manual_seed(23)
+    hkv, g = 2, 2
+    cache, table = _cache(kind, kv, page, hkv, d, block, gen)
+    q = torch.randn(sum(ql), hkv * g, d, generator=gen).to(BF16)
+    cu = [0]
+    for n in ql:
+        cu.append(cu[-1] + n)
+    ref, ref_lse, bound, lse_bound = decode_reference(q, cache[0], cache[2], cache[1], cache[3], cu, kv, table, d ** -0.5,
+                                                      causal, window)
+    want_nan = torch.zeros(ref.shape, dtype=torch.bool)
+    dirty = _clone(cache)
+    raw = [t.view(torch.uint8).flatten(0, 1) for t in dirty[:2]]
+    for s, n in enumerate(kv):
+        first = max(0, n - ql[s] - window + 1) if window else 0
+        at = cache8.rows(table, s, 0, n, page, cache[0].shape[0])
+        for r in raw:
+            r[at[:first]] = 0x7f if kind == "e4m3" else 0x80
+        for b in range(first // block):
+            row = int(at[b * block]) // block
+            dirty[2].flatten(0, 1)[row] = float("nan")
+            dirty[3].flatten(0, 1)[row] = math.inf if b % 2 else float("nan")
+        if kind == "e4m3":
+            # column 5 of the key before the last, column 9 of a key at the window's start
+            for key, col in ((n - 2, 5), (first + 1, 9)):
+                raw[1][at[key], 0, col] = 0xff
+                for i in range(ql[s]):
+                    pos = i + n - ql[s]
+                    if (not causal or key <= pos) and (not window or key > pos - window):
+                        want_nan[cu[s] + i, :g, col] = True
+    lse = torch.empty(q.shape[:2], device="cuda")
+    dev = _dev(dirty)
+    out = mt.paged_decode(q.cuda(), dev[0], dev[1], torch.tensor(cu, dtype=torch.int32).cuda(), cu_of(kv, "cuda"),
+                          table.cuda(), max(ql), max_kv, causal=causal, window=window, lse_out=lse, k_scale=dev[2],
+                          v_scale=dev[3]).cpu()
+    assert torch.equal(torch.isnan(out), want_nan)
+    check_decode(torch.where(want_nan, ref.to(out.dtype), out), lse, ref, ref_lse, bound, lse_bound, BF16)
+
+
+def test_decode_many_sequences(mt):
+    """Equal pieces of more sequences than one scan of them takes, some without
+    keys, queries or both, ragged over page ends."""
+    gen = torch.Generator().manual_seed(24)
+    kv = torch.randint(1, 700, (203,), generator=gen).tolist()
+    ql = torch.randint(1, 4, (203,), generator=gen).tolist()
+    for i in range(0, 203, 7):
+        kv[i] = 0
+    for i in range(3, 203, 11):
+        ql[i] = 0
+    kv[70:134] = [0] * 64
+    kv[150], kv[202] = 5000, 2600
+    cu = [0]
+    for n in ql:
+        cu.append(cu[-1] + n)
+    for kind, page, block, causal, window in (("e4m3", 48, 16, True, 0), ("int8", 64, 32, False, 300)):
+        cache, table = _cache(kind, kv, page, 2, 64, block, gen)
+        q = torch.randn(cu[-1], 4, 64, generator=gen).to(F16)
+        ref = decode_reference(q, cache[0], cache[2], cache[1], cache[3], cu, kv, table, 0.125, causal, window)
+        poison_free_rows(cache[0], kv, table)
+        poison_free_rows(cache[1], kv, table)
+        lse = torch.empty(q.shape[:2], device="cuda")
+        dev = _dev(cache)
+        out = mt.paged_decode(q.cuda(), dev[0], dev[1], torch.tensor(cu, dtype=torch.int32).cuda(), cu_of(kv, "cuda"),
+                              table.cuda(), 3, 5000, causal=causal, window=window, lse_out=lse, k_scale=dev[2], v_scale=dev[3])
+        check_decode(out, lse, *ref, F16)
+
+
+@pytest.mark.parametrize("kind,max_kv", [("e4m3", 60000), ("int8", 60000), ("e4m3", 1000)])
+def test_decode_long_waves(mt, kind, max_kv):
+    """More tiles to a wave than one fetch of lookups holds: many sequences over the
+    same pages; and a max_seqlen_kv that is too small costs time, no keys."""
+    gen = torch.Generator().manual_seed(25)
+    kv = [59999, 51200 - 7]
+    n = 64 if max_kv > 1000 else 2
+    cache, table = _cache(kind, kv, 256, 1, 64, 16, gen)
+    q = torch.randn(2 * n, 2, 64, generator=gen).to(BF16)
+    ref = decode_reference(q, cache[0], cache[2], cache[1], cache[3], [0, n, 2 * n], kv, table, 0.125)
+    lens = [kv[0]] * n + [kv[1]] * n
+    lse = torch.empty(q.shape[:2], device="cuda")
+    dev = _dev(cache)
+    out = mt.paged_decode(q.cuda(), dev[0], dev[1], torch.arange(2 * n + 1, dtype=torch.int32).cuda(), cu_of(lens, "cuda"),
+                          table.repeat_interleave(n, 0).cuda(), 1, max_kv, lse_out=lse, k_scale=dev[2], v_scale=dev[3])
+    check_decode(out, lse, *ref, BF16)
 
 
 def test_decode_too_small_max_seqlen_q(mt):
