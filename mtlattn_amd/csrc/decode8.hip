@@ -403,10 +403,16 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
             // (rows' window bands start at qi + coff - W + 1 <= coff + q_len - W)
             if ((kt + kKT > ke) || (p->causal && kt + kKT - 1 > coff) || (p->window > 0 && kt < coff + q_len - p->window)) {
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
+                for (int b = 0; b < KB; ++b) {
+                    bool sees = false;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        sc[b][r] = (uint32_t)(kt + 16 * b + 4 * lg + r - first) < width ? sc[b][r] : kNegInf;
+                    for (int r = 0; r < 4; ++r) {
+                        const bool in = (uint32_t)(kt + 16 * b + 4 * lg + r - first) < width;
+                        sees = sees || in;
+                        sc[b][r] = in ? sc[b][r] : kNegInf;
+                    }
+                    vs[b] = sees ? vs[b] : 0.f;
+                }
                 // (0 * NaN: the keys before a window may lie in pages of another use by now)
                 if (C::code == E4M3::code) {
                     uint32_t nan = 0;
@@ -455,8 +461,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 const int b = e >> 1, r = 2 * (e & 1);
                 const float e0 = __builtin_amdgcn_exp2f(sc[b][r] - m_use), e1 = __builtin_amdgcn_exp2f(sc[b][r + 1] - m_use);
                 l_run += e0 + e1;
-                // (no weight, no value: the scale of a block that is masked may be anything)
-                const float p0 = e0 == 0.f ? 0.f : e0 * vs[b], p1 = e1 == 0.f ? 0.f : e1 * vs[b];
+                const float p0 = e0 * vs[b], p1 = e1 * vs[b];
                 const uint32_t h = BF16::pack2(p0, p1);
                 hi[e] = h;
                 lw[e] = BF16::pack2(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
