@@ -360,9 +360,9 @@ typedef struct mtlattn_cache8 {
  * attention over the cache then takes for its queries and keys.
  * For each block and kv head that gets rows, with a = the largest magnitude
  * among their finite values (at least 2^-92): need = the smallest power of two
- * with a <= 448 need (e4m3), a / 127 (int8). A block that already holds tokens of
- * the sequence keeps a larger scale; a smaller one grows to `need`, and the
- * earlier tokens' codes are rounded to it. Codes are the nearest to value /
+ * with a <= 448 need (e4m3), a * fp32(1 / 127) (int8). A block that already
+ * holds tokens of the sequence keeps a larger scale; a smaller one grows to
+ * `need`, and the earlier tokens' codes are rounded to it. Codes are the nearest to value /
  * scale, ties to even; infinities take the largest code, NaN stays NaN in e4m3
  * and is 0 in int8. Nothing else of the cache changes.
  * Rows whose logical position is negative (more rows than tokens), or whose

@@ -233,8 +233,8 @@ def paged_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_s
     one scale for each block of 16, 32, 64, 128 or 256 tokens and kv head.
 
     A block's scale fits the largest finite magnitude of its rows: the
-    smallest power of two with magnitude <= 448 * scale (e4m3), magnitude /
-    127 (int8). Tokens appended to a block that holds earlier ones raise its
+    smallest power of two with magnitude <= 448 * scale (e4m3), magnitude *
+    fp32(1 / 127) (int8). Tokens appended to a block that holds earlier ones raise its
     scale where they need it, and the earlier codes are rounded to the new
     scale. Infinities take the largest code; NaN stays NaN in e4m3 and is 0
     in int8. Rows without a place (a table column or page that does not

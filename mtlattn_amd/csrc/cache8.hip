@@ -4,7 +4,8 @@
 // Write. Sequence s's new rows become its last logical tokens. A (block of
 // tokens, kv head) has one scale:
 //   a = max |x| over the block's new rows' finite values, at least 2^-92
-//   need = the smallest 2^k with a <= 448 2^k (e4m3), a / 127 (int8)
+//   need = the smallest 2^k with a <= 448 2^k (e4m3), a times the fp32 value of
+//          1 / 127 (int8), as torch divides by 127 on the GPU
 //   scale' = max(scale, need) if the block held earlier tokens of the sequence,
 //            else need
 //   code = nearest(x / scale'), +-448 or +-127 at most (an infinity too); NaN
@@ -109,7 +110,7 @@ __device__ inline void store8<F32>(float* p, const float* f) {
 template <typename C>
 __device__ inline float scale_for(float a) {
     a = fmaxf(a, 0x1p-92f);
-    if (C::code == I8::code) return a / 127.f;
+    if (C::code == I8::code) return a * (1.f / 127.f);
     // a = m 2^e with m in [0.5, 1); 448 = 0.875 * 2^9
     const uint32_t bits = __float_as_uint(a);
     const int e = (int)(bits >> 23) - 126;

@@ -29,7 +29,7 @@ def scale_for(amax, dtype):
     """fp32 scale of a block whose largest finite magnitude is amax."""
     amax = max(float(amax), 2.0 ** -92)
     if dtype == torch.int8:
-        return float(torch.tensor(amax / 127.0, dtype=torch.float64).float())
+        return float(torch.tensor(amax, dtype=torch.float32) * torch.tensor(1.0 / 127.0, dtype=torch.float32))
     k = math.ceil(math.log2(amax / 448.0))
     while 448.0 * 2.0 ** k < amax:
         k += 1
