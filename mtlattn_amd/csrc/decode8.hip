@@ -52,7 +52,8 @@ struct Dec8Params {
     int rpw;            // heads of a row that a workgroup of the combine takes
     float scale_log2;
     int causal, window, bias_v4;
-    float* o_part; float* lse_part;     // [hkv][n_hg][pieces + num_seqs][16] rows
+    float* o_part; float* lse_part;     // [hkv][n_hg][pieces][2][16] rows: of the sequence that an earlier
+                                        // piece began, of the one that begins in this piece and goes on
     uint16_t* out; float* lse_out;
 };
 
@@ -115,17 +116,30 @@ struct SeqGroup {
     }
     __device__ inline int total() const { return __builtin_amdgcn_readlane(sum, 63); }
 };
-
-// Units of a piece: all work in p->pieces equal ones. `grp` holds the first group.
-__device__ inline int piece_units(CParams* p, const SeqGroup& grp, int lane, int& work) {
-    work = grp.total();
-    for (int g0 = 64; g0 < p->num_seqs; g0 += 64) {
-        SeqGroup more;
-        more.load(p, g0, lane);
-        work += more.total();
-    }
-    return max((work + p->pieces - 1) / p->pieces, 1);
+__device__ inline int wave_sum(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return uniform(x);
 }
+
+// The units of all sequences after the first group, whose own are `work`. Four groups'
+// offsets are under way at once.
+__device__ inline int all_units(CParams* p, int work, int lane) {
+    int n = 0;
+    for (int g0 = 64; g0 < p->num_seqs; g0 += 256) {
+        SeqGroup more[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) more[i].fetch(p, g0 + 64 * i + lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            more[i].finish(p);
+            n += g0 + 64 * i + lane < p->num_seqs ? more[i].n : 0;
+        }
+    }
+    return work + (p->num_seqs > 64 ? wave_sum(n) : 0);
+}
+// Units of a piece: all work in p->pieces equal ones.
+__device__ inline int piece_units(CParams* p, int work) { return max((work + p->pieces - 1) / p->pieces, 1); }
 
 // Waits until at most N of this wave's vector memory operations are pending; LDS
 // reads stay behind it.
@@ -228,8 +242,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
     int g0 = 0, before = 0, u, u_end;
     if (p->pieces > 0) {
         grp.scan(p, 0, lane);
-        int work;
-        const int units = piece_units(p, grp, lane, work);
+        const int work = all_units(p, grp.total(), lane), units = piece_units(p, work);
         if ((int64_t)piece * units >= work) return;
         u = piece * units;
         u_end = min(work - u, units) + u;
@@ -264,7 +277,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         const int q_len = __builtin_amdgcn_readlane(grp.q_len, l), q_start = __builtin_amdgcn_readlane(grp.q_start, l);
         const int lo = __builtin_amdgcn_readlane(grp.lo, l);
         const int t0 = p->pieces > 0 ? before + __builtin_amdgcn_readlane(grp.sum, l) - n_units : 0;
-        const bool whole = p->pieces == 0 || (u == t0 && t0 + n_units <= u_end);
+        const bool begins = u == t0, whole = p->pieces == 0 || (begins && t0 + n_units <= u_end);
         const int ks = lo + ((u - t0) << p->unit_log2);
         const int ke = min(kv_len, lo + (min(n_units, u_end - t0) << p->unit_log2));
         u = p->pieces > 0 ? t0 + n_units : u_end;
@@ -514,7 +527,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
             return (int64_t)(q_start + n - h2 * q_len) * p->hq + hk * p->g + hgi * p->hpb + h2;
         };
         auto part_row = [&](int n) {
-            return ((int64_t)(hk * p->n_hg + hgi) * (p->pieces + p->num_seqs) + s + piece) * 16 + n;
+            return (((int64_t)(hk * p->n_hg + hgi) * p->pieces + piece) * 2 + (begins ? 1 : 0)) * 16 + n;
         };
         auto put_lse = [&](int n, float m, float lsum) {
             const float lse = !(lsum <= 0.f) ? m * kLn2 + logf(lsum) : kNegInf;
@@ -609,28 +622,45 @@ __global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params) {
     __shared__ float sm[G], sl[G];
     const int tid = threadIdx.x, lane = tid & 63, split = G / p->rpw, per = p->hq / p->rpw;
     const int row = blockIdx.x / per, head = (blockIdx.x - row * per) * p->rpw + tid / (TPR * split);
-    // the row's sequence, the units before it, and all work
-    SeqGroup grp;
+    // the row's sequence, the units before it, and all work (four groups of 64 sequences
+    // at once after the first: 1024 sequences of up to 4096 keys 830 -> 819 us)
     int s = -1, q_len = 0, q_start = 0, n_units = 0, t0 = 0, work = 0;
-    for (int g0 = 0; g0 < p->num_seqs; g0 += 64) {
-        grp.load(p, g0, lane);
-        const uint64_t in = __ballot(g0 + lane < p->num_seqs && row >= grp.q_start && row < grp.q_start + grp.q_len);
-        if (in != 0) {
-            const int l = __builtin_ctzll(in);
-            s = g0 + l;
-            q_len = __builtin_amdgcn_readlane(grp.q_len, l);
-            q_start = __builtin_amdgcn_readlane(grp.q_start, l);
-            n_units = __builtin_amdgcn_readlane(grp.n, l);
-            t0 = work + __builtin_amdgcn_readlane(grp.sum, l) - n_units;
+    auto take = [&](SeqGroup& grp, int at) __attribute__((always_inline)) {
+        grp.finish(p);
+        const int n = at < p->num_seqs ? grp.n : 0, behind = row - grp.q_start;
+        work += n;
+        t0 += behind >= grp.q_len ? n : 0;
+        if (at < p->num_seqs && behind >= 0 && behind < grp.q_len) {
+            s = at;
+            q_len = grp.q_len;
+            q_start = grp.q_start;
+            n_units = n;
         }
-        work += grp.total();
+    };
+    SeqGroup grp;
+    grp.fetch(p, lane);
+    take(grp, lane);
+    for (int g0 = 64; g0 < p->num_seqs; g0 += 256) {
+        SeqGroup more[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) more[i].fetch(p, g0 + 64 * i + lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) take(more[i], g0 + 64 * i + lane);
     }
-    if (s < 0) return;
-    const int units = max((work + p->pieces - 1) / p->pieces, 1);
+    const uint64_t in = __ballot(s >= 0);
+    if (in == 0) return;
+    const int own = __builtin_ctzll(in);
+    q_len = __builtin_amdgcn_readlane(q_len, own);
+    q_start = __builtin_amdgcn_readlane(q_start, own);
+    n_units = __builtin_amdgcn_readlane(n_units, own);
+    work = wave_sum(work);
+    t0 = wave_sum(t0);
+    const int units = piece_units(p, work);
     const int first = t0 / units, count = n_units > 0 ? (t0 + n_units - 1) / units - first + 1 : 0;
     const int qi = row - q_start, hk = head / p->g, hh_full = head - hk * p->g;
     const int hgi = hh_full / p->hpb, n = (hh_full - hgi * p->hpb) * q_len + qi;
-    const int64_t base = ((int64_t)(hk * p->n_hg + hgi) * (p->pieces + p->num_seqs) + s + first) * 16 + n;
+    // its partials: the second of `first`, then the first ones of the following pieces
+    const int64_t base = (((int64_t)(hk * p->n_hg + hgi) * p->pieces + first) * 2) * 16 + n;
     const int g = tid / TPR, d = 4 * (tid % TPR);
     float m = kNegInf, l = 0.f;
     f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -639,7 +669,8 @@ __global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params) {
         f32x4_t oi[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t at = base + (int64_t)min(i0 + u * split, count - 1) * 16;
+            const int i = min(i0 + u * split, count - 1);
+            const int64_t at = base + (int64_t)(i == 0 ? 1 : 2 * i) * 16;
             li[u] = p->lse_part[at];
             oi[u] = *reinterpret_cast<const f32x4_t*>(p->o_part + at * D + d);
         }
@@ -754,14 +785,14 @@ Dec8Plan make_dec8_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
         // Pieces for every workgroup that the CUs hold, of whole token rows (8 heads); few
         // tiles (under 4 a wave) on fewer heads and more waves each, with fewer partials: one
         // sequence of 2048 keys 13.3 us with 2 heads, 17.3 with 8.
-        const int64_t tiles = (int64_t)g.num_seqs * max_kv / kKT * g.hkv * n_hg;
-        plan.hw = heads(tiles < (int64_t)cus * 8 * 4 ? 2 : 8);
+        const double tiles = (double)g.num_seqs * (double)max_kv / kKT * g.hkv * n_hg;
+        plan.hw = heads(tiles < cus * 8 * 4 ? 2 : 8);
         const int resident = g.bias == nullptr ? (g.d == 64 ? 2 : 1) : (g.d == 64 ? 3 : 1);
         // (a multiple of 8 where there are as many: a piece's workgroups share an XCD)
         const int per = g.hkv / plan.hw * n_hg, slots = cus * resident;
         plan.pieces = slots / 8 >= per ? slots / 8 / per * 8 : std::max(1, slots / per);
     }
-    plan.rows = plan.pieces > 0 ? (int64_t)g.hkv * n_hg * (plan.pieces + g.num_seqs) * 16 : 0;
+    plan.rows = (int64_t)g.hkv * n_hg * plan.pieces * 2 * 16;
     return plan;
 }
 
