@@ -367,7 +367,8 @@ typedef struct mtlattn_cache8 {
  * and is 0 in int8. Nothing else of the cache changes.
  * Rows whose logical position is negative (more rows than tokens), or whose
  * table column or page does not exist, are not written. Blocks that get rows
- * must belong to one sequence each. No workspace; deterministic.
+ * must belong to one sequence each, and keys and values must not share memory.
+ * No workspace; deterministic.
  */
 int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype,
                          const void* k, int64_t k_row_stride,

@@ -1016,6 +1016,9 @@ int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype, const void* k, 
         return fail(MTLATTN_ERR_INVALID, "cache8_write: row strides must cover a row");
     if (!aligned16(k, k_row_stride, dtype) || !aligned16(v, v_row_stride, dtype) || !cache8_aligned(c, 8))
         return fail(MTLATTN_ERR_UNSUPPORTED, "cache8_write: k/v rows must be 16-byte aligned, cache rows 8-byte aligned");
+    const int64_t scales = c->num_pages * (c->page_size / c->block) * (int64_t)c->num_heads_kv;
+    if (c->k == c->v || (c->k_scale < c->v_scale + scales && c->v_scale < c->k_scale + scales))
+        return fail(MTLATTN_ERR_INVALID, "cache8_write: keys and values must not share codes or scales");
     Cache8Args a = cache8_args(c, total, num_seqs, cu_seqlens, cu_seqlens_kv);
     a.k = const_cast<void*>(k); a.v = const_cast<void*>(v);
     a.k_rs = k_row_stride; a.v_rs = v_row_stride;

@@ -98,6 +98,10 @@ def test_bad_calls_are_refused():
     assert write(cache(v_scale=FAKE + 2)) == uns
     assert decode(problem(), cache(k=FAKE + 8)) == uns
     assert decode(problem(), cache(k_row_stride=264)) == uns
+    # keys and values in the same memory: their blocks' waves would race
+    assert write(cache(v=FAKE)) == inv
+    assert write(cache(v=FAKE + (1 << 30))) == inv                       # (the scales)
+    assert write(cache(v=FAKE + (1 << 30), v_scale=FAKE + 16)) == inv
     # nothing to do is no error, whatever the row pointers
     assert write(cache(), total=0, k=None, v=None) == capi.OK
     assert read(cache(), total=0, k=None, v=None) == capi.OK
@@ -124,6 +128,9 @@ def test_decode_limits():
     assert need > 0
     assert decode(p, cache(), max_kv=30000, ws=FAKE, ws_bytes=need - 1) == capi.ERR_WORKSPACE
     assert decode(p, cache(), max_kv=30000, ws=None, ws_bytes=need) == capi.ERR_WORKSPACE
+    # (which does not grow with the batch)
+    p = problem(num_seqs=4096, total_q=4096, total_kv=4096 * 30000)
+    assert capi.lib().mtlattn_decode8_workspace_size(ctypes.byref(p), 30000) == need
     assert capi.lib().mtlattn_decode8_workspace_size(ctypes.byref(problem(head_dim=96)), 30000) == 0
 
 
