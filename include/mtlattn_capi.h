@@ -367,7 +367,7 @@ typedef struct mtlattn_cache8 {
  * and is 0 in int8. Nothing else of the cache changes.
  * Rows whose logical position is negative (more rows than tokens), or whose
  * table column or page does not exist, are not written. Blocks that get rows
- * must belong to one sequence each, and keys and values must not share memory.
+ * must stand once in the block tables, and keys and values must not share memory.
  * No workspace; deterministic.
  */
 int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype,
@@ -394,6 +394,9 @@ int mtlattn_cache8_read(const mtlattn_cache8* c, int32_t dtype,
  * mtlattn_paged_decode over an 8-bit cache: same computation, options and
  * limits (p->dtype is the type of q and out), on values code * scale. Query rows
  * past the 16 / (heads per group) that p->max_seqlen_q promised come back NaN.
+ * Rows of no sequence are left as they were. Keys that a row does not see do not
+ * reach it, NaN codes and scales included. max_seqlen_kv shapes the launch only;
+ * p->total_kv bounds the logical lengths.
  * Workspace: mtlattn_decode8_workspace_size(p, max_seqlen_kv) bytes.
  */
 size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv);

@@ -206,7 +206,8 @@ def paged_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_table, 
 
     With k_scale and v_scale the cache is one of 8-bit codes (see
     paged_cache_write): float8_e4m3fn or int8 for any q type, values code *
-    scale."""
+    scale. Keys that a row does not see do not reach it, NaN codes and scales
+    included."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if (k_scale is None) != (v_scale is None):
@@ -239,8 +240,8 @@ def paged_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_s
     scale. Infinities take the largest code; NaN stays NaN in e4m3 and is 0
     in int8. Rows without a place (a table column or page that does not
     exist, more rows than tokens) are not written, so a page of -1 drops its
-    rows. A block that gets rows must belong to one sequence: copy shared
-    pages first. D: a multiple of 8 in [16, 256]."""
+    rows. A page that gets rows must stand once in the block tables: copy
+    shared pages first. D: a multiple of 8 in [16, 256]."""
     _C.paged_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, cu_seqlens.int(), cu_seqlens_kv.int(),
                          block_table.int())
 

@@ -405,6 +405,91 @@ def test_decode_long_waves(mt, kind, max_kv):
     check_decode(out, lse, *ref, BF16)
 
 
+@pytest.mark.parametrize("d,kv,max_kv", [(128, [300, 41, 512], 512), (64, [300, 41, 512], 512),
+                                         (128, [3000, 41, 900], 3000), (64, [2600, 1, 33], 2600)])
+def test_c_entry_padded_batch(mt, d, kv, max_kv):
+    """The C entry on a padded batch: rows before the first and behind the last
+    sequence stay as they were, and a workspace of the size that the query says is
+    enough."""
+    from mtlattn_amd import capi
+    gen = torch.Generator().manual_seed(41)
+    cache, table = _cache("e4m3", kv, 64, 4, d, 32, gen)
+    dev, dtable = _dev(cache), table.cuda()
+    cu = torch.tensor([2, 3, 5, 6], dtype=torch.int32, device="cuda")
+    ck = cu_of(kv, "cuda")
+    q = torch.randn(9, 8, d, generator=gen).to(BF16).cuda()
+    want = mt.paged_decode(q, dev[0], dev[1], cu, ck, dtable, 2, max_kv, causal=True, k_scale=dev[2], v_scale=dev[3])
+    p = capi.problem_for(q, dev[0][0], cu, ck, 2, d ** -0.5, causal=True)
+    p.total_kv = sum(kv)
+    c = capi.Cache8(code=capi.CODE_E4M3, page_size=64, block=32, num_heads_kv=4, head_dim=d, num_pages=dev[0].shape[0],
+                    k=dev[0].data_ptr(), k_row_stride=4 * d, v=dev[1].data_ptr(), v_row_stride=4 * d,
+                    k_scale=dev[2].data_ptr(), v_scale=dev[3].data_ptr(), block_table=dtable.data_ptr(),
+                    block_table_stride=dtable.shape[1])
+    import ctypes
+    need = capi.lib().mtlattn_decode8_workspace_size(ctypes.byref(p), max_kv)
+    assert (need > 0) == (max_kv > 2048)
+    ws = torch.full((need + 256,), 0xa5, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((9, 8), 7.0, device="cuda")
+    capi.call("mtlattn_decode8", p, q.data_ptr(), 8 * d, c, max_kv, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need,
+              torch.cuda.current_stream().cuda_stream)
+    assert bool((ws[need:] == 0xa5).all())
+    assert torch.equal(out[2:6], want[2:6])
+    # (the first of two queries on one key sees none: -inf)
+    assert not bool(torch.isnan(lse[2:6]).any()) and bool((lse[2:6] != 7.0).all())
+    for t in (out, lse):
+        assert bool((t[:2] == 7.0).all()) and bool((t[6:] == 7.0).all())
+
+
+def test_two_streams_at_once(mt):
+    """Calls on two streams at the same time do not meet: each result is that of the
+    call alone, bit for bit."""
+    gen = torch.Generator().manual_seed(42)
+    work = []
+    for kind, kv in (("e4m3", [2500, 700, 3000, 64]), ("int8", [1000, 2900, 17])):
+        cache, table = _cache(kind, kv, 32, 8, 128, 32, gen)
+        q = torch.randn(len(kv), 16, 128, generator=gen).to(BF16).cuda()
+        dev = _dev(cache)
+        args = (q, dev[0], dev[1], cu_of([1] * len(kv), "cuda"), cu_of(kv, "cuda"), table.cuda(), 1, max(kv))
+        kw = dict(causal=True, k_scale=dev[2], v_scale=dev[3])
+        work.append((args, kw, mt.paged_decode(*args, **kw)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(8):
+        for i, (args, kw, _) in enumerate(work):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(mt.paged_decode(*args, **kw))
+    torch.cuda.synchronize()
+    for i, (_, _, want) in enumerate(work):
+        for out in got[i]:
+            assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kv,max_kv", [([100, 333], 333), ([2100, 70], 2100)])
+def test_decode_mask_by_sequence(mt, kv, max_kv):
+    """A 4-D bias, indexed by sequence and sequence-local row: the result of the same
+    bias row by row, bit for bit. Keys at -inf for every row of a sequence's head
+    leave the row empty."""
+    gen = torch.Generator().manual_seed(43)
+    cache, table = _cache("int8", kv, 16, 2, 64, 16, gen)
+    q = torch.randn(4, 4, 64, generator=gen).to(F16).cuda()
+    bias = torch.randn(2, 4, 2, max_kv, generator=gen)
+    bias[1, 2, 1] = -math.inf
+    rows = bias.permute(0, 2, 1, 3).reshape(4, 4, max_kv).contiguous()
+    dev = _dev(cache)
+    outs = []
+    for b in (bias, rows):
+        lse = torch.empty(4, 4, device="cuda")
+        out = mt.paged_decode(q, dev[0], dev[1], cu_of([2, 2], "cuda"), cu_of(kv, "cuda"), table.cuda(), 2, max_kv,
+                              attn_bias=b.cuda(), lse_out=lse, k_scale=dev[2], v_scale=dev[3])
+        outs.append((out, lse))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert bool((outs[0][0][3, 2] == 0).all()) and float(outs[0][1][3, 2]) == -math.inf
+    ref = decode_reference(q.cpu(), cache[0], cache[2], cache[1], cache[3], [0, 2, 4], kv, table, 0.125, False, 0, rows)
+    check_decode(outs[0][0], outs[0][1], *ref, F16)
+
+
 def test_decode_too_small_max_seqlen_q(mt):
     """Query rows past what max_seqlen_q promised are NaN, the others right --
     both where a workgroup takes whole sequences and where they are cut."""
