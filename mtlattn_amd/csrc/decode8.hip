@@ -773,18 +773,19 @@ Dec8Plan make_dec8_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
     if ((max_kv <= 1024 || (max_kv <= 2048 && seq_heads > 32)) && g.num_seqs <= 8 * 65535) {
         // One workgroup per sequence, no second launch; as many of its waves on a head as
         // the CUs have room for: a wave takes about 1 us per tile, which a bandwidth-bound
-        // stream hides. bf16, D = 128, 32/8 heads, up to 1024 keys: 16 sequences 13.4 us
-        // with 8 waves on a head, 17.2 with 4, 45 with 1; 64 27.7 / 24.2 / 44.9, 256 102 /
-        // 88 / 82. Pieces took 19.1, 29.1 and 98; of up to 2048 keys (16, 64, 256
-        // sequences) 22.7, 50.4 and 170 against 18.8, 48.9 and 155, of up to 4096 (64)
-        // 86 against 89.
+        // stream hides. bf16, D = 128, 32/8 heads, up to 1024 keys: 16 sequences 11.5 us
+        // with 8 waves on a head, 16.1 with 4, 42.6 with 1; 64 25.0 / 22.0 / 45.1, 256
+        // 81.9 / 66.9 / 63.3. Pieces took 16.3, 25.9 and 66.8; of up to 2048 keys (16, 64,
+        // 256 sequences) 18.5, 37.1 and 133.9 against 17.5, 34.0 and 131.3, of up to 4096
+        // (64) 62 against 68.
         int hw = 1;
         while (seq_heads > (int64_t)cus * hw && hw < plan.waves) hw *= 2;
         plan.hw = heads(hw);
     } else {
         // Pieces for every workgroup that the CUs hold, of whole token rows (8 heads); few
         // tiles (under 4 a wave) on fewer heads and more waves each, with fewer partials: one
-        // sequence of 2048 keys 13.3 us with 2 heads, 17.3 with 8.
+        // sequence of 2048 keys 12.0 us with 2 heads, 16.7 with 8, 16.4 as a whole; four of
+        // 4096 16.0 and 16.8.
         const double tiles = (double)g.num_seqs * (double)max_kv / kKT * g.hkv * n_hg;
         plan.hw = heads(tiles < cus * 8 * 4 ? 2 : 8);
         const int resident = g.bias == nullptr ? (g.d == 64 ? 2 : 1) : (g.d == 64 ? 3 : 1);
