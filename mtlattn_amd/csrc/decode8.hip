@@ -97,7 +97,8 @@ struct SeqGroup {
         q_start = min(max(q0, 0), tq);
         len = min(min(max(k1, k0), tk) - k0, 0x7fff0000);    // (room for a few tiles in an int)
         q_len = min(max(q1, q_start), tq) - q_start;
-        lo = p->window > 0 ? max(0, len - q_len - p->window + 1) & ~(kKT - 1) : 0;
+        // (64 bits: a window may be any positive int, and q_len longer than len)
+        lo = p->window > 0 ? (int)max((int64_t)len - q_len - p->window + 1, (int64_t)0) & ~(kKT - 1) : 0;
         sum = n = q_len > 0 ? (len - lo + (1 << p->unit_log2) - 1) >> p->unit_log2 : 0;
     }
     __device__ inline void scan(CParams* p, int g0, int lane) {
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         const int head = hk * p->g + hgi * p->hpb + hh;
         const int64_t grow = q_start + qi;
         // keys [first, first + width) are the row's
-        const int first = p->window > 0 ? max(ks, qi + coff - p->window + 1) : ks;
+        const int first = p->window > 0 ? (int)max((int64_t)qi + coff - p->window + 1, (int64_t)ks) : ks;
         const uint32_t width = (uint32_t)max(0, (p->causal ? min(ke, qi + coff + 1) : ke) - first);
 
         // operand kc = 2 c + h: codes 64 c + 16 lg + 8 h .. + 7 of a row

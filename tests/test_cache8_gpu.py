@@ -490,6 +490,22 @@ def test_decode_mask_by_sequence(mt, kv, max_kv):
     check_decode(outs[0][0], outs[0][1], *ref, F16)
 
 
+@pytest.mark.parametrize("kv", [[3, 700, 5, 0], [3, 2500, 5, 0]])
+def test_decode_largest_window(mt, kv):
+    """A window of any size that no key lies before, with sequences shorter than
+    their queries: the result without a window."""
+    gen = torch.Generator().manual_seed(44)
+    cache, table = _cache("e4m3", kv, 32, 2, 64, 32, gen)
+    ql = [4, 2, 4, 3]
+    q = torch.randn(sum(ql), 4, 64, generator=gen).to(BF16).cuda()
+    dev = _dev(cache)
+    outs = [mt.paged_decode(q, dev[0], dev[1], cu_of(ql, "cuda"), cu_of(kv, "cuda"), table.cuda(), 4, max(kv),
+                            causal=True, window=w, k_scale=dev[2], v_scale=dev[3]) for w in (0, 2**31 - 1, 2**40)]
+    check = decode_reference(q.cpu(), cache[0], cache[2], cache[1], cache[3], cu_of(ql).tolist(), kv, table, 0.125, True)
+    for out in outs:
+        check_decode(out, None, *check, BF16)
+
+
 def test_decode_too_small_max_seqlen_q(mt):
     """Query rows past what max_seqlen_q promised are NaN, the others right --
     both where a workgroup takes whole sequences and where they are cut."""
