@@ -11,9 +11,12 @@
 //     softmax weight, both uniform over 16 keys (a block is a multiple of 16
 //     tokens). The codes are converted exactly (cache8.h) to the query's type for
 //     Q K^T, to bf16 for P V.
-//   * P s_v, which spans fp32's range, goes into the P V product as the sum of two
-//     bf16 values (16 significant bits), so that the weights are not what limits an
-//     fp16 result.
+//   * P s_v, which spans fp32's range, goes into the P V product as the sum of three
+//     bf16 values: all 24 bits of it. (Two of them, 16 bits, left results of up to 2^-18 of
+//     sum P |v| off, which shows where weights next to each other cancel; the third costs
+//     0.7% of a long stream's time (64 sequences of 8192-65536 keys, 787 -> 792 us) and 4%
+//     of a short call's (16 of 128-2048, 18.4 -> 19.1). Up to 5 rows would have room for
+//     the parts as columns of one product: no faster, its branch costs what it saves.)
 //   * One wave takes one kv head, the waves of a workgroup neighbouring heads of
 //     the same tokens, so that whole token rows are read at about the same time
 //     (one head's 128 bytes of each row at a time stream at 5.0 TB/s, 8 heads' at
@@ -468,24 +471,31 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 for (int db = 0; db < DB; ++db) oacc[db] *= corr;
             }
             const float m_use = m_run == kNegInf ? 0.f : m_run;
-            // P^T operand, slots j < 4: key 4 lg + j, then 16 + 4 lg + j - 4
-            u32x4_t hi, lw;
+            // P^T operand, slots j < 4: key 4 lg + j, then 16 + 4 lg + j - 4, in three parts of 8
+            // bits each: the upper half of a float, of what it leaves (exact), and so on
+            float wt[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int b = e >> 1, r = 2 * (e & 1);
-                const float e0 = __builtin_amdgcn_exp2f(sc[b][r] - m_use), e1 = __builtin_amdgcn_exp2f(sc[b][r + 1] - m_use);
-                l_run += e0 + e1;
-                const float p0 = e0 * vs[b], p1 = e1 * vs[b];
-                const uint32_t h = BF16::pack2(p0, p1);
-                hi[e] = h;
-                lw[e] = BF16::pack2(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
+            for (int e = 0; e < 8; ++e) {
+                const float x = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - m_use);
+                l_run += x;
+                wt[e] = x * vs[e >> 2];
             }
+            u32x4_t pt[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = __float_as_uint(wt[2 * e]), y = __float_as_uint(wt[2 * e + 1]);
+                    pt[i][e] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                    wt[2 * e] -= __uint_as_float(x & 0xffff0000u);
+                    wt[2 * e + 1] -= __uint_as_float(y & 0xffff0000u);
+                }
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
                 const u32x2_t x = C::template unpack4<BF16>(vc[db][0]), y = C::template unpack4<BF16>(vc[db][1]);
                 const u32x4_t va = u32x4_t{x[0], x[1], y[0], y[1]};
-                oacc[db] = mfma16<BF16>(va, hi, oacc[db]);
-                oacc[db] = mfma16<BF16>(va, lw, oacc[db]);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) oacc[db] = mfma16<BF16>(va, pt[i], oacc[db]);
             }
         };
 
