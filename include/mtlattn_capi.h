@@ -394,9 +394,11 @@ int mtlattn_cache8_read(const mtlattn_cache8* c, int32_t dtype,
  * mtlattn_paged_decode over an 8-bit cache: same computation, options and
  * limits (p->dtype is the type of q and out), on values code * scale. Query rows
  * past the 16 / (heads per group) that p->max_seqlen_q promised come back NaN.
- * Rows of no sequence are left as they were. Keys that a row does not see do not
- * reach it, NaN codes and scales included. max_seqlen_kv shapes the launch only;
- * p->total_kv bounds the logical lengths.
+ * Rows of no sequence are left as they were. Keys that a row does not see (for
+ * their place, the causal mask or the window) do not reach it, whatever their codes
+ * and scales; those that it sees do as the definition says: an infinite v_scale makes
+ * infinities, or NaN where signs meet or a code or a weight is 0. max_seqlen_kv
+ * shapes the launch only; p->total_kv bounds the logical lengths.
  * Workspace: mtlattn_decode8_workspace_size(p, max_seqlen_kv) bytes.
  */
 size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv);

@@ -206,8 +206,8 @@ def paged_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_table, 
 
     With k_scale and v_scale the cache is one of 8-bit codes (see
     paged_cache_write): float8_e4m3fn or int8 for any q type, values code *
-    scale. Keys that a row does not see do not reach it, NaN codes and scales
-    included."""
+    scale. Keys that a row does not see do not reach it, whatever their codes
+    and scales."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if (k_scale is None) != (v_scale is None):

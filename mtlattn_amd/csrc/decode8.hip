@@ -321,6 +321,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         // row of this head from its page, and the scales, which arrive in LDS.
         uint64_t vkp = 0, vvp = 0;
         float vks = 0.f, vvs = 0.f;
+        bool inf_scale = false;                          // one of vvs is an infinity
         auto lookup_key = [&](int i0) { return min(ks + (tw + (i0 + lane / KB) * TW) * kKT + 16 * (lane % KB), ke - 1) & ~15; };
         auto page_of = [&](int key) { return p->page_log2 >= 0 ? key >> p->page_log2 : key / p->page_size; };
         auto table_entry = [&](int i0) { return bt + min(page_of(lookup_key(i0)), bt_last); };
@@ -490,6 +491,20 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                     wt[2 * e] -= __uint_as_float(x & 0xffff0000u);
                     wt[2 * e + 1] -= __uint_as_float(y & 0xffff0000u);
                 }
+            if (inf_scale) {
+                // (inf - inf: an infinity is its first part alone; inf * 0: keys that the row does
+                // not see are no terms)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t key = (uint32_t)(kt + 16 * (e >> 1) + 4 * lg + 2 * (e & 1) - first), h = pt[0][e];
+                    const uint32_t see = (key < width ? 0xffffu : 0u) | (key + 1 < width ? 0xffff0000u : 0u);
+                    const uint32_t fin = ((h & 0x7fffu) != 0x7f80u ? 0xffffu : 0u) |
+                                         ((h & 0x7fff0000u) != 0x7f800000u ? 0xffff0000u : 0u);
+                    pt[0][e] &= see;
+                    pt[1][e] &= see & fin;
+                    pt[2][e] &= see & fin;
+                }
+            }
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
                 const u32x2_t x = C::template unpack4<BF16>(vc[db][0]), y = C::template unpack4<BF16>(vc[db][1]);
@@ -513,6 +528,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 if (i % TPV == 0) {
                     vks = *reinterpret_cast<const float*>(look + 256 + 4 * lane) * p->scale_log2;
                     vvs = *reinterpret_cast<const float*>(look + 512 + 4 * lane);
+                    inf_scale = __any(fabsf(vvs) == kPosInf);
                 }
                 step(i, buf);
                 wait_lds();

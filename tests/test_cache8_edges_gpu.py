@@ -1,5 +1,5 @@
 """The 8-bit paged K/V cache on the GPU where its arithmetic and its index code
-are at their edges."""
+are at their edges: weights next to each other, scales of the caller's own."""
 
 import math
 
@@ -7,12 +7,12 @@ import pytest
 import torch
 
 from oracle import cache8
-from tests.cache8_helpers import CODES, check_decode, decode_reference, pages_for
+from tests.cache8_helpers import CODES, check_decode, decode_reference, pages_for, random_cache
 from tests.helpers import cu_of
 
 pytestmark = pytest.mark.gpu
 
-BF16, F16 = torch.bfloat16, torch.float16
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
 @pytest.fixture(scope="module")
@@ -26,6 +26,10 @@ def _offsets(lens, start=0):
     for n in lens:
         c.append(c[-1] + n)
     return c
+
+
+def _int32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
@@ -60,3 +64,84 @@ def test_decode_weights_in_32_bits(mt, kind, dt):
     size = cache8.values(vc, vs).view(pages, 16, hkv, d)[table[:, 0].long(), 0].abs().repeat_interleave(hq // hkv, 1)
     bound = (2.0 ** -20 + 2.0 ** -23.8 + 2.0 ** -24) * size
     check_decode(out, None, ref, ref_lse, bound, None, dt)
+
+
+def _by_definition(q, kc, ks, vc, vs, ql, kv, table, causal, window):
+    """fp64 attention, each row over the keys that it sees and no others (an
+    infinite value times the weight of a key that is not seen is no term)."""
+    page, pages = kc.shape[1], kc.shape[0]
+    k, v = cache8.values(kc, ks), cache8.values(vc, vs)
+    g = q.shape[1] // kc.shape[2]
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    row = 0
+    for s, n in enumerate(kv):
+        at = cache8.rows(table, s, 0, n, page, pages)
+        for i in range(ql[s]):
+            end = i + n - ql[s]
+            lo = max(0, end - window + 1) if window else 0
+            see = at[lo:end + 1 if causal else n]
+            for h in range(q.shape[1]):
+                p = torch.softmax((k[see, h // g] * q[row, h].double()).sum(-1) / math.sqrt(q.shape[2]), 0)
+                out[row, h] = (p[:, None] * v[see, h // g]).sum(0)
+            row += 1
+    return out
+
+
+@pytest.mark.parametrize("kind,dt,d,block,page,ql,kv,causal,window", [
+    ("e4m3", BF16, 128, 16, 16, [1, 4, 2], [100, 203, 31], True, 0),
+    ("e4m3", F16, 64, 32, 96, [4, 1, 3], [333, 640, 65], True, 50),
+    ("int8", BF16, 128, 16, 64, [2, 4, 1], [2500, 70, 900], True, 70),
+    ("int8", F16, 64, 64, 64, [1, 3], [700, 2900], False, 0),
+])
+def test_decode_infinite_value_scales(mt, kind, dt, d, block, page, ql, kv, causal, window):
+    """A caller's own value scale that is an infinity gives what the definition
+    gives, an infinity or, where signs meet or a code is 0, a NaN; also in a block
+    whose other keys the row does not see."""
+    gen = torch.Generator().manual_seed(53)
+    hkv, g = 2, 2
+    table, pages = pages_for(kv, page, gen)
+    kc, ks = random_cache(kind, pages, page, hkv, d, block, gen)
+    vc, vs = random_cache(kind, pages, page, hkv, d, block, gen)
+    ks *= 2.0 ** -4 if kind == "e4m3" else 2.0 ** -2             # (no weight of a seen key underflows)
+    # half of the columns have one sign, so that infinities stay
+    mag = vc.float().abs()
+    mag[..., ::2] = mag[..., ::2].clamp(min=1)
+    vc = torch.where(torch.arange(d) % 2 == 0, mag, vc.float()).to(vc.dtype)
+    flat = vs.flatten(0, 1)
+    for s, n in enumerate(kv):
+        if s == 1:                                              # (a sequence without)
+            continue
+        first = max(0, n - ql[s] - window + 1) if window else 0
+        # the last block, which the sequence fills in part, and the first that a row sees
+        for key, x in ((n - 1, math.inf), (first, -math.inf if s == 2 else math.inf)):
+            flat[int(cache8.rows(table, s, key, key + 1, page, pages)[0]) // block, 0] = x
+    q = torch.randn(sum(ql), hkv * g, d, generator=gen).to(dt)
+    cu = _offsets(ql)
+    ref = _by_definition(q, kc, ks, vc, vs, ql, kv, table, causal, window)
+    clean = torch.where(torch.isinf(vs), torch.ones_like(vs), vs)
+    _, _, bound, _ = decode_reference(q, kc, ks, vc, clean, cu, kv, table, d ** -0.5, causal, window)
+    assert all(int(f(ref).sum()) >= d for f in (torch.isinf, torch.isnan, torch.isfinite))
+    out = mt.paged_decode(q.cuda(), kc.cuda(), vc.cuda(), _int32(cu), cu_of(kv, "cuda"), table.cuda(), max(ql), max(kv),
+                          causal=causal, window=window, k_scale=ks.cuda(), v_scale=vs.cuda()).cpu()
+    assert torch.equal(torch.isnan(out), torch.isnan(ref))
+    inf = torch.isinf(ref)
+    assert torch.equal(out[inf].double(), ref[inf]) and not bool(torch.isinf(out[~inf]).any())
+    fin = torch.isfinite(ref)
+    check_decode(out[fin], None, ref[fin], None, bound[fin], None, dt)
+
+
+def test_decode_largest_value_scales(mt):
+    """Value scales up to the largest float beside small codes: a weight of 1 times
+    the scale is above bf16's largest value, the result is not."""
+    gen = torch.Generator().manual_seed(54)
+    kv, hkv, d = [1, 40], 2, 64
+    table, pages = pages_for(kv, 16, gen)
+    kc, ks = random_cache("e4m3", pages, 16, hkv, d, 16, gen)
+    vc = (torch.randint(-3, 4, (pages, 16, hkv, d), generator=gen) * 2.0 ** -9).to(torch.float8_e4m3fn)
+    vs = torch.full((pages, 1, hkv), torch.finfo(F32).max)
+    vs[::2] = -torch.finfo(F32).max
+    q = torch.randn(2, 4, d, generator=gen).to(BF16)
+    out = mt.paged_decode(q.cuda(), kc.cuda(), vc.cuda(), cu_of([1, 1], "cuda"), cu_of(kv, "cuda"), table.cuda(), 1, 40,
+                          k_scale=ks.cuda(), v_scale=vs.cuda())
+    ref, ref_lse, bound, _ = decode_reference(q, kc, ks, vc, vs, [0, 1, 2], kv, table, d ** -0.5)
+    check_decode(out, None, ref, ref_lse, bound, None, BF16)
