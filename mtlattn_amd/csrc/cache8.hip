@@ -117,6 +117,14 @@ __device__ inline float scale_for(float a) {
     return ldexpf(1.f, e - 9 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));
 }
 
+// y, rounded to fp32 from an exact value that r's sign says it is below (r > 0) or above,
+// as the odd one of the two floats next to that value: what is then rounded to fewer bits
+// is rounded as if from the exact value.
+__device__ inline float to_odd(float y, float r) {
+    const uint32_t b = __float_as_uint(y), more = (r > 0.f) == (b >> 31 == 0) ? 1u : ~0u;
+    return (r > 0.f || r < 0.f) && (b & 1u) == 0 ? __uint_as_float(b + more) : y;
+}
+
 // Four values as codes of this scale (pow2: the scale is a power of two; odd: there
 // may be values that are not finite or too large for the scale).
 template <typename C>
@@ -124,8 +132,19 @@ __device__ inline uint32_t encode4(const float* x, float scale, float inv, bool 
 template <>
 __device__ inline uint32_t encode4<E4M3>(const float* x, float scale, float inv, bool pow2, bool odd) {
     float y[4];
+    if (pow2) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = pow2 ? x[i] * inv : x[i] / scale;
+        for (int i = 0; i < 4; ++i) y[i] = x[i] * inv;
+    } else {
+        // A caller's own scale m 2^e: x 2^-e / m, whose remainder is exact in one FMA.
+        const int e = (int)(__float_as_uint(scale) >> 23) - 127;
+        const float m = __uint_as_float((__float_as_uint(scale) & 0x7fffffu) | 0x3f800000u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float v = ldexpf(x[i], -e), q = v / m;
+            y[i] = to_odd(q, fmaf(-q, m, v));
+        }
+    }
     if (odd) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -165,19 +184,25 @@ __device__ inline uint32_t encode4<I8>(const float* x, float scale, float inv, b
     return w;
 }
 
-// Four codes of `scale` as codes of the larger scale `now`. In 64 bits: the
+// Four codes of `scale` as codes of the larger scale `now`. For int8 in 64 bits: the
 // scales of 16-bit rows are ratios of small numbers, so that quotients lie next to
-// ties, closer than an fp32 rounding.
+// ties, closer than an fp32 rounding. For e4m3 `now`, which a block has grown to, is a
+// power of two: a code times the ratio of the scales, the product's error in one FMA.
 template <typename C>
-__device__ inline uint32_t recode4(uint32_t w, double scale, double now) {
+__device__ inline uint32_t recode4(uint32_t w, float scale, float now) {
     float f[4];
     C::to_float4(w, f);
+    if (C::code == E4M3::code) {
+        const float ratio = scale / now;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const double x = (double)f[i] * scale / now;
-        f[i] = (float)(C::code == I8::code ? __builtin_rint(x) : x);
+        for (int i = 0; i < 4; ++i) {
+            const float y = f[i] * ratio;
+            f[i] = to_odd(y, fmaf(f[i], ratio, -y));
+        }
+        return encode4<E4M3>(f, 1.f, 1.f, true, true);
     }
-    if (C::code == E4M3::code) return encode4<E4M3>(f, 1.f, 1.f, true, true);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = (float)__builtin_rint((double)f[i] * scale / now);
     return encode4<I8>(f, 1.f, 1.f, true, true);
 }
 

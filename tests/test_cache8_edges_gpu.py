@@ -1,5 +1,6 @@
 """The 8-bit paged K/V cache on the GPU where its arithmetic and its index code
-are at their edges: weights next to each other, scales of the caller's own."""
+are at their edges: weights next to each other, quotients next to ties, scales of
+the caller's own."""
 
 import math
 
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 from oracle import cache8
-from tests.cache8_helpers import CODES, check_decode, decode_reference, pages_for, random_cache
+from tests.cache8_helpers import CODES, check_decode, decode_reference, pages_for, random_cache, same_codes
 from tests.helpers import cu_of
 
 pytestmark = pytest.mark.gpu
@@ -19,6 +20,10 @@ BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 def mt():
     import mtlattn
     return mtlattn
+
+
+def _dev(ts):
+    return [t.cuda() for t in ts]
 
 
 def _offsets(lens, start=0):
@@ -145,3 +150,66 @@ def test_decode_largest_value_scales(mt):
                           k_scale=ks.cuda(), v_scale=vs.cuda())
     ref, ref_lse, bound, _ = decode_reference(q, kc, ks, vc, vs, [0, 1, 2], kv, table, d ** -0.5)
     check_decode(out, None, ref, ref_lse, bound, None, BF16)
+
+
+def _next_to(x, gen):
+    """fp32 values at x (fp64, exact), rounded, and up to one step to either side."""
+    y = x.float()
+    step = torch.randint(-1, 2, y.shape, generator=gen, dtype=torch.int32)
+    return (y.view(torch.int32) + step).view(F32)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_write_next_to_ties_of_held_scales(mt, kind, dt):
+    """Tokens into blocks that hold earlier ones at scales of the caller's own, any
+    fp32 value: quotients less than an fp32 rounding from a tie, for new codes where
+    the held scale stays and for the held ones where it grows."""
+    g = torch.Generator().manual_seed(57)
+    n, hkv, d, block = 24, 4, 64, 16
+    kv, new = [16] * n, [8] * n
+    table, pages = pages_for(kv, block, g)
+    cache = []
+    top = cache8.QMAX[CODES[kind]]
+    for _ in range(2):
+        codes, _ = random_cache(kind, pages, block, hkv, d, block, g)
+        # scales m 2^e: e4m3 keeps those with 448 2^e above the rows' magnitudes and lets
+        # the others grow, int8 compares them with the largest magnitude / 127
+        m = _next_to(1.0 + torch.rand(pages, 1, hkv, generator=g, dtype=torch.float64), g)
+        # ratios of a tie to a code: recoded, that code lies next to the tie
+        tie = torch.randint(8, 16, m.shape, generator=g).double() + 0.5
+        code = torch.randint(8, 16, m.shape, generator=g).double()
+        r = tie / code
+        r = torch.where(r < 1, 2 * r, r)
+        m[::2] = _next_to(r, g)[::2]
+        scale = torch.ldexp(m, torch.randint(-8, 3, m.shape, generator=g))
+        if kind == "e4m3":
+            codes = torch.where(torch.rand(codes.shape, generator=g) < 0.5, codes.float(),
+                                torch.ldexp(code.unsqueeze(-1).float(), torch.randint(-6, 5, codes.shape, generator=g)))
+            codes = codes.to(CODES[kind])
+        cache += [codes, scale]
+    cache = [cache[0], cache[2], cache[1], cache[3]]
+    rows = []
+    for x in (2, 3):
+        sc = cache[x][table[:, 0].long(), 0].double()[:, None, :, None]       # [n, 1, hkv, 1]
+        if kind == "e4m3":
+            t = (torch.randint(8, 16, (n, 8, hkv, d), generator=g).double() + 0.5)
+            t = torch.ldexp(t, torch.randint(-9, 5, t.shape, generator=g))
+        else:
+            t = torch.randint(0, 127, (n, 8, hkv, d), generator=g).double() + 0.5
+        t *= torch.randint(0, 2, t.shape, generator=g) * 2 - 1
+        t = t.clamp(-top, top)
+        # sequences with every third head's magnitudes above what the scale holds
+        t[::2, 0, ::3, 0] = top * 1.7
+        x = t * sc
+        rows.append((_next_to(x, g) if dt == F32 else x.to(dt)).reshape(8 * n, hkv, d))
+    dev = _dev(cache)
+    before = [c.clone() for c in cache[2:]]
+    mt.paged_cache_write(rows[0].cuda(), rows[1].cuda(), *dev, cu_of(new, "cuda"), cu_of(kv, "cuda"), table.cuda())
+    for x in (0, 1):
+        cache8.write(cache[x], cache[2 + x], rows[x], _offsets(new), kv, table)
+        used = table[:, 0].long()
+        grew = cache[2 + x][used] > before[x][used]
+        assert bool(grew.any()) and not bool(grew.all())
+        assert torch.equal(dev[2 + x].cpu(), cache[2 + x])
+        assert same_codes(dev[x], cache[x]), int((dev[x].cpu().view(torch.uint8) != cache[x].view(torch.uint8)).sum())
