@@ -367,7 +367,9 @@ typedef struct mtlattn_cache8 {
  * and is 0 in int8. Nothing else of the cache changes.
  * Rows whose logical position is negative (more rows than tokens), or whose
  * table column or page does not exist, are not written. Blocks that get rows
- * must stand once in the block tables, and keys and values must not share memory.
+ * must stand once in the block tables. Codes and scales must share memory neither
+ * with each other nor with the rows (K and V side by side in the token rows of one
+ * buffer, at the same stride, do not); such calls are refused.
  * No workspace; deterministic.
  */
 int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype,

@@ -241,7 +241,9 @@ def paged_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_s
     in int8. Rows without a place (a table column or page that does not
     exist, more rows than tokens) are not written, so a page of -1 drops its
     rows. A page that gets rows must stand once in the block tables: copy
-    shared pages first. D: a multiple of 8 in [16, 256]."""
+    shared pages first. Caches, scales and k / v must not share memory (caches
+    that are slices of one tensor's token rows do not). D: a multiple of 8 in
+    [16, 256]."""
     _C.paged_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, cu_seqlens.int(), cu_seqlens_kv.int(),
                          block_table.int())
 

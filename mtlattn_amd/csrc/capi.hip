@@ -373,6 +373,28 @@ bool cache8_aligned(const mtlattn_cache8* c, int64_t to) {
            (uintptr_t)c->k_scale % 4 == 0 && (uintptr_t)c->v_scale % 4 == 0;
 }
 
+// `n` rows of `bytes` bytes, `stride` bytes apart.
+struct Rows {
+    int64_t at, stride, bytes, n;
+    int64_t end() const { return at + (n - 1) * stride + bytes; }
+};
+
+// Whether two sets of rows share a byte: rows side by side, at the same stride, and one
+// row in the gaps of others do not; of other rows whose spans overlap it is not asked.
+bool share_memory(const Rows& a, const Rows& b) {
+    if (a.end() <= b.at || b.end() <= a.at) return false;
+    if (a.n == 1 || b.n == 1) {
+        const Rows &one = a.n == 1 ? a : b, &rows = a.n == 1 ? b : a;
+        // the first of the rows that ends behind the start of the one
+        const int64_t behind = one.at - rows.at - rows.bytes;
+        const int64_t i = behind < 0 ? 0 : behind / rows.stride + 1;
+        return i < rows.n && rows.at + i * rows.stride < one.end();
+    }
+    if (a.stride != b.stride) return true;
+    const int64_t off = ((b.at - a.at) % a.stride + a.stride) % a.stride;
+    return off < a.bytes || off + b.bytes > a.stride;
+}
+
 // The rows of a write or a read (pointers apart).
 int check_cache8_rows(int32_t dtype, int64_t total, int32_t num_seqs, const int32_t* cu, const int32_t* cu_kv,
                       const char* what) {
@@ -1016,9 +1038,16 @@ int mtlattn_cache8_write(const mtlattn_cache8* c, int32_t dtype, const void* k, 
         return fail(MTLATTN_ERR_INVALID, "cache8_write: row strides must cover a row");
     if (!aligned16(k, k_row_stride, dtype) || !aligned16(v, v_row_stride, dtype) || !cache8_aligned(c, 8))
         return fail(MTLATTN_ERR_UNSUPPORTED, "cache8_write: k/v rows must be 16-byte aligned, cache rows 8-byte aligned");
-    const int64_t scales = c->num_pages * (c->page_size / c->block) * (int64_t)c->num_heads_kv;
-    if (c->k == c->v || (c->k_scale < c->v_scale + scales && c->v_scale < c->k_scale + scales))
-        return fail(MTLATTN_ERR_INVALID, "cache8_write: keys and values must not share codes or scales");
+    // what a workgroup writes, another one must neither write nor read
+    const int64_t tokens = c->num_pages * c->page_size, es = dtype == MTLATTN_DTYPE_F32 ? 4 : 2;
+    const int64_t scales = tokens / c->block * c->num_heads_kv * (int64_t)sizeof(float);
+    const Rows mem[6] = {{(int64_t)c->k, c->k_row_stride, row, tokens}, {(int64_t)c->v, c->v_row_stride, row, tokens},
+                         {(int64_t)c->k_scale, scales, scales, 1},      {(int64_t)c->v_scale, scales, scales, 1},
+                         {(int64_t)k, k_row_stride * es, row * es, total}, {(int64_t)v, v_row_stride * es, row * es, total}};
+    for (int i = 0; i < 4; ++i)
+        for (int j = i + 1; j < 6; ++j)
+            if (share_memory(mem[i], mem[j]))
+                return fail(MTLATTN_ERR_INVALID, "cache8_write: codes, scales and the rows to write must not share memory");
     Cache8Args a = cache8_args(c, total, num_seqs, cu_seqlens, cu_seqlens_kv);
     a.k = const_cast<void*>(k); a.v = const_cast<void*>(v);
     a.k_rs = k_row_stride; a.v_rs = v_row_stride;
