@@ -411,6 +411,15 @@ int mtlattn_decode8(const mtlattn_problem* p,
                     void* workspace, size_t workspace_bytes,
                     void* stream);
 
+/*
+ * How mtlattn_decode8 would lay out `p` on the current device (256 CUs are assumed
+ * without one): `waves` per workgroup, which take `heads` kv heads, waves / heads of
+ * them each; the work in `pieces` pieces with partial results (0: a workgroup takes
+ * whole sequences).
+ */
+int mtlattn_decode8_layout(const mtlattn_problem* p, int64_t max_seqlen_kv,
+                           int32_t* waves, int32_t* heads, int32_t* pieces);
+
 /* Number of split-KV work-item slots per (kv head, head group) the forward's
  * decode routing would use for `p` (0 = the call is not routed to split-KV).
  * The automatic path cuts each sequence's KV into fixed-length chunks (about

@@ -57,6 +57,7 @@ class MtlattnError(RuntimeError):
 
 _P, _C8 = ctypes.POINTER(Problem), ctypes.POINTER(Cache8)
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
+_i32p = ctypes.POINTER(ctypes.c_int32)
 
 # name -> (restype, argtypes); checked against the header by the CPU tests
 SIGNATURES = {
@@ -86,6 +87,7 @@ SIGNATURES = {
     "mtlattn_cache8_write": (ctypes.c_int, [_C8, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "mtlattn_cache8_read": (ctypes.c_int, [_C8, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp]),
     "mtlattn_decode8_workspace_size": (_sz, [_P, _i64]),
+    "mtlattn_decode8_layout": (ctypes.c_int, [_P, _i64, _i32p, _i32p, _i32p]),
     "mtlattn_decode8": (ctypes.c_int, [_P, _vp, _i64, _C8, _i64, _vp, _vp, _vp, _sz, _vp]),
     "mtlattn_pack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "mtlattn_unpack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64,

@@ -1074,6 +1074,22 @@ size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seql
     return plan8_bytes(p, plan8(p, max_seqlen_kv));
 }
 
+int mtlattn_decode8_layout(const mtlattn_problem* p, int64_t max_seqlen_kv, int32_t* waves, int32_t* heads,
+                           int32_t* pieces) {
+    const int rc = check_problem(p);
+    if (rc != MTLATTN_OK) return rc;
+    if (!splitkv_supported(p))
+        return fail(MTLATTN_ERR_UNSUPPORTED, "decode8: half/bf16, D in {64,128}, max_seqlen_q in [1, 16]");
+    if (max_seqlen_kv < 0) return fail(MTLATTN_ERR_INVALID, "decode8: negative max_seqlen_kv");
+    if (waves == nullptr || heads == nullptr || pieces == nullptr)
+        return fail(MTLATTN_ERR_INVALID, "decode8_layout: null output pointer");
+    const Dec8Plan plan = plan8(p, max_seqlen_kv);
+    *waves = plan.waves;
+    *heads = plan.hw;
+    *pieces = plan.pieces;
+    return ok();
+}
+
 int mtlattn_decode8(const mtlattn_problem* p, const void* q, int64_t q_row_stride, const mtlattn_cache8* c,
                     int64_t max_seqlen_kv, void* out, float* lse, void* workspace, size_t workspace_bytes,
                     void* stream) {
