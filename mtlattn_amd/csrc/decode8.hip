@@ -683,7 +683,10 @@ __global__ __launch_bounds__(NT) void combine8_kernel(Dec8Params) {
     work = wave_sum(work);
     t0 = wave_sum(t0);
     const int units = piece_units(p, work);
-    const int first = t0 / units, count = n_units > 0 ? (t0 + n_units - 1) / units - first + 1 : 0;
+    // (offsets that overlap may make more units than an int holds, here or in the decode:
+    // whatever the sums, no partial but the workspace's)
+    const int first = min(max(t0 / units, 0), p->pieces - 1);
+    const int count = n_units > 0 ? min((t0 + n_units - 1) / units - first + 1, p->pieces - first) : 0;
     const int qi = row - q_start, hk = head / p->g, hh_full = head - hk * p->g;
     const int hgi = hh_full / p->hpb, n = (hh_full - hgi * p->hpb) * q_len + qi;
     // its partials: the second of `first`, then the first ones of the following pieces

@@ -1,11 +1,13 @@
 """Decode over the 8-bit K/V cache in every layout of its work, against the fp64
 oracle; writing and reading for batches of more sequences than a wave has lanes."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
+from mtlattn_amd import capi
 from oracle import cache8
 from tests import cache8_layouts
 from tests.cache8_helpers import check_decode, decode_reference, pages_for, poison_free_rows, random_cache, same_codes
@@ -109,3 +111,47 @@ def test_write_and_read_many_sequences(mt, n, kind, dt):
         for x in (0, 1):
             want = cache8.read(cache[x], cache[2 + x], at, kv, table, total).float().to(dt)
             assert torch.equal(got[x].cpu(), want)
+
+
+def test_malformed_offsets_stay_in_the_workspace(mt):
+    """KV offsets that go up and down claim more keys in all than an int counts (a
+    multiple of 2^32 less 2^17 units of 32): the call ends, writes nothing but its
+    rows, and calls after it are right."""
+    n, hq, hkv, d, page = 128, 8, 8, 64, 256
+    g = torch.Generator().manual_seed(61)
+    kv = [700, 40]
+    table, pages = pages_for(kv, page, g)
+    kc, ks = random_cache("int8", pages, page, hkv, d, 64, g)
+    vc, vs = random_cache("int8", pages, page, hkv, d, 64, g)
+    dev = [t.cuda() for t in (kc, vc, ks, vs)]
+    wide = torch.zeros(n, 4, dtype=torch.int32, device="cuda")
+    cu_kv = torch.tensor([0, 2 ** 31 - 1] * (n // 2) + [0], dtype=torch.int32, device="cuda")
+    q = torch.randn(n + 2, hq, d, generator=g).to(BF16).cuda()
+    cu = torch.arange(1, n + 2, dtype=torch.int32, device="cuda")
+    p = capi.problem_for(q, dev[0][0], cu, cu_kv, 1, d ** -0.5, causal=True)
+    p.total_kv = 2 ** 31 - 1
+    x = [ctypes.c_int32() for _ in range(3)]
+    capi.call("mtlattn_decode8_layout", ctypes.byref(p), 100000, *[ctypes.byref(i) for i in x])
+    assert x[0].value == x[1].value and x[2].value > 0      # (a unit is 32 keys, so that the sum wraps to -2^17)
+    keys = min(2 ** 31 - 1, 0x7fff0000)
+    assert ((n // 2) * -(-keys // 32)) % 2 ** 32 == 2 ** 32 - 2 ** 17
+    c = capi.Cache8(code=capi.CODE_INT8, page_size=page, block=64, num_heads_kv=hkv, head_dim=d, num_pages=pages,
+                    k=dev[0].data_ptr(), k_row_stride=hkv * d, v=dev[1].data_ptr(), v_row_stride=hkv * d,
+                    k_scale=dev[2].data_ptr(), v_scale=dev[3].data_ptr(), block_table=wide.data_ptr(),
+                    block_table_stride=wide.shape[1])
+    need = capi.lib().mtlattn_decode8_workspace_size(ctypes.byref(p), 100000)
+    ws = torch.zeros(need + 256, dtype=torch.uint8, device="cuda")
+    ws[need:] = 0xa5
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((n + 2, hq), 7.0, device="cuda")
+    capi.call("mtlattn_decode8", p, q.data_ptr(), hq * d, c, 100000, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need,
+              torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert bool((ws[need:] == 0xa5).all())
+    for t in (out, lse):
+        assert bool((t[0] == 7.0).all()) and bool((t[n + 1] == 7.0).all())
+    # every partial of the workspace is 0, and so are the rows that are written from it
+    assert bool(((out[1:n + 1] == 0) | (out[1:n + 1] == 7.0)).all())
+    out = mt.paged_decode(q[:2], dev[0], dev[1], cu_of([1, 1], "cuda"), cu_of(kv, "cuda"), table.cuda(), 1, 700,
+                          causal=True, k_scale=dev[2], v_scale=dev[3])
+    check_decode(out, None, *decode_reference(q[:2].cpu(), kc, ks, vc, vs, [0, 1, 2], kv, table, d ** -0.5, True), BF16)
