@@ -321,7 +321,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         // row of this head from its page, and the scales, which arrive in LDS.
         uint64_t vkp = 0, vvp = 0;
         float vks = 0.f, vvs = 0.f;
-        bool inf_scale = false;                          // one of vvs is an infinity
+        bool inf_scale = false;                          // one of V's was an infinity
         auto lookup_key = [&](int i0) { return min(ks + (tw + (i0 + lane / KB) * TW) * kKT + 16 * (lane % KB), ke - 1) & ~15; };
         auto page_of = [&](int key) { return p->page_log2 >= 0 ? key >> p->page_log2 : key / p->page_size; };
         auto table_entry = [&](int i0) { return bt + min(page_of(lookup_key(i0)), bt_last); };
@@ -491,20 +491,6 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                     wt[2 * e] -= __uint_as_float(x & 0xffff0000u);
                     wt[2 * e + 1] -= __uint_as_float(y & 0xffff0000u);
                 }
-            if (inf_scale) {
-                // (inf - inf: an infinity is its first part alone; inf * 0: keys that the row does
-                // not see are no terms)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t key = (uint32_t)(kt + 16 * (e >> 1) + 4 * lg + 2 * (e & 1) - first), h = pt[0][e];
-                    const uint32_t see = (key < width ? 0xffffu : 0u) | (key + 1 < width ? 0xffff0000u : 0u);
-                    const uint32_t fin = ((h & 0x7fffu) != 0x7f80u ? 0xffffu : 0u) |
-                                         ((h & 0x7fff0000u) != 0x7f800000u ? 0xffff0000u : 0u);
-                    pt[0][e] &= see;
-                    pt[1][e] &= see & fin;
-                    pt[2][e] &= see & fin;
-                }
-            }
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
                 const u32x2_t x = C::template unpack4<BF16>(vc[db][0]), y = C::template unpack4<BF16>(vc[db][1]);
@@ -528,7 +514,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
                 if (i % TPV == 0) {
                     vks = *reinterpret_cast<const float*>(look + 256 + 4 * lane) * p->scale_log2;
                     vvs = *reinterpret_cast<const float*>(look + 512 + 4 * lane);
-                    inf_scale = __any(fabsf(vvs) == kPosInf);
+                    // (infinite ones come in after the loop)
+                    inf_scale = inf_scale || __any(fabsf(vvs) == kPosInf);
+                    vvs = fabsf(vvs) == kPosInf ? 0.f : vvs;
                 }
                 step(i, buf);
                 wait_lds();
@@ -547,6 +535,33 @@ __global__ __launch_bounds__(NW * 64, D == 64 && NW == 8 ? 4 : 2) void decode8_k
         }
 
         p = params();
+        // A caller's own scales of V that are infinities: each key of theirs that a row sees
+        // adds its codes times the infinity, whatever its weight but 0.
+        if (inf_scale) {
+#pragma clang loop unroll(disable)
+            for (int j = 0; j < KB * n_my; ++j) {
+                const int k0 = ks + (tw + j / KB * TW) * kKT + 16 * (j % KB);
+                if (k0 >= ke) break;
+                const int pg = min(max(bt[min(page_of(k0), bt_last)], 0), p->num_pages - 1);
+                const int row = (pg - page_of(k0)) * p->page_size + k0;
+                const float inf = p->v_scale[(int64_t)(row >> p->block_log2) * p->hkv + hk];
+                if (fabsf(inf) != kPosInf) continue;
+#pragma clang loop unroll(disable)
+                for (int key = k0; key < min(k0 + 16, ke); ++key) {
+                    if ((uint32_t)(key - first) >= width) continue;
+                    float x = inf;
+                    if (BIAS) x *= key < p->bias_cols && brow[key] == kNegInf ? 0.f : 1.f;
+                    const uint8_t* vp = vbase + (int64_t)(row + key - k0) * p->v_rs + 4 * lg;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        float f[4];
+                        C::to_float4(*reinterpret_cast<const uint32_t*>(vp + 16 * db), f);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) oacc[db][r] += f[r] * x;
+                    }
+                }
+            }
+        }
         const float lt = quad_sum(l_run);
         // where row n of this wave's head goes: the output, or a partial
         auto out_row = [&](int n) {

@@ -71,7 +71,7 @@ def test_decode_weights_in_32_bits(mt, kind, dt):
     check_decode(out, None, ref, ref_lse, bound, None, dt)
 
 
-def _by_definition(q, kc, ks, vc, vs, ql, kv, table, causal, window):
+def _by_definition(q, kc, ks, vc, vs, ql, kv, table, causal, window, bias=None):
     """fp64 attention, each row over the keys that it sees and no others (an
     infinite value times the weight of a key that is not seen is no term)."""
     page, pages = kc.shape[1], kc.shape[0]
@@ -86,22 +86,27 @@ def _by_definition(q, kc, ks, vc, vs, ql, kv, table, causal, window):
             lo = max(0, end - window + 1) if window else 0
             see = at[lo:end + 1 if causal else n]
             for h in range(q.shape[1]):
-                p = torch.softmax((k[see, h // g] * q[row, h].double()).sum(-1) / math.sqrt(q.shape[2]), 0)
+                x = (k[see, h // g] * q[row, h].double()).sum(-1) / math.sqrt(q.shape[2])
+                if bias is not None:
+                    x = x + bias[row, 0, lo:lo + len(see)].double()
+                p = torch.softmax(x, 0)
                 out[row, h] = (p[:, None] * v[see, h // g]).sum(0)
             row += 1
     return out
 
 
-@pytest.mark.parametrize("kind,dt,d,block,page,ql,kv,causal,window", [
-    ("e4m3", BF16, 128, 16, 16, [1, 4, 2], [100, 203, 31], True, 0),
-    ("e4m3", F16, 64, 32, 96, [4, 1, 3], [333, 640, 65], True, 50),
-    ("int8", BF16, 128, 16, 64, [2, 4, 1], [2500, 70, 900], True, 70),
-    ("int8", F16, 64, 64, 64, [1, 3], [700, 2900], False, 0),
+@pytest.mark.parametrize("kind,dt,d,block,page,ql,kv,causal,window,biased", [
+    ("e4m3", BF16, 128, 16, 16, [1, 4, 2], [100, 203, 31], True, 0, False),
+    ("e4m3", F16, 64, 32, 96, [4, 1, 3], [333, 640, 65], True, 50, False),
+    ("int8", BF16, 128, 16, 64, [2, 4, 1], [2500, 70, 900], True, 70, False),
+    ("int8", F16, 64, 64, 64, [1, 3], [700, 2900], False, 0, False),
+    ("e4m3", BF16, 64, 16, 48, [3, 1, 2], [200, 77, 3000], True, 0, True),
+    ("int8", F16, 128, 32, 32, [2, 4], [400, 64], True, 90, True),
 ])
-def test_decode_infinite_value_scales(mt, kind, dt, d, block, page, ql, kv, causal, window):
+def test_decode_infinite_value_scales(mt, kind, dt, d, block, page, ql, kv, causal, window, biased):
     """A caller's own value scale that is an infinity gives what the definition
-    gives, an infinity or, where signs meet or a code is 0, a NaN; also in a block
-    whose other keys the row does not see."""
+    gives, an infinity or, where signs meet or a code or a weight is 0, a NaN; also
+    in a block whose other keys the row does not see."""
     gen = torch.Generator().manual_seed(53)
     hkv, g = 2, 2
     table, pages = pages_for(kv, page, gen)
@@ -122,12 +127,17 @@ def test_decode_infinite_value_scales(mt, kind, dt, d, block, page, ql, kv, caus
             flat[int(cache8.rows(table, s, key, key + 1, page, pages)[0]) // block, 0] = x
     q = torch.randn(sum(ql), hkv * g, d, generator=gen).to(dt)
     cu = _offsets(ql)
-    ref = _by_definition(q, kc, ks, vc, vs, ql, kv, table, causal, window)
+    bias = None
+    if biased:                      # (the first sequence's second row: weights of 0 among its infinite values)
+        bias = torch.randn(sum(ql), 1, max(kv), generator=gen)
+        bias[1, 0, kv[0] - 5:] = -math.inf
+    ref = _by_definition(q, kc, ks, vc, vs, ql, kv, table, causal, window, bias)
     clean = torch.where(torch.isinf(vs), torch.ones_like(vs), vs)
-    _, _, bound, _ = decode_reference(q, kc, ks, vc, clean, cu, kv, table, d ** -0.5, causal, window)
+    _, _, bound, _ = decode_reference(q, kc, ks, vc, clean, cu, kv, table, d ** -0.5, causal, window, bias)
     assert all(int(f(ref).sum()) >= d for f in (torch.isinf, torch.isnan, torch.isfinite))
     out = mt.paged_decode(q.cuda(), kc.cuda(), vc.cuda(), _int32(cu), cu_of(kv, "cuda"), table.cuda(), max(ql), max(kv),
-                          causal=causal, window=window, k_scale=ks.cuda(), v_scale=vs.cuda()).cpu()
+                          causal=causal, window=window, attn_bias=None if bias is None else bias.cuda(), k_scale=ks.cuda(),
+                          v_scale=vs.cuda()).cpu()
     assert torch.equal(torch.isnan(out), torch.isnan(ref))
     inf = torch.isinf(ref)
     assert torch.equal(out[inf].double(), ref[inf]) and not bool(torch.isinf(out[~inf]).any())
