@@ -210,7 +210,9 @@ __device__ inline uint32_t recode4(uint32_t w, float scale, float now) {
 // (block, head) meet in LDS for its largest magnitude. A workgroup holds W waves:
 // W / (block / 16) heads of one block, K or V; the other heads, then the other side,
 // of the block come next in the grid. ITER * 64 lanes hold 8 values each, 16 d
-// values in all, in registers between the two uses of them.
+// values in all, in registers between the two uses of them. (They do not fit where a
+// workgroup has 16 waves, blocks of 256 tokens, and D > 128 in int8: of 128 registers a
+// lane, 33 values go to memory for fp32 rows and 1 for 16-bit ones.)
 // The blocks that a sequence's new rows touch are numbered over the sequences, 64 of
 // them at a time, one lane each (total / block + 2 num_seqs bounds them); a wave's
 // rows do not need the page table, so that their loads and its lookup go out

@@ -14,13 +14,13 @@
 //   * P s_v, which spans fp32's range, goes into the P V product as the sum of three
 //     bf16 values: all 24 bits of it. (Two of them, 16 bits, left results of up to 2^-18 of
 //     sum P |v| off, which shows where weights next to each other cancel; the third costs
-//     0.7% of a long stream's time (64 sequences of 8192-65536 keys, 787 -> 792 us) and 4%
-//     of a short call's (16 of 128-2048, 18.4 -> 19.1). Up to 5 rows would have room for
+//     0.7% of a long stream's time (64 sequences of 8192-65536 keys, 785 -> 791 us) and 3%
+//     of a short call's (16 of 128-2048, 18.4 -> 19.0). Up to 5 rows would have room for
 //     the parts as columns of one product: no faster, its branch costs what it saves.)
 //   * One wave takes one kv head, the waves of a workgroup neighbouring heads of
 //     the same tokens, so that whole token rows are read at about the same time
 //     (one head's 128 bytes of each row at a time stream at 5.0 TB/s, 8 heads' at
-//     6.0; the arithmetic is hidden in both: without it the times are within 2%).
+//     6.0; the arithmetic is hidden in both: without it the times are within 3%).
 //     With fewer kv heads than waves the others take the next tiles.
 //   * Tiles of 32 keys go straight from HBM into the wave's LDS (two of them in
 //     turn, no workgroup barriers), K as rows for the operand reads, V for the
@@ -62,8 +62,9 @@ struct Dec8Params {
 
 // The kernels read their parameters where they lie. A fresh pointer (params) keeps
 // the compiler from holding a loop's worth of them, and of what follows from them, in
-// registers: it spilled up to 86 scalars before the first load (32 sequences of up to
-// 16384 keys, window 2048, 16 heads, D = 64: 34.8 us, 31.7 without).
+// registers: it put up to 86 scalars into lanes of vector registers before the first
+// load (32 sequences of up to 16384 keys, window 2048, 16 heads, D = 64: 34.8 us, 31.7
+// with a fresh pointer). 32 to 54 still go there, by instance, none to memory.
 typedef const __attribute__((address_space(4))) Dec8Params CParams;
 __device__ inline CParams* params() {
     uint64_t a = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
@@ -818,19 +819,19 @@ Dec8Plan make_dec8_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
     if ((max_kv <= 1024 || (max_kv <= 2048 && seq_heads > 32)) && g.num_seqs <= 8 * 65535) {
         // One workgroup per sequence, no second launch; as many of its waves on a head as
         // the CUs have room for: a wave takes about 1 us per tile, which a bandwidth-bound
-        // stream hides. bf16, D = 128, 32/8 heads, up to 1024 keys: 16 sequences 11.5 us
-        // with 8 waves on a head, 16.1 with 4, 42.6 with 1; 64 25.0 / 22.0 / 45.1, 256
-        // 81.9 / 66.9 / 63.3. Pieces took 16.3, 25.9 and 66.8; of up to 2048 keys (16, 64,
-        // 256 sequences) 18.5, 37.1 and 133.9 against 17.5, 34.0 and 131.3, of up to 4096
-        // (64) 62 against 68.
+        // stream hides. bf16, D = 128, 32/8 heads, up to 1024 keys: 16 sequences 12.1 us
+        // with 8 waves on a head, 17.4 with 4, 47.7 with 1; 64 26.0 / 22.9 / 50.5, 256
+        // 84.7 / 69.3 / 66.4. Pieces took 16.8, 26.4 and 67.6; of up to 2048 keys (16, 64,
+        // 256 sequences) 19.0, 37.9 and 136 against 18.7, 36.1 and 136-140, of up to 4096
+        // (64) 62 against 69.
         int hw = 1;
         while (seq_heads > (int64_t)cus * hw && hw < plan.waves) hw *= 2;
         plan.hw = heads(hw);
     } else {
         // Pieces for every workgroup that the CUs hold, of whole token rows (8 heads); few
         // tiles (under 4 a wave) on fewer heads and more waves each, with fewer partials: one
-        // sequence of 2048 keys 12.0 us with 2 heads, 16.7 with 8, 16.4 as a whole; four of
-        // 4096 16.0 and 16.8.
+        // sequence of 2048 keys 12.3 us with 2 heads, 17.4 with 8, 17.6 as a whole; four of
+        // 4096 16.1 and 16.8.
         const double tiles = (double)g.num_seqs * (double)max_kv / kKT * g.hkv * n_hg;
         plan.hw = heads(tiles < cus * 8 * 4 ? 2 : 8);
         const int resident = g.bias == nullptr ? (g.d == 64 ? 2 : 1) : (g.d == 64 ? 3 : 1);
