@@ -420,6 +420,93 @@ int mtlattn_decode8(const mtlattn_problem* p,
 int mtlattn_decode8_layout(const mtlattn_problem* p, int64_t max_seqlen_kv,
                            int32_t* waves, int32_t* heads, int32_t* pieces);
 
+/*
+ * Position rotation of queries and keys, with their per-head norms in the same
+ * pass. No counterpart in the reference. For each row and head, x of D values:
+ *   xh = x / sqrt(mean(x^2) + eps) * weight      (xh = x without weights)
+ *   y_a = scale (a cos t - b sin t), y_b = scale (b cos t + a sin t),
+ *   t = positions[row] * inv_freq[i]
+ * for the pairs (a, b) = (xh[i], xh[i + rotary_dim / 2]), or, interleaved,
+ * (xh[2 i], xh[2 i + 1]), i < rotary_dim / 2; elements from rotary_dim on are xh.
+ * Angles are formed in 64 bits, all else in fp32, rounded once.
+ */
+typedef struct mtlattn_rotary {
+    int32_t dtype;            /* MTLATTN_DTYPE_* of the rows */
+    int32_t num_heads_q;
+    int32_t num_heads_kv;
+    int32_t head_dim;         /* D, 1 .. 256 */
+    int32_t rotary_dim;       /* even, 0 (no rotation) .. D */
+    int32_t interleaved;      /* 0 / 1 */
+    float scale;
+    float eps;
+    int64_t total;            /* rows */
+    const int32_t* positions;      /* device int32 [total] */
+    const float* inv_freq;         /* device fp32 [rotary_dim / 2] */
+    const void* q_weight;          /* device [D], both or neither (NULL: no norms) */
+    const void* k_weight;
+    int32_t weight_dtype;     /* MTLATTN_DTYPE_F32, or dtype */
+} mtlattn_rotary;
+
+/*
+ * q [total, Hq, D] and k [total, Hkv, D] into q_out and k_out (row strides in
+ * elements). q_out may be q, k_out may be k (same pointer and stride);
+ * otherwise outputs share memory with nothing. No workspace.
+ * D and rotary_dim multiples of 16 and 16-byte aligned rows take the fast kernel.
+ */
+int mtlattn_rotary_fwd(const mtlattn_rotary* r,
+                       const void* q, int64_t q_row_stride,
+                       const void* k, int64_t k_row_stride,
+                       void* q_out, int64_t q_out_row_stride,
+                       void* k_out, int64_t k_out_row_stride,
+                       void* stream);
+
+/*
+ * Its backward: from dq_out and dk_out, the gradients dq and dk of q and k and,
+ * with norms, of the weights (dq_weight, dk_weight [D] of weight_dtype; NULL:
+ * not wanted). q and k are read with norms only. Outputs share memory with
+ * nothing. Workspace (with norms): fp32 sums of the weights' gradients, added in
+ * a fixed order: the same results from run to run.
+ */
+size_t mtlattn_rotary_bwd_workspace_size(const mtlattn_rotary* r);
+int mtlattn_rotary_bwd(const mtlattn_rotary* r,
+                       const void* q, int64_t q_row_stride,
+                       const void* k, int64_t k_row_stride,
+                       const void* dq_out, int64_t dq_out_row_stride,
+                       const void* dk_out, int64_t dk_out_row_stride,
+                       void* dq, int64_t dq_row_stride,
+                       void* dk, int64_t dk_row_stride,
+                       void* dq_weight, void* dk_weight,
+                       void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
+ * New rows into the 16-bit paged cache of mtlattn_paged_decode: sequence s's rows
+ * cu_seqlens[s] .. cu_seqlens[s + 1] of k and v [r->total, Hkv, D] become its last
+ * logical tokens, whose count cu_seqlens_kv (prefix sums, with the new tokens)
+ * gives. k is normed and rotated on the way as r says (rotary_dim 0, k_weight NULL:
+ * copied), and so is q, when it is not NULL, into q_out. r->positions NULL: a
+ * token's place in its sequence. With q NULL, q_weight and num_heads_q are
+ * not used. dtype fp16 or bf16, any page_size >= 1.
+ * Rows whose logical position is negative, or whose table column or page does not
+ * exist, are not written to the cache (their q is still turned); q_out rows of no
+ * sequence are 0. Nothing else of the cache changes. Cache rows that
+ * get tokens must stand once in the block tables. q_out may be q; otherwise
+ * caches, q_out and the rows must not share memory (K and V side by side in the token rows
+ * of one buffer do not); such calls are refused. No workspace; deterministic.
+ */
+int mtlattn_cache_append(const mtlattn_rotary* r,
+                         const void* q, int64_t q_row_stride,
+                         void* q_out, int64_t q_out_row_stride,
+                         const void* k, int64_t k_row_stride,
+                         const void* v, int64_t v_row_stride,
+                         void* k_cache, int64_t k_cache_row_stride,
+                         void* v_cache, int64_t v_cache_row_stride,
+                         int32_t page_size, int64_t num_pages,
+                         const int32_t* block_table, int64_t block_table_stride,
+                         int32_t num_seqs,
+                         const int32_t* cu_seqlens, const int32_t* cu_seqlens_kv,
+                         void* stream);
+
 /* Number of split-KV work-item slots per (kv head, head group) the forward's
  * decode routing would use for `p` (0 = the call is not routed to split-KV).
  * The automatic path cuts each sequence's KV into fixed-length chunks (about

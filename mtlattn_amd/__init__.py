@@ -262,6 +262,129 @@ def paged_cache_read(k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_seqlens_
                                block_table.int(), int(total), dtype)
 
 
+def paged_cache_append(k, v, k_cache, v_cache, cu_seqlens, cu_seqlens_kv, block_table, q=None, positions=None,
+                       inv_freq=None, interleaved=False, scale=1.0, q_weight=None, k_weight=None, eps=1e-6):
+    """Append new K/V rows to the 16-bit paged cache that paged_decode and
+    paged_tree_decode read, in place, with the keys (and the queries)
+    rotated to their positions on the way (no reference counterpart).
+
+    k, v: [M, Hkv, D] (fp16/bf16, row-strided views allowed), rows
+    cu_seqlens[s]..cu_seqlens[s+1] being the last logical tokens of sequence
+    s, of cu_seqlens_kv[s+1] - cu_seqlens_kv[s] in all: the offsets that
+    paged_decode then takes for its queries and keys. k_cache, v_cache:
+    [num_pages, page_size, Hkv, D] of k's dtype, any page_size; block_table
+    as for paged_decode.
+
+    inv_freq, interleaved, scale, q_weight, k_weight, eps: the rotation and
+    the norms, as for rotary; without inv_freq nothing is rotated, without
+    weights nothing normed, and with neither k is copied. positions: int [M],
+    by default each token's place in its sequence (drafted tokens of a tree
+    take their depths). q: [M, Hq, D], normed and rotated likewise.
+    Returns q's rows (None without q); rows of no sequence are 0.
+
+    Rows without a place (a table column or page that does not exist, more
+    rows than tokens) are not written, so a page of -1 drops its rows. Cache
+    rows that get tokens must stand once in the block tables: copy shared
+    pages first. The caches must not share memory with each other or with
+    q, k and v (caches that are slices of one tensor's token rows do not).
+    Not differentiable."""
+    if positions is not None:
+        positions = positions.int()
+    return _C.paged_cache_append(k, v, k_cache, v_cache, cu_seqlens.int(), cu_seqlens_kv.int(), block_table.int(), q,
+                                 positions, inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))
+
+
+# ---- position rotation ----
+
+
+class _RotaryFn(torch.autograd.Function):
+    """Autograd node for rotary. Without norms the backward is the rotation
+    back and needs nothing of the forward; with them it recomputes the norms
+    from q and k."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, q_weight, k_weight, eps):
+        ctx.args = (interleaved, scale)
+        ctx.eps = eps
+        ctx.normed = q_weight is not None
+        rows = (q, k, q_weight, k_weight) if ctx.normed else ()
+        ctx.save_for_backward(positions, inv_freq, *rows)
+        return _C.rotary(q, k, positions, inv_freq, interleaved, scale, q_weight, k_weight, eps)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, inv_freq, *rows = ctx.saved_tensors
+        q, k, q_weight, k_weight = rows if ctx.normed else (dq, dk, None, None)
+        dq, dk, dqw, dkw = _C.rotary_bwd(q, k, dq, dk, positions, inv_freq, *ctx.args, q_weight, k_weight, ctx.eps)
+        return dq, dk, None, None, None, None, dqw, dkw, None
+
+
+def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=None, k_weight=None, eps=1e-6):
+    """Rotate queries and keys to their positions, with their per-head norms
+    in the same pass (no reference counterpart). Differentiable in q, k and
+    the weights.
+
+    q: [M, Hq, D]; k: [M, Hkv, D] (fp32/fp16/bf16, row-strided views allowed,
+    D <= 256). positions: int [M]. inv_freq: fp32 [R / 2], the angle of a
+    pair per position, R <= D (see rotary_frequencies): the first R elements
+    of a head are rotated, pairs (i, i + R / 2), or (2 i, 2 i + 1) where
+    interleaved; the others pass. scale multiplies what is rotated.
+    q_weight, k_weight: [D] (fp32 or q's dtype), both or neither: heads are
+    first divided by sqrt(mean(x^2) + eps) and multiplied by the weight.
+    Angles are formed in 64 bits, everything else in fp32, rounded once to
+    q's dtype. Returns (q, k), contiguous."""
+    args = (positions.int(), inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        if (q_weight is None) != (k_weight is None):
+            raise ValueError("mtlattn: q_weight and k_weight go together")
+        return _RotaryFn.apply(q, k, *args)
+    return _C.rotary(q, k, *args)
+
+
+def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_length=4096, beta_fast=32.0, beta_slow=1.0,
+                       device="cuda"):
+    """(inv_freq, scale) for rotary and paged_cache_append: the angles per
+    position base^(-2 i / dim), i < dim / 2, for the `dim` elements of a head
+    that are rotated, scaled to a context `factor` times the trained one:
+
+    None: as trained; "linear": positions divided by factor; "ntk": base
+    times factor^(dim / (dim - 2)), so that the slowest pair turns factor
+    times slower and the fastest as before; "yarn": pairs that turn fewer
+    than beta_slow times over original_length as "linear", more than
+    beta_fast times as trained, a linear blend in between, and a scale of
+    0.1 ln(factor) + 1 (others: 1). Computed in 64 bits, returned in fp32 on
+    `device`."""
+    dim = int(dim)
+    if dim < 2 or dim % 2 != 0:
+        raise ValueError(f"mtlattn: the rotated part of a head must be even and positive (got {dim})")
+    if not base > 0 or not factor > 0:
+        raise ValueError("mtlattn: base and factor must be positive")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"mtlattn: unknown scaling {scaling!r} (None, 'linear', 'ntk' or 'yarn')")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    scale = 1.0
+    if scaling == "ntk":
+        if dim == 2:
+            raise ValueError("mtlattn: 'ntk' needs more than one pair")
+        base = base * factor ** (dim / (dim - 2))
+    freq = torch.pow(torch.tensor(float(base), dtype=torch.float64), -i / dim)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if not original_length > 0 or not beta_fast > beta_slow > 0:
+            raise ValueError("mtlattn: 'yarn' needs a positive original_length and beta_fast > beta_slow > 0")
+        # the pair (as a real number) that turns `turns` times over the trained length
+        def pair(turns):
+            return dim * math.log(original_length / (2 * math.pi * turns)) / (2 * math.log(base))
+        low = min(max(math.floor(pair(beta_fast)), 0), dim // 2 - 1)
+        high = min(max(math.ceil(pair(beta_slow)), 0), dim // 2 - 1)
+        slow = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        freq = freq * (1.0 - slow) + freq / factor * slow
+        if factor > 1:
+            scale = 0.1 * math.log(factor) + 1.0
+    return freq.float().to(device), scale
+
+
 # ---- dense scaled_dot_product_attention adapter ----
 
 _ORIG_SDPA = None

@@ -49,13 +49,24 @@ class Cache8(ctypes.Structure):
     ]
 
 
+class Rotary(ctypes.Structure):
+    """struct mtlattn_rotary (field order and widths as in the header)."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("num_heads_q", ctypes.c_int32), ("num_heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("eps", ctypes.c_float), ("total", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("weight_dtype", ctypes.c_int32),
+    ]
+
+
 class MtlattnError(RuntimeError):
     def __init__(self, fn, rc, msg):
         super().__init__(f"{fn} failed ({rc}): {msg}")
         self.rc = rc
 
 
-_P, _C8 = ctypes.POINTER(Problem), ctypes.POINTER(Cache8)
+_P, _C8, _R = ctypes.POINTER(Problem), ctypes.POINTER(Cache8), ctypes.POINTER(Rotary)
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
@@ -89,6 +100,12 @@ SIGNATURES = {
     "mtlattn_decode8_workspace_size": (_sz, [_P, _i64]),
     "mtlattn_decode8_layout": (ctypes.c_int, [_P, _i64, _i32p, _i32p, _i32p]),
     "mtlattn_decode8": (ctypes.c_int, [_P, _vp, _i64, _C8, _i64, _vp, _vp, _vp, _sz, _vp]),
+    "mtlattn_rotary_fwd": (ctypes.c_int, [_R, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "mtlattn_rotary_bwd_workspace_size": (_sz, [_R]),
+    "mtlattn_rotary_bwd": (ctypes.c_int, [_R, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp,
+                                          _vp, _sz, _vp]),
+    "mtlattn_cache_append": (ctypes.c_int, [_R, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32,
+                                            _i64, _vp, _i64, _i32, _vp, _vp, _vp]),
     "mtlattn_pack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "mtlattn_unpack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                              _vp]),

@@ -42,12 +42,6 @@ struct Cache8KParams {
     uint32_t div_head;                         // ceil(2^16 / (d / 8))
 };
 
-// Logical length of sequence s (the offsets are not bounded by a tensor).
-__device__ inline int kv_length(const int* __restrict__ cu_kv, int s) {
-    const int64_t n = (int64_t)cu_kv[s + 1] - cu_kv[s];
-    return (int)min(max(n, (int64_t)0), (int64_t)0x7fff0000);      // (room for a block in an int)
-}
-
 // Eight values of a row, as they are stored, and as fp32.
 template <typename T>
 struct Raw8 {

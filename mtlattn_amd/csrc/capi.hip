@@ -406,6 +406,63 @@ int check_cache8_rows(int32_t dtype, int64_t total, int32_t num_seqs, const int3
     return MTLATTN_OK;
 }
 
+// The rotation as every entry takes it. heads_q 0: no queries.
+int check_rotary(const mtlattn_rotary* r, bool append, const char* what) {
+    if (r == nullptr) return fail(MTLATTN_ERR_INVALID, "%s: null rotation descriptor", what);
+    if (r->dtype != MTLATTN_DTYPE_F32 && r->dtype != MTLATTN_DTYPE_F16 && r->dtype != MTLATTN_DTYPE_BF16)
+        return fail(MTLATTN_ERR_INVALID, "%s: unsupported dtype code %d", what, r->dtype);
+    if (r->total < 0 || r->total > 0x7fffffffLL) return fail(MTLATTN_ERR_INVALID, "%s: bad row count", what);
+    if (r->head_dim < 1 || r->head_dim > 256)
+        return fail(MTLATTN_ERR_INVALID, "%s: head_dim %d unsupported (expected 1..256)", what, r->head_dim);
+    if (r->num_heads_q < 0 || r->num_heads_kv < 1 || r->num_heads_q > 65536 || r->num_heads_kv > 65536)
+        return fail(MTLATTN_ERR_INVALID, "%s: bad head counts (%d, %d)", what, r->num_heads_q, r->num_heads_kv);
+    if (r->rotary_dim < 0 || r->rotary_dim > r->head_dim || r->rotary_dim % 2 != 0)
+        return fail(MTLATTN_ERR_INVALID, "%s: rotary_dim (%d) must be even and at most head_dim (%d)", what, r->rotary_dim,
+                    r->head_dim);
+    if (r->rotary_dim > 0 && r->total > 0 && (r->inv_freq == nullptr || (!append && r->positions == nullptr)))
+        return fail(MTLATTN_ERR_INVALID, "%s: null positions/inv_freq pointer", what);
+    if ((r->q_weight != nullptr || r->k_weight != nullptr) && r->weight_dtype != MTLATTN_DTYPE_F32 &&
+        r->weight_dtype != r->dtype)
+        return fail(MTLATTN_ERR_INVALID, "%s: weights must be fp32 or of the rows' type", what);
+    if (r->num_heads_q > 0 && (r->q_weight == nullptr) != (r->k_weight == nullptr))
+        return fail(MTLATTN_ERR_INVALID, "%s: q_weight and k_weight go together", what);
+    return MTLATTN_OK;
+}
+
+// [total, heads, D] rows of r by a row stride, in bytes.
+Rows rotary_rows(const mtlattn_rotary* r, const void* ptr, int64_t row_stride, int heads) {
+    const int64_t es = elem_size(r->dtype);
+    return {(int64_t)ptr, row_stride * es, (int64_t)heads * r->head_dim * es, r->total};
+}
+// (elements at their own alignment; offsets of rows far below 2^63)
+bool rotary_rows_ok(const mtlattn_rotary* r, const void* ptr, int64_t row_stride, int heads) {
+    return ptr != nullptr && (uintptr_t)ptr % elem_size(r->dtype) == 0 && row_stride < (int64_t(1) << 31) &&
+           (r->total == 1 || row_stride >= (int64_t)heads * r->head_dim);
+}
+
+RopeArgs rope_args(const mtlattn_rotary* r) {
+    RopeArgs a{};
+    a.weight[0] = r->q_weight;
+    a.weight[1] = r->k_weight;
+    a.w_dtype = r->weight_dtype;
+    a.positions = r->positions;
+    a.inv_freq = r->inv_freq;
+    a.scale = r->scale;
+    a.eps = r->eps;
+    a.interleaved = r->interleaved != 0;
+    a.hq = r->num_heads_q;
+    a.hkv = r->num_heads_kv;
+    a.d = r->head_dim;
+    a.rot = r->rotary_dim;
+    a.total = r->total;
+    return a;
+}
+
+size_t rotary_bwd_bytes(const mtlattn_rotary* r) {
+    if (r->k_weight == nullptr) return 0;
+    return (size_t)rope_part_wgs(r->total) * 2 * (size_t)r->head_dim * sizeof(float);
+}
+
 Cache8Args cache8_args(const mtlattn_cache8* c, int64_t total, int32_t num_seqs, const int32_t* cu, const int32_t* cu_kv) {
     Cache8Args a{};
     a.code = c->code;
@@ -1067,6 +1124,152 @@ int mtlattn_cache8_read(const mtlattn_cache8* c, int32_t dtype, void* k, void* v
     Cache8Args a = cache8_args(c, total, num_seqs, cu_seqlens, cu_seqlens_kv);
     a.k = k; a.v = v;
     return launch_status(launch_cache8_read(dtype, a, (hipStream_t)stream), "8-bit cache read");
+}
+
+int mtlattn_rotary_fwd(const mtlattn_rotary* r, const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride,
+                       void* q_out, int64_t q_out_row_stride, void* k_out, int64_t k_out_row_stride, void* stream) {
+    const int rc = check_rotary(r, false, "rotary_fwd");
+    if (rc != MTLATTN_OK) return rc;
+    if (r->num_heads_q < 1) return fail(MTLATTN_ERR_INVALID, "rotary_fwd: no query heads");
+    if (r->total == 0) return ok();
+    if (!rotary_rows_ok(r, q, q_row_stride, r->num_heads_q) || !rotary_rows_ok(r, k, k_row_stride, r->num_heads_kv) ||
+        !rotary_rows_ok(r, q_out, q_out_row_stride, r->num_heads_q) ||
+        !rotary_rows_ok(r, k_out, k_out_row_stride, r->num_heads_kv))
+        return fail(MTLATTN_ERR_INVALID, "rotary_fwd: q/k/q_out/k_out must be aligned rows whose strides cover a row");
+    const Rows in[2] = {rotary_rows(r, q, q_row_stride, r->num_heads_q), rotary_rows(r, k, k_row_stride, r->num_heads_kv)};
+    const Rows out[2] = {rotary_rows(r, q_out, q_out_row_stride, r->num_heads_q),
+                         rotary_rows(r, k_out, k_out_row_stride, r->num_heads_kv)};
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2; ++j)
+            if (share_memory(out[i], in[j]) && !(i == j && out[i].at == in[j].at && out[i].stride == in[j].stride))
+                return fail(MTLATTN_ERR_INVALID, "rotary_fwd: an output may share memory with its own input alone, row by row");
+    if (share_memory(out[0], out[1])) return fail(MTLATTN_ERR_INVALID, "rotary_fwd: q_out and k_out must not share memory");
+    RopeArgs a = rope_args(r);
+    a.in[0] = q; a.in[1] = k;
+    a.in_rs[0] = q_row_stride; a.in_rs[1] = k_row_stride;
+    a.out[0] = q_out; a.out[1] = k_out;
+    a.out_rs[0] = q_out_row_stride; a.out_rs[1] = k_out_row_stride;
+    return launch_status(launch_rope(r->dtype, a, (hipStream_t)stream), "rotation");
+}
+
+size_t mtlattn_rotary_bwd_workspace_size(const mtlattn_rotary* r) {
+    if (check_rotary(r, false, "rotary_bwd") != MTLATTN_OK) return 0;
+    return rotary_bwd_bytes(r);
+}
+
+int mtlattn_rotary_bwd(const mtlattn_rotary* r, const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride,
+                       const void* dq_out, int64_t dq_out_row_stride, const void* dk_out, int64_t dk_out_row_stride,
+                       void* dq, int64_t dq_row_stride, void* dk, int64_t dk_row_stride, void* dq_weight,
+                       void* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_rotary(r, false, "rotary_bwd");
+    if (rc != MTLATTN_OK) return rc;
+    if (r->num_heads_q < 1) return fail(MTLATTN_ERR_INVALID, "rotary_bwd: no query heads");
+    const bool norm = r->k_weight != nullptr;
+    if (!norm && (dq_weight != nullptr || dk_weight != nullptr))
+        return fail(MTLATTN_ERR_INVALID, "rotary_bwd: gradients of weights that there are not");
+    RopeArgs a = rope_args(r);
+    a.backward = true;
+    if (r->total == 0 && !norm) return ok();
+    if (r->total > 0) {
+        const void* in[4] = {dq_out, dk_out, q, k};
+        const int64_t in_rs[4] = {dq_out_row_stride, dk_out_row_stride, q_row_stride, k_row_stride};
+        void* out[2] = {dq, dk};
+        const int64_t out_rs[2] = {dq_row_stride, dk_row_stride};
+        const int heads[2] = {r->num_heads_q, r->num_heads_kv};
+        for (int i = 0; i < (norm ? 4 : 2); ++i)
+            if (!rotary_rows_ok(r, in[i], in_rs[i], heads[i & 1]))
+                return fail(MTLATTN_ERR_INVALID, "rotary_bwd: q/k/dq_out/dk_out must be aligned rows whose strides cover a row");
+        for (int i = 0; i < 2; ++i) {
+            if (!rotary_rows_ok(r, out[i], out_rs[i], heads[i]))
+                return fail(MTLATTN_ERR_INVALID, "rotary_bwd: dq/dk must be aligned rows whose strides cover a row");
+            for (int j = 0; j < (norm ? 4 : 2); ++j)
+                if (share_memory(rotary_rows(r, out[i], out_rs[i], heads[i]), rotary_rows(r, in[j], in_rs[j], heads[j & 1])))
+                    return fail(MTLATTN_ERR_INVALID, "rotary_bwd: outputs and inputs must not share memory");
+        }
+        if (share_memory(rotary_rows(r, dq, dq_row_stride, heads[0]), rotary_rows(r, dk, dk_row_stride, heads[1])))
+            return fail(MTLATTN_ERR_INVALID, "rotary_bwd: dq and dk must not share memory");
+        for (int i = 0; i < 2; ++i) {
+            a.in[i] = in[i];
+            a.in_rs[i] = in_rs[i];
+            a.out[i] = out[i];
+            a.out_rs[i] = out_rs[i];
+            a.x[i] = norm ? in[2 + i] : nullptr;
+            a.x_rs[i] = norm ? in_rs[2 + i] : 0;
+        }
+    }
+    const size_t need = rotary_bwd_bytes(r);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return fail(MTLATTN_ERR_WORKSPACE, "rotary_bwd: workspace too small (%zu < %zu bytes)", workspace_bytes, need);
+    if (need > 0 && (uintptr_t)workspace % 4 != 0)
+        return fail(MTLATTN_ERR_WORKSPACE, "rotary_bwd: the workspace must be 4-byte aligned");
+    a.part = (float*)workspace;
+    a.part_wgs = rope_part_wgs(r->total);
+    a.dw[0] = dq_weight;
+    a.dw[1] = dk_weight;
+    return launch_status(launch_rope(r->dtype, a, (hipStream_t)stream), "rotation backward");
+}
+
+int mtlattn_cache_append(const mtlattn_rotary* r, const void* q, int64_t q_row_stride, void* q_out, int64_t q_out_row_stride,
+                         const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, void* k_cache,
+                         int64_t k_cache_row_stride, void* v_cache, int64_t v_cache_row_stride, int32_t page_size,
+                         int64_t num_pages, const int32_t* block_table, int64_t block_table_stride, int32_t num_seqs,
+                         const int32_t* cu_seqlens, const int32_t* cu_seqlens_kv, void* stream) {
+    if (r == nullptr) return fail(MTLATTN_ERR_INVALID, "cache_append: null rotation descriptor");
+    mtlattn_rotary d = *r;
+    if (q == nullptr) {
+        if (q_out != nullptr) return fail(MTLATTN_ERR_INVALID, "cache_append: q_out without q");
+        d.num_heads_q = 0;
+        d.q_weight = nullptr;
+    } else if (d.num_heads_q < 1) {
+        return fail(MTLATTN_ERR_INVALID, "cache_append: no query heads");
+    }
+    const int rc = check_rotary(&d, true, "cache_append");
+    if (rc != MTLATTN_OK) return rc;
+    if (!is16(d.dtype)) return fail(MTLATTN_ERR_UNSUPPORTED, "cache_append: half/bf16");
+    if (q != nullptr && d.rotary_dim == 0 && d.k_weight == nullptr)
+        return fail(MTLATTN_ERR_INVALID, "cache_append: q has neither a norm nor a rotation to take");
+    if (page_size < 1) return fail(MTLATTN_ERR_INVALID, "cache_append: page_size must be positive (got %d)", page_size);
+    if (num_pages < 1 || num_pages > 0x7fffffffLL || num_pages * (int64_t)page_size > 0x7fffffffLL)
+        return fail(MTLATTN_ERR_INVALID, "cache_append: num_pages * page_size must be in [1, 2^31)");
+    if (block_table_stride < 1) return fail(MTLATTN_ERR_INVALID, "cache_append: block_table_stride must be >= 1");
+    if (num_seqs < 1 || cu_seqlens == nullptr || cu_seqlens_kv == nullptr)
+        return fail(MTLATTN_ERR_INVALID, "cache_append: cu_seqlens and cu_seqlens_kv must both be [B+1]");
+    if (d.total == 0) return ok();
+    if (block_table == nullptr || k_cache == nullptr || v_cache == nullptr)
+        return fail(MTLATTN_ERR_INVALID, "cache_append: null k_cache/v_cache/block_table pointer");
+    mtlattn_rotary c = d;                                       // (the caches' rows)
+    c.total = num_pages * (int64_t)page_size;
+    if (!rotary_rows_ok(&d, k, k_row_stride, d.num_heads_kv) || !rotary_rows_ok(&d, v, v_row_stride, d.num_heads_kv) ||
+        (q != nullptr && (!rotary_rows_ok(&d, q, q_row_stride, d.num_heads_q) ||
+                          !rotary_rows_ok(&d, q_out, q_out_row_stride, d.num_heads_q))) ||
+        !rotary_rows_ok(&c, k_cache, k_cache_row_stride, d.num_heads_kv) ||
+        !rotary_rows_ok(&c, v_cache, v_cache_row_stride, d.num_heads_kv))
+        return fail(MTLATTN_ERR_INVALID, "cache_append: rows must be aligned, their strides cover a row");
+    // what is written: q_out, the caches; what else is read
+    const Rows mem[6] = {rotary_rows(&c, k_cache, k_cache_row_stride, d.num_heads_kv),
+                         rotary_rows(&c, v_cache, v_cache_row_stride, d.num_heads_kv),
+                         rotary_rows(&d, k, k_row_stride, d.num_heads_kv),
+                         rotary_rows(&d, v, v_row_stride, d.num_heads_kv),
+                         rotary_rows(&d, q_out, q_out_row_stride, d.num_heads_q),
+                         rotary_rows(&d, q, q_row_stride, d.num_heads_q)};
+    const int n = q != nullptr ? 6 : 4;
+    for (int i = 0; i < 2; ++i)
+        for (int j = i + 1; j < n; ++j)
+            if (share_memory(mem[i], mem[j]))
+                return fail(MTLATTN_ERR_INVALID, "cache_append: caches, q_out and the rows must not share memory");
+    if (q != nullptr && (share_memory(mem[4], mem[2]) || share_memory(mem[4], mem[3]) ||
+                         (share_memory(mem[4], mem[5]) && !(q_out == q && q_out_row_stride == q_row_stride))))
+        return fail(MTLATTN_ERR_INVALID, "cache_append: caches, q_out and the rows must not share memory");
+    RopeArgs a = rope_args(&d);
+    a.append = true;
+    a.in[0] = q; a.in[1] = k; a.in[2] = v;
+    a.in_rs[0] = q_row_stride; a.in_rs[1] = k_row_stride; a.in_rs[2] = v_row_stride;
+    a.out[0] = q_out; a.out[1] = k_cache; a.out[2] = v_cache;
+    a.out_rs[0] = q_out_row_stride; a.out_rs[1] = k_cache_row_stride; a.out_rs[2] = v_cache_row_stride;
+    a.cu = cu_seqlens; a.cu_kv = cu_seqlens_kv;
+    a.block_table = block_table; a.bt_stride = block_table_stride;
+    a.num_seqs = num_seqs; a.page_size = page_size; a.num_pages = (int)num_pages;
+    return launch_status(launch_rope(d.dtype, a, (hipStream_t)stream), "cache append");
 }
 
 size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv) {

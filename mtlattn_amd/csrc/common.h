@@ -519,6 +519,13 @@ __device__ inline SeqRange seq_range(const int* __restrict__ cu, int s, int64_t 
     return {a, b};
 }
 
+// Logical length of sequence s in a paged cache (its offsets are not bounded by a
+// tensor; room for a block in an int).
+__device__ inline int kv_length(const int* __restrict__ cu_kv, int s) {
+    const int64_t n = (int64_t)cu_kv[s + 1] - cu_kv[s];
+    return (int)min(max(n, (int64_t)0), (int64_t)0x7fff0000);
+}
+
 // Largest s in [0, num_seqs) with cu[s] / tile + s <= t (binary search; all
 // lanes compute the same value).
 __device__ inline int find_seq_for_tile(const int* __restrict__ cu, int num_seqs, int tile, int t,

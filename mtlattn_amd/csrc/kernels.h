@@ -214,6 +214,33 @@ struct Cache8Args {
     int64_t k_rs, v_rs;
 };
 
+// Position rotation of q and k rows with per-head norms (launch_rope): rows in and
+// out by row strides (elements), [total, heads, d]. append: the keys and values go
+// to the rows of a paged cache (out[1], out[2] are the caches, out_rs their token
+// strides; hq == 0: no queries), by offsets as in Cache8Args; positions null: the
+// token's place in its sequence. backward: in = gradients of the rotated rows, out
+// = those of x; with norms x holds the rows, part room for part_wgs * 2 * d floats
+// and dw (nullable) the weights' gradients.
+struct RopeArgs {
+    const void* in[3]; int64_t in_rs[3];
+    void* out[3]; int64_t out_rs[3];
+    const void* x[2]; int64_t x_rs[2];
+    const void* weight[2];                     // null: no norm
+    int w_dtype;
+    const int* positions; const float* inv_freq;
+    float scale, eps;
+    int interleaved, hq, hkv, d, rot;          // rot: elements of a head that turn
+    int64_t total;
+    bool append, backward;
+    const int* cu; const int* cu_kv; const int* block_table;
+    int64_t bt_stride;
+    int num_seqs, page_size, num_pages;
+    float* part;
+    int part_wgs;
+    void* dw[2];
+};
+int rope_part_wgs(int64_t total);
+
 // Launchers return hipSuccess or the launch error. `dtype` is MTLATTN_DTYPE_*.
 hipError_t launch_fwd_mfma(int dtype, const FwdArgs& a, hipStream_t st);
 hipError_t launch_fwd_dense(int dtype, const DenseArgs& a, hipStream_t st);
@@ -254,6 +281,7 @@ hipError_t launch_decode(int dtype, const DecodeArgs& a, hipStream_t st);
 hipError_t launch_decode8(int dtype, int code, const Dec8Args& a, hipStream_t st);
 hipError_t launch_cache8_write(int dtype, const Cache8Args& a, hipStream_t st);
 hipError_t launch_cache8_read(int dtype, const Cache8Args& a, hipStream_t st);
+hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st);
 hipError_t launch_pad_pack(int esize, int B, int N, int H, int D, const void* src, int64_t sb, int64_t sh,
                            int64_t sn, const int* lens, int* cu, void* dst, hipStream_t st);
 hipError_t launch_pad_unpack(int esize, int B, int N, int H, int D, const void* src, const int* lens, const int* cu,

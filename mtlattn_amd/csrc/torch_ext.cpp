@@ -11,6 +11,7 @@
 #include <c10/core/DeviceGuard.h>
 
 #include <tuple>
+#include <vector>
 
 #include "../../include/mtlattn_capi.h"
 
@@ -497,6 +498,191 @@ std::tuple<at::Tensor, at::Tensor> paged_cache_read(const at::Tensor& k_cache, c
     return {k, v};
 }
 
+// Rows [M, H, D] with a free row stride.
+void check_rows3(const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), "mtlattn: ", name, " must be a GPU (HIP) tensor");
+    TORCH_CHECK(t.dim() == 3 && t.size(1) > 0 && t.size(2) >= 1 && t.size(2) <= 256, "mtlattn: ", name,
+                " must be [M, H, D] with D in 1..256");
+    TORCH_CHECK(t.size(0) == 0 || ((t.size(2) == 1 || t.stride(2) == 1) && (t.size(1) == 1 || t.stride(1) == t.size(2))),
+                "mtlattn: inner dims must be contiguous ([M, H, D] with row-only striding)");
+    dtype_code(t.scalar_type());
+}
+
+// A 16-bit paged cache [num_pages, page_size, Hkv, D] (token rows may be strided) for rows like x.
+void check_cache16(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& x) {
+    TORCH_CHECK(k_cache.is_cuda() && v_cache.is_cuda(), "mtlattn: k_cache/v_cache must be GPU tensors");
+    TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() && k_cache.numel() > 0,
+                "mtlattn: k_cache/v_cache must both be [num_pages, page_size, Hkv, D]");
+    const int64_t page_size = k_cache.size(1), Hkv = k_cache.size(2), D = k_cache.size(3);
+    for (const auto& c : {k_cache, v_cache}) {
+        TORCH_CHECK(c.scalar_type() == x.scalar_type(), "mtlattn: dtype mismatch");
+        TORCH_CHECK((D == 1 || c.stride(3) == 1) && (Hkv == 1 || c.stride(2) == D),
+                    "mtlattn: cache inner dims [Hkv, D] must be contiguous");
+        TORCH_CHECK(c.size(0) <= 1 || page_size <= 1 || c.stride(0) == page_size * c.stride(1),
+                    "mtlattn: cache pages must be page_size consecutive token rows");
+        TORCH_CHECK(c.get_device() == x.get_device(), "mtlattn: rows and caches must be on the same device");
+    }
+}
+
+// The scalar part of a rotation (no reference counterpart) over q [M, Hq, D] and k
+// [M, Hkv, D]. inv_freq: fp32 [R / 2] of the first R elements of a head; weights
+// [D], fp32 or of the rows' type. The descriptor points into `keep`, which the
+// caller keeps.
+mtlattn_rotary make_rotary(const at::Tensor& k, int64_t heads_q, const c10::optional<at::Tensor>& positions,
+                           const c10::optional<at::Tensor>& inv_freq, bool interleaved, double scale,
+                           const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight, double eps,
+                           std::vector<at::Tensor>& keep) {
+    mtlattn_rotary r;
+    std::memset(&r, 0, sizeof(r));
+    r.dtype = dtype_code(k.scalar_type());
+    r.num_heads_q = (int32_t)std::min<int64_t>(heads_q, 0x7fffffff);
+    r.num_heads_kv = (int32_t)std::min<int64_t>(k.size(1), 0x7fffffff);
+    r.head_dim = (int32_t)k.size(2);
+    r.interleaved = interleaved ? 1 : 0;
+    r.scale = (float)scale;
+    r.eps = (float)eps;
+    r.total = k.size(0);
+    auto here = [&](const at::Tensor& t) { return t.is_cuda() && t.get_device() == k.get_device(); };
+    if (defined(inv_freq)) {
+        TORCH_CHECK(here(*inv_freq) && inv_freq->scalar_type() == at::kFloat && inv_freq->dim() == 1 &&
+                        2 * inv_freq->numel() <= k.size(2),
+                    "mtlattn: inv_freq must be an fp32 [R / 2] GPU tensor, R at most the head dim");
+        keep.push_back(inv_freq->contiguous());
+        r.inv_freq = keep.back().data_ptr<float>();
+        r.rotary_dim = (int32_t)(2 * inv_freq->numel());
+    }
+    if (defined(positions)) {
+        TORCH_CHECK(here(*positions) && positions->scalar_type() == at::kInt && positions->dim() == 1 &&
+                        positions->numel() == k.size(0),
+                    "mtlattn: positions must be an int32 [M] GPU tensor");
+        keep.push_back(positions->contiguous());
+        r.positions = keep.back().data_ptr<int32_t>();
+    }
+    const c10::optional<at::Tensor>* weights[2] = {&q_weight, &k_weight};
+    for (int i = 0; i < 2; ++i) {
+        if (!defined(*weights[i])) continue;
+        const at::Tensor& t = **weights[i];
+        TORCH_CHECK(here(t) && t.dim() == 1 && t.numel() == k.size(2) &&
+                        (t.scalar_type() == at::kFloat || t.scalar_type() == k.scalar_type()),
+                    "mtlattn: q_weight/k_weight must be [D] GPU tensors, fp32 or of the rows' type");
+        const int code = dtype_code(t.scalar_type());
+        TORCH_CHECK(i == 0 || r.q_weight == nullptr || code == r.weight_dtype,
+                    "mtlattn: q_weight and k_weight must be of one type");
+        r.weight_dtype = code;
+        keep.push_back(t.contiguous());
+        (i == 0 ? r.q_weight : r.k_weight) = keep.back().data_ptr();
+    }
+    return r;
+}
+
+// q and k rows of one rotation.
+void check_rotated(const at::Tensor& q, const at::Tensor& k) {
+    check_rows3(q, "q");
+    check_rows3(k, "k");
+    TORCH_CHECK(q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.scalar_type() == k.scalar_type() &&
+                    q.get_device() == k.get_device(),
+                "mtlattn: q and k must have the same tokens, head dim, dtype and device");
+}
+
+// Rows that do not overlap (a broadcast over tokens is laid out); gradients also with
+// their inner dims contiguous.
+at::Tensor laid_out(const at::Tensor& t) {
+    return t.size(0) > 1 && t.stride(0) < t.size(1) * t.size(2) ? t.contiguous() : t;
+}
+at::Tensor gradient_rows(const at::Tensor& t) {
+    const bool inner = t.dim() == 3 && (t.size(2) == 1 || t.stride(2) == 1) && (t.size(1) == 1 || t.stride(1) == t.size(2));
+    return inner ? laid_out(t) : t.contiguous();
+}
+
+// _C.rotary: q and k with their heads normed and rotated.
+std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& positions,
+                                          const at::Tensor& inv_freq, bool interleaved, double scale,
+                                          c10::optional<at::Tensor> q_weight, c10::optional<at::Tensor> k_weight,
+                                          double eps) {
+    check_rotated(q_, k_);
+    const c10::OptionalDeviceGuard guard(q_.device());
+    const auto q = laid_out(q_), k = laid_out(k_);
+    std::vector<at::Tensor> keep;
+    const mtlattn_rotary r =
+        make_rotary(k, q.size(1), positions, inv_freq, interleaved, scale, q_weight, k_weight, eps, keep);
+    auto qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+    check_rc(mtlattn_rotary_fwd(&r, q.data_ptr(), row_stride(q), k.data_ptr(), row_stride(k), qo.data_ptr(), row_stride(qo),
+                                ko.data_ptr(), row_stride(ko), current_stream(q)));
+    return {qo, ko};
+}
+
+// _C.rotary_bwd: its gradients (dq, dk, dq_weight, dk_weight), the weights' undefined
+// without norms. q and k: the rows with norms, else any tensors of their shapes.
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> rotary_bwd(
+    const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& dq_out_, const at::Tensor& dk_out_,
+    const at::Tensor& positions, const at::Tensor& inv_freq, bool interleaved, double scale, c10::optional<at::Tensor> q_weight,
+    c10::optional<at::Tensor> k_weight, double eps) {
+    const c10::OptionalDeviceGuard guard(q_.device());
+    const auto q = gradient_rows(q_), k = gradient_rows(k_), dq_out = gradient_rows(dq_out_), dk_out = gradient_rows(dk_out_);
+    check_rotated(q, k);
+    check_rotated(dq_out, dk_out);
+    TORCH_CHECK(q.sizes() == dq_out.sizes() && k.sizes() == dk_out.sizes() && q.scalar_type() == dq_out.scalar_type() &&
+                    q.get_device() == dq_out.get_device(),
+                "mtlattn: gradients must be like q and k");
+    std::vector<at::Tensor> keep;
+    const mtlattn_rotary r =
+        make_rotary(k, q.size(1), positions, inv_freq, interleaved, scale, q_weight, k_weight, eps, keep);
+    auto dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
+    c10::optional<at::Tensor> dqw, dkw;
+    if (r.q_weight != nullptr) dqw = at::empty({k.size(2)}, q_weight->options());
+    if (r.k_weight != nullptr) dkw = at::empty({k.size(2)}, k_weight->options());
+    const size_t ws_bytes = mtlattn_rotary_bwd_workspace_size(&r);
+    at::Tensor ws = workspace((int64_t)ws_bytes, q);
+    check_rc(mtlattn_rotary_bwd(&r, q.data_ptr(), row_stride(q), k.data_ptr(), row_stride(k), dq_out.data_ptr(),
+                                row_stride(dq_out), dk_out.data_ptr(), row_stride(dk_out), dq.data_ptr(), row_stride(dq),
+                                dk.data_ptr(), row_stride(dk), dqw ? dqw->data_ptr() : nullptr,
+                                dkw ? dkw->data_ptr() : nullptr, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
+                                current_stream(q)));
+    return {dq, dk, dqw, dkw};
+}
+
+// _C.paged_cache_append: rows k, v [M, Hkv, D] into a 16-bit paged cache, k (and q, whose
+// rows are returned) normed and rotated on the way.
+c10::optional<at::Tensor> paged_cache_append(const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& k_cache,
+                                             const at::Tensor& v_cache, const at::Tensor& cu_seqlens,
+                                             const at::Tensor& cu_seqlens_kv, const at::Tensor& block_table,
+                                             c10::optional<at::Tensor> q_, c10::optional<at::Tensor> positions,
+                                             c10::optional<at::Tensor> inv_freq, bool interleaved, double scale,
+                                             c10::optional<at::Tensor> q_weight, c10::optional<at::Tensor> k_weight,
+                                             double eps) {
+    check_qkv(k_, k_, v_);
+    check_cu(cu_seqlens, cu_seqlens_kv, k_);
+    const bool has_q = q_.has_value() && q_->defined();
+    if (has_q) check_rotated(*q_, k_);
+    const c10::OptionalDeviceGuard guard(k_.device());
+    const auto k = laid_out(k_), v = laid_out(v_);
+    const auto q = has_q ? c10::optional<at::Tensor>(laid_out(*q_)) : c10::nullopt;
+    check_cache16(k_cache, v_cache, k);
+    TORCH_CHECK(k.size(1) == k_cache.size(2) && k.size(2) == k_cache.size(3),
+                "mtlattn: k/v heads and head dim must be the cache's");
+    TORCH_CHECK(block_table.is_cuda() && block_table.get_device() == k.get_device() &&
+                    block_table.scalar_type() == at::kInt && block_table.dim() == 2 &&
+                    block_table.size(0) == cu_seqlens.numel() - 1 && block_table.size(1) > 0,
+                "mtlattn: block_table must be an int32 [B, max_pages] GPU tensor");
+    std::vector<at::Tensor> keep;
+    const mtlattn_rotary r = make_rotary(k, has_q ? q->size(1) : 0, positions, inv_freq, interleaved, scale, q_weight,
+                                         k_weight, eps, keep);
+    auto cu = cu_seqlens.contiguous(), cu_kv = cu_seqlens_kv.contiguous(), bt = block_table.contiguous();
+    c10::optional<at::Tensor> qo;
+    if (has_q) qo = at::empty(q->sizes(), q->options());
+    const int64_t row = k.size(1) * k.size(2);
+    check_rc(mtlattn_cache_append(&r, has_q ? q->data_ptr() : nullptr, has_q ? row_stride(*q) : 0,
+                                  qo ? qo->data_ptr() : nullptr, qo ? row_stride(*qo) : 0, k.data_ptr(), row_stride(k),
+                                  v.data_ptr(), row_stride(v), k_cache.data_ptr(),
+                                  k_cache.size(1) > 1 ? k_cache.stride(1) : k_cache.size(0) > 1 ? k_cache.stride(0) : row,
+                                  v_cache.data_ptr(),
+                                  v_cache.size(1) > 1 ? v_cache.stride(1) : v_cache.size(0) > 1 ? v_cache.stride(0) : row,
+                                  (int32_t)std::min<int64_t>(k_cache.size(1), 0x7fffffff), k_cache.size(0),
+                                  bt.data_ptr<int32_t>(), bt.size(1), (int32_t)(cu.numel() - 1), cu.data_ptr<int32_t>(),
+                                  cu_kv.data_ptr<int32_t>(), current_stream(k)));
+    return qo;
+}
+
 // _C.paged_decode8: paged_decode over an 8-bit cache.
 at::Tensor paged_decode8(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                          const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& cu_seqlens_q,
@@ -698,6 +884,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("paged_cache_read", &paged_cache_read, "the last tokens of each sequence out of an 8-bit cache",
           py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seqlens"),
           py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("total"), py::arg("dtype"));
+    m.def("rotary", &rotary, "q and k with their heads normed and rotated", py::arg("q"), py::arg("k"),
+          py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0,
+          py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6);
+    m.def("rotary_bwd", &rotary_bwd, "gradients of rotary", py::arg("q"), py::arg("k"), py::arg("dq_out"),
+          py::arg("dk_out"), py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false,
+          py::arg("scale") = 1.0, py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(),
+          py::arg("eps") = 1e-6);
+    m.def("paged_cache_append", &paged_cache_append, "rows into a 16-bit paged KV cache, normed and rotated on the way",
+          py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"), py::arg("cu_seqlens"),
+          py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("q") = py::none(), py::arg("positions") = py::none(),
+          py::arg("inv_freq") = py::none(), py::arg("interleaved") = false, py::arg("scale") = 1.0,
+          py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6);
     m.def("paged_decode8", &paged_decode8, "paged_decode over an 8-bit cache", py::arg("q"), py::arg("k_cache"),
           py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seqlens_q"),
           py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("max_seqlen_q"), py::arg("max_seqlen_kv"),
