@@ -507,6 +507,37 @@ int mtlattn_cache_append(const mtlattn_rotary* r,
                          const int32_t* cu_seqlens, const int32_t* cu_seqlens_kv,
                          void* stream);
 
+/*
+ * Attention of a tree of drafted tokens over the cache of mtlattn_paged_decode. No
+ * counterpart in the reference. Sequence s's queries, rows cu_seqlens_q[s] ..
+ * cu_seqlens_q[s + 1], are its last logical tokens, whose keys are in the cache
+ * already (mtlattn_cache_append); query i sees every key before them, and of them
+ * token j iff tree_mask's byte j of the query's row is not 0 (j < tree_cols; itself
+ * included only if the mask says so).
+ *   out[row] = sum_j softmax_j(p->scale * q k_j) v_j over the seen keys, lse as for the
+ *   forward; rows that see no key: 0 and -inf. Keys that a row does not see do not reach it, whatever
+ *   their values.
+ *   p            : dtype fp16/bf16, D in {64, 128}, cu_seqlens_kv the logical lengths
+ *                  (prefix sums); total_kv, causal, window and bias are not read.
+ *                  max_seqlen_q shapes the launch only, and so does max_seqlen_kv
+ *   tree_mask    : bytes [total_q, tree_cols], row stride in bytes, tree_cols in [1, 256]
+ *   the cache    : as for mtlattn_paged_decode, page_size a multiple of 16
+ * Rows of no sequence are left as they were. Deterministic.
+ * Workspace: mtlattn_tree_decode_workspace_size(p, max_seqlen_kv) bytes, 16-byte aligned.
+ */
+size_t mtlattn_tree_decode_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv);
+int mtlattn_tree_decode(const mtlattn_problem* p,
+                        const void* q, int64_t q_row_stride,
+                        const void* k_cache, int64_t k_row_stride,
+                        const void* v_cache, int64_t v_row_stride,
+                        int32_t page_size, int64_t num_pages,
+                        const int32_t* block_table, int64_t block_table_stride,
+                        int64_t max_seqlen_kv,
+                        const uint8_t* tree_mask, int64_t tree_mask_row_stride, int32_t tree_cols,
+                        void* out, float* lse,
+                        void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 /* Number of split-KV work-item slots per (kv head, head group) the forward's
  * decode routing would use for `p` (0 = the call is not routed to split-KV).
  * The automatic path cuts each sequence's KV into fixed-length chunks (about

@@ -294,6 +294,32 @@ def paged_cache_append(k, v, k_cache, v_cache, cu_seqlens, cu_seqlens_kv, block_
                                  positions, inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))
 
 
+def paged_tree_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_table, tree_mask, max_seqlen_q,
+                      max_seqlen_kv, scale=None, lse_out=None):
+    """Attention of a tree of drafted tokens over a paged KV cache, as
+    speculative decoding verifies them (no reference counterpart).
+
+    q: [Mq, Hq, D]: sequence s's rows cu_seqlens_q[s]..cu_seqlens_q[s+1] are
+    its drafted tokens, which are its last logical tokens; their keys and
+    values are in the cache already (paged_cache_append, with the tokens'
+    depths as positions). tree_mask: bool [Mq, T], T <= 256: a query sees
+    every key before the drafted tokens, and of those token j of its sequence
+    iff tree_mask[row, j] (itself too only if the mask says so; columns past
+    the sequence's tokens are not read, tokens past T are seen by none).
+    k_cache, v_cache, block_table, cu_seqlens_kv, max_seqlen_kv, lse_out as
+    for paged_decode (fp16/bf16, D in {64, 128}, page_size a multiple of 16).
+    max_seqlen_q: the longest tree (any number; it shapes the launch, and so
+    does max_seqlen_kv). scale defaults to 1/sqrt(D).
+
+    Rows that see nothing are 0 (LSE -inf). Nothing of a key that a row does
+    not see reaches it, infinities and NaN included. Forward only; the same
+    from run to run. Returns [Mq, Hq, D]."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    return _C.paged_tree_decode(q, k_cache, v_cache, cu_seqlens_q.int(), cu_seqlens_kv.int(), block_table.int(),
+                                tree_mask, int(max_seqlen_q), int(max_seqlen_kv), float(scale), lse_out)
+
+
 # ---- position rotation ----
 
 

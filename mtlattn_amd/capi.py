@@ -106,6 +106,9 @@ SIGNATURES = {
                                           _vp, _sz, _vp]),
     "mtlattn_cache_append": (ctypes.c_int, [_R, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32,
                                             _i64, _vp, _i64, _i32, _vp, _vp, _vp]),
+    "mtlattn_tree_decode_workspace_size": (_sz, [_P, _i64]),
+    "mtlattn_tree_decode": (ctypes.c_int, [_P, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _i64, _i64, _vp, _i64,
+                                           _i32, _vp, _vp, _vp, _sz, _vp]),
     "mtlattn_pack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "mtlattn_unpack_padded": (ctypes.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                              _vp]),

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1270,6 +1271,63 @@ int mtlattn_cache_append(const mtlattn_rotary* r, const void* q, int64_t q_row_s
     a.block_table = block_table; a.bt_stride = block_table_stride;
     a.num_seqs = num_seqs; a.page_size = page_size; a.num_pages = (int)num_pages;
     return launch_status(launch_rope(d.dtype, a, (hipStream_t)stream), "cache append");
+}
+
+size_t mtlattn_tree_decode_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv) {
+    if (check_problem(p) != MTLATTN_OK || max_seqlen_kv < 0) return 0;
+    return make_tree_plan(make_geo(p), p->max_seqlen_q, max_seqlen_kv, device_cus()).bytes;
+}
+
+int mtlattn_tree_decode(const mtlattn_problem* p, const void* q, int64_t q_row_stride, const void* k_cache,
+                        int64_t k_row_stride, const void* v_cache, int64_t v_row_stride, int32_t page_size,
+                        int64_t num_pages, const int32_t* block_table, int64_t block_table_stride, int64_t max_seqlen_kv,
+                        const uint8_t* tree_mask, int64_t tree_mask_row_stride, int32_t tree_cols, void* out, float* lse,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_problem(p);
+    if (rc != MTLATTN_OK) return rc;
+    if (!is16(p->dtype)) return fail(MTLATTN_ERR_UNSUPPORTED, "tree_decode: half/bf16");
+    if (!decode_head_dim(p->head_dim)) return fail(MTLATTN_ERR_UNSUPPORTED, "tree_decode: D in {64,128}");
+    if (p->max_seqlen_q < 1) return fail(MTLATTN_ERR_INVALID, "tree_decode: max_seqlen_q must be positive");
+    if (!(fabsf(p->scale) < INFINITY)) return fail(MTLATTN_ERR_INVALID, "tree_decode: scale must be finite");
+    if (page_size < 16 || page_size % 16 != 0)
+        return fail(MTLATTN_ERR_INVALID, "tree_decode: page_size must be a positive multiple of 16 (got %d)", page_size);
+    if (num_pages < 1 || num_pages > 0x7fffffffLL || num_pages * (int64_t)page_size > 0x7fffffffLL)
+        return fail(MTLATTN_ERR_INVALID, "tree_decode: num_pages * page_size must be in [1, 2^31)");
+    if (block_table_stride < 1) return fail(MTLATTN_ERR_INVALID, "tree_decode: block_table_stride must be >= 1");
+    if (max_seqlen_kv < 0) return fail(MTLATTN_ERR_INVALID, "tree_decode: negative max_seqlen_kv");
+    if (tree_cols < 1 || tree_cols > kTreeMaxCols)
+        return fail(MTLATTN_ERR_UNSUPPORTED, "tree_decode: a mask of 1 to %d columns (got %d)", kTreeMaxCols, tree_cols);
+    if (p->total_q * (p->num_heads_q / p->num_heads_kv) > 0x7fffffffLL)
+        return fail(MTLATTN_ERR_UNSUPPORTED, "tree_decode: more than 2^31 query rows");
+    if (p->total_q == 0) return ok();
+    if (q == nullptr || out == nullptr || k_cache == nullptr || v_cache == nullptr || block_table == nullptr ||
+        tree_mask == nullptr)
+        return fail(MTLATTN_ERR_INVALID, "tree_decode: null q/k_cache/v_cache/block_table/tree_mask/out pointer");
+    const int64_t qrow = (int64_t)p->num_heads_q * p->head_dim, row = (int64_t)p->num_heads_kv * p->head_dim;
+    if ((p->total_q > 1 && (q_row_stride < qrow || tree_mask_row_stride < 0)) || k_row_stride < row || v_row_stride < row)
+        return fail(MTLATTN_ERR_INVALID, "tree_decode: row strides must cover a row");
+    if (!aligned16(q, q_row_stride, p->dtype) || !aligned16(k_cache, k_row_stride, p->dtype) ||
+        !aligned16(v_cache, v_row_stride, p->dtype) || ((uintptr_t)out & 15u) != 0)
+        return fail(MTLATTN_ERR_UNSUPPORTED, "tree_decode: q/k/v rows must be 16-byte aligned");
+    if (!tile_stride_ok(k_row_stride) || !tile_stride_ok(v_row_stride))
+        return fail(MTLATTN_ERR_UNSUPPORTED, "tree_decode: cache row strides must be below 2^24");
+    TreeArgs a{};
+    a.geo = make_geo(p);
+    a.plan = make_tree_plan(a.geo, p->max_seqlen_q, max_seqlen_kv, device_cus());
+    if (workspace == nullptr || workspace_bytes < a.plan.bytes)
+        return fail(MTLATTN_ERR_WORKSPACE, "tree_decode: workspace too small (%zu < %zu bytes)", workspace_bytes,
+                    a.plan.bytes);
+    if ((uintptr_t)workspace % 16 != 0)
+        return fail(MTLATTN_ERR_WORKSPACE, "tree_decode: the workspace must be 16-byte aligned");
+    a.q = q; a.q_rs = q_row_stride;
+    a.k = k_cache; a.k_rs = k_row_stride;
+    a.v = v_cache; a.v_rs = v_row_stride;
+    a.page_size = page_size; a.num_pages = (int)num_pages;
+    a.block_table = block_table; a.bt_stride = block_table_stride;
+    a.mask = tree_mask; a.mask_rs = tree_mask_row_stride; a.mask_cols = tree_cols;
+    a.o = out; a.lse = lse;
+    a.workspace = workspace;
+    return launch_status(launch_tree(p->dtype, a, (hipStream_t)stream), "tree decode");
 }
 
 size_t mtlattn_decode8_workspace_size(const mtlattn_problem* p, int64_t max_seqlen_kv) {

@@ -241,6 +241,28 @@ struct RopeArgs {
 };
 int rope_part_wgs(int64_t total);
 
+// Attention of drafted tokens' trees over a 16-bit paged cache (launch_tree): rows of
+// 32, 64 or 128 per workgroup, `grid` workgroups, workspace bytes.
+constexpr int kTreeMaxCols = 256;              // columns of the mask
+struct TreePlan {
+    int rows = 128, grid = 1;
+    size_t bytes = 0;
+};
+TreePlan make_tree_plan(const Geometry& g, int max_q, int64_t max_kv, int cus);
+struct TreeArgs {
+    Geometry geo;                              // (no total_kv, causal, window, bias)
+    const void* q; int64_t q_rs;
+    const void* k; int64_t k_rs;               // caches, token strides
+    const void* v; int64_t v_rs;
+    int page_size, num_pages;
+    const int* block_table; int64_t bt_stride;
+    const uint8_t* mask; int64_t mask_rs; int mask_cols;
+    void* o;                                   // contiguous [total_q, hq, d]
+    float* lse;                                // nullable
+    TreePlan plan;
+    void* workspace;
+};
+
 // Launchers return hipSuccess or the launch error. `dtype` is MTLATTN_DTYPE_*.
 hipError_t launch_fwd_mfma(int dtype, const FwdArgs& a, hipStream_t st);
 hipError_t launch_fwd_dense(int dtype, const DenseArgs& a, hipStream_t st);
@@ -282,6 +304,7 @@ hipError_t launch_decode8(int dtype, int code, const Dec8Args& a, hipStream_t st
 hipError_t launch_cache8_write(int dtype, const Cache8Args& a, hipStream_t st);
 hipError_t launch_cache8_read(int dtype, const Cache8Args& a, hipStream_t st);
 hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st);
+hipError_t launch_tree(int dtype, const TreeArgs& a, hipStream_t st);
 hipError_t launch_pad_pack(int esize, int B, int N, int H, int D, const void* src, int64_t sb, int64_t sh,
                            int64_t sn, const int* lens, int* cu, void* dst, hipStream_t st);
 hipError_t launch_pad_unpack(int esize, int B, int N, int H, int D, const void* src, const int* lens, const int* cu,

@@ -683,6 +683,66 @@ c10::optional<at::Tensor> paged_cache_append(const at::Tensor& k_, const at::Ten
     return qo;
 }
 
+// _C.paged_tree_decode: attention of drafted tokens' trees over a 16-bit paged cache.
+at::Tensor paged_tree_decode(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                             const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_kv,
+                             const at::Tensor& block_table, const at::Tensor& tree_mask, int64_t max_seqlen_q,
+                             int64_t max_seqlen_kv, double scale, c10::optional<at::Tensor> lse_out) {
+    check_rows3(q, "q");
+    check_cache16(k_cache, v_cache, q);
+    const int64_t D = q.size(2), Hkv = k_cache.size(2), page_size = k_cache.size(1);
+    TORCH_CHECK(k_cache.size(3) == D, "mtlattn: k_cache head dim must match q");
+    TORCH_CHECK(q.size(1) % Hkv == 0, "mtlattn: query heads must be a multiple of kv heads");
+    check_cu(cu_seqlens_q, cu_seqlens_kv, q);
+    TORCH_CHECK(block_table.is_cuda() && block_table.get_device() == q.get_device() &&
+                    block_table.scalar_type() == at::kInt && block_table.dim() == 2 &&
+                    block_table.size(0) == cu_seqlens_q.numel() - 1,
+                "mtlattn: block_table must be an int32 [B, max_pages] GPU tensor");
+    TORCH_CHECK(max_seqlen_kv >= 0 && block_table.size(1) * page_size >= max_seqlen_kv,
+                "mtlattn: block_table has ", block_table.size(1), " pages of ", page_size,
+                " tokens per sequence, fewer than max_seqlen_kv (", max_seqlen_kv, ")");
+    TORCH_CHECK(tree_mask.is_cuda() && tree_mask.get_device() == q.get_device() &&
+                    tree_mask.scalar_type() == at::kBool && tree_mask.dim() == 2 && tree_mask.size(0) == q.size(0) &&
+                    tree_mask.size(1) >= 1,
+                "mtlattn: tree_mask must be a bool [total_q, T] GPU tensor");
+    const c10::OptionalDeviceGuard guard(q.device());
+    auto cu_q = cu_seqlens_q.contiguous(), cu_kv = cu_seqlens_kv.contiguous(), bt = block_table.contiguous();
+    const auto qr = laid_out(q);
+    const auto mask = tree_mask.size(1) == 1 || tree_mask.stride(1) == 1 ? tree_mask : tree_mask.contiguous();
+    auto out = at::empty({q.size(0), q.size(1), D}, q.options());
+    float* lse = nullptr;
+    if (defined(lse_out)) {
+        const at::Tensor& l = *lse_out;
+        TORCH_CHECK(l.is_cuda() && l.get_device() == q.get_device() && l.scalar_type() == at::kFloat && l.is_contiguous() &&
+                        l.dim() == 2 && l.size(0) == q.size(0) && l.size(1) == q.size(1),
+                    "mtlattn: lse_out must be a contiguous fp32 [total_q, H] GPU tensor");
+        lse = l.data_ptr<float>();
+    }
+    mtlattn_problem p;
+    std::memset(&p, 0, sizeof(p));
+    p.dtype = dtype_code(q.scalar_type());
+    p.num_seqs = (int32_t)(cu_q.numel() - 1);
+    p.total_q = q.size(0);
+    p.num_heads_q = (int32_t)q.size(1);
+    p.num_heads_kv = (int32_t)Hkv;
+    p.head_dim = (int32_t)D;
+    p.max_seqlen_q = (int32_t)std::max<int64_t>(std::min<int64_t>(max_seqlen_q, 0x7fffffff), -1);
+    p.scale = (float)scale;
+    p.cu_seqlens_q = cu_q.data_ptr<int32_t>();
+    p.cu_seqlens_kv = cu_kv.data_ptr<int32_t>();
+    const size_t ws_bytes = mtlattn_tree_decode_workspace_size(&p, max_seqlen_kv);
+    at::Tensor ws = workspace((int64_t)ws_bytes, q);
+    const int64_t row = Hkv * D;
+    const int64_t krs = k_cache.size(1) > 1 ? k_cache.stride(1) : row, vrs = v_cache.size(1) > 1 ? v_cache.stride(1) : row;
+    check_rc(mtlattn_tree_decode(&p, qr.data_ptr(), row_stride(qr), k_cache.data_ptr(), krs, v_cache.data_ptr(), vrs,
+                                 (int32_t)std::min<int64_t>(page_size, 0x7fffffff), k_cache.size(0), bt.data_ptr<int32_t>(),
+                                 bt.size(1), max_seqlen_kv, (const uint8_t*)mask.data_ptr(),
+                                 mask.size(0) > 1 ? mask.stride(0) : mask.size(1),
+                                 (int32_t)std::min<int64_t>(mask.size(1), 0x7fffffff), out.data_ptr(), lse, ws.data_ptr(),
+                                 ws_bytes, current_stream(q)));
+    return out;
+}
+
 // _C.paged_decode8: paged_decode over an 8-bit cache.
 at::Tensor paged_decode8(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                          const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& cu_seqlens_q,
@@ -896,6 +956,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("q") = py::none(), py::arg("positions") = py::none(),
           py::arg("inv_freq") = py::none(), py::arg("interleaved") = false, py::arg("scale") = 1.0,
           py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6);
+    m.def("paged_tree_decode", &paged_tree_decode, "attention of drafted tokens' trees over a paged KV cache", py::arg("q"),
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("cu_seqlens_q"), py::arg("cu_seqlens_kv"), py::arg("block_table"),
+          py::arg("tree_mask"), py::arg("max_seqlen_q"), py::arg("max_seqlen_kv"), py::arg("scale"),
+          py::arg("lse_out") = py::none());
     m.def("paged_decode8", &paged_decode8, "paged_decode over an 8-bit cache", py::arg("q"), py::arg("k_cache"),
           py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seqlens_q"),
           py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("max_seqlen_q"), py::arg("max_seqlen_kv"),
