@@ -242,10 +242,10 @@ struct RopeArgs {
 int rope_part_wgs(int64_t total);
 
 // Attention of drafted tokens' trees over a 16-bit paged cache (launch_tree): rows of
-// 32, 64 or 128 per workgroup, `pieces` of the work of each kv head, workspace bytes.
+// 32 to 256 per workgroup, `side` workgroups with other rows side by side, `pieces` of the work, workspace bytes.
 constexpr int kTreeMaxCols = 256;              // columns of the mask
 struct TreePlan {
-    int rows = 128, pieces = 1;
+    int rows = 128, side = 1, pieces = 1;
     size_t bytes = 0;
 };
 TreePlan make_tree_plan(const Geometry& g, int max_q, int64_t max_kv, int cus);

@@ -34,6 +34,25 @@
 #include "kernels.h"
 #include "../../include/mtlattn_capi.h"
 
+#ifndef LB64
+#define LB64 2
+#endif
+#ifndef A32
+#define A32 4, 1, 128, 2
+#define H32 1
+#define K32 128
+#endif
+#ifndef A64
+#define A64 4, 2, 64, 2
+#define H64 2
+#define K64 64
+#endif
+#ifndef A128
+#define A128 4, 4, 64, 2
+#define H128 2
+#define K128 64
+#endif
+#define A256 8, 8, 128, 2
 namespace mtlattn {
 
 namespace {
@@ -49,12 +68,12 @@ struct TreeKParams {
     int64_t q_rs, k_rs, v_rs, bt_stride, total_q;
     int num_seqs, hq, hkv, g, mask_cols;
     int page_size, page_log2, num_pages;               // page_log2: -1 where the page is no power of two
-    int pieces;                                        // workgroups: pieces * hkv
+    int pieces, side;                                  // workgroups: pieces * hkv * side (row tiles side by side)
     float scale_log2;                                  // > 0; q's bits are changed by (x & q_and) ^ q_xor
     uint32_t q_and, q_xor;
     int4* desc;                                        // per workgroup: first query, rows, row tile and pieces of the
                                                        // unit that it begins and leaves to others (pieces 0: none)
-    float* part_lse; float* part_o;                    // [pieces][hkv][2][ROWS], [pieces][hkv][2][ROWS][D]
+    float* part_lse; float* part_o;                    // [workgroups][2][ROWS], [workgroups][2][ROWS][D]
 };
 
 // The kernel reads its parameters where they lie: a fresh pointer keeps the compiler
@@ -73,10 +92,10 @@ __device__ inline const char* uniform(const char* x) {
     return (const char*)((uint64_t)(uint32_t)uniform((int)(a >> 32)) << 32 | (uint32_t)uniform((int)(uint32_t)a));
 }
 
-// The units of a sequence: first query, queries, keys, key tiles, row tiles, and the work of
-// one kv head's in key tiles.
+// The units of a sequence: first query, queries, keys, key tiles, rounds of row tiles (`side`
+// of them at a time), and the work of one of the workgroups side by side in key tiles.
 struct SeqWork {
-    int q0, n, len, tiles, rows;
+    int q0, n, len, tiles, rounds;
     int64_t work;
 };
 template <int ROWS, int KT>
@@ -87,22 +106,41 @@ __device__ inline SeqWork seq_work(CParams* p, int s) {
     w.n = r.end - r.start;
     w.len = kv_length(p->cu_kv, s);
     w.tiles = max(1, (w.len + KT - 1) / KT);           // (without keys: rows of 0)
-    w.rows = (w.n * p->g + ROWS - 1) / ROWS;
-    w.work = (int64_t)w.tiles * w.rows;
+    w.rounds = ((w.n * p->g + ROWS - 1) / ROWS + p->side - 1) / p->side;
+    w.work = (int64_t)w.tiles * w.rounds;
     return w;
 }
 __device__ inline int64_t lane_value64(int64_t x, int l) {
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, l), hi = __builtin_amdgcn_readlane((int)(x >> 32), l);
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
-// Sums over the lanes up to and with each one.
+// x + the value `ctrl` moves here from another lane (0 where there is none).
+template <int CTRL, int ROWS_MASK>
+__device__ inline int add_dpp(int x) {
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS_MASK, 0xf, false);
+}
+// Sums over the lanes up to and with each one: by lane moves in 32 bits where they hold it.
 __device__ inline int64_t wave_scan64(int64_t x, int lane) {
+    if (!__any(x >= (1 << 24))) {
+        int y = (int)x;
+        y = add_dpp<0x111, 0xf>(y);                    // row_shr 1, 2, 4, 8: within 16 lanes
+        y = add_dpp<0x112, 0xf>(y);
+        y = add_dpp<0x114, 0xf>(y);
+        y = add_dpp<0x118, 0xf>(y);
+        y = add_dpp<0x142, 0xa>(y);                    // row_bcast 15: into the second and the fourth 16
+        y = add_dpp<0x143, 0xc>(y);                    // row_bcast 31: into the upper 32
+        return y;
+    }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const int64_t y = __shfl_up((long long)x, o);
         if (lane >= o) x += y;
     }
     return x;
+}
+// a / b of non-negative numbers, in 32 bits where those hold them.
+__device__ inline int64_t quotient(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 // 32 bits of a token's mask for the keys from node `base` of the tree on (keys before the tree: 1).
@@ -115,10 +153,12 @@ __device__ inline uint32_t mask_bits(const uint32_t* words, int base) {
 }
 
 // Ones in the halves of w that are finite.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+template <typename T>
+constexpr uint32_t kInf16 = T::code == BF16::code ? 0x7f80u : 0x7c00u;
 template <typename T>
 __device__ inline uint32_t finite_halves(uint32_t w) {
-    constexpr uint32_t top = T::code == BF16::code ? 0x7f80u : 0x7c00u;
-    return ((w & 0x7fffu) >= top ? 0u : 0xffffu) | ((w >> 16 & 0x7fffu) >= top ? 0u : 0xffff0000u);
+    return ((w & 0x7fffu) >= kInf16<T> ? 0u : 0xffffu) | ((w >> 16 & 0x7fffu) >= kInf16<T> ? 0u : 0xffff0000u);
 }
 
 // The bits of the tokens' masks of a row tile, a wave per token: bytes in, ballots out.
@@ -145,7 +185,7 @@ __device__ inline void load_masks(CParams* p, uint32_t (*s_mask)[kMaskWords], in
 }
 
 template <typename T, int D, int NW, int RW, int KT, int NBUF>
-__global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 ? 2 : 1) void tree_kernel(TreeKParams) {
+__global__ __launch_bounds__(NW * 64, NW <= 4 && NBUF * KT * D * 4 <= 40 * 1024 ? LB64 : NW <= 4 && NBUF * KT * D * 4 <= 72 * 1024 ? 2 : 1) void tree_kernel(TreeKParams) {
     constexpr int KW = NW / RW, ROWS = 32 * RW;
     constexpr int NKB = KT / 32 / KW;                  // 32-key blocks of a wave
     constexpr int NPC = 2 * NKB;                       // 16-key chunks of P
@@ -161,19 +201,24 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
     static_assert((KW - 1) * RW * kShare <= NBUF * STAGE, "the waves' results meet in the ring");
     __shared__ __attribute__((aligned(1024))) char smem[NBUF * STAGE];
     __shared__ uint32_t s_mask[ROWS][kMaskWords];
+    __shared__ int s_odd;
 
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
     const int l32 = lane & 31, hi = lane >> 5, rw = w % RW, kw = w / RW;
 
-    // the piece: all work of a kv head, and where this piece's share begins. The kv heads of
-    // a piece run side by side, so that whole rows of the cache are read together.
-    int id, piece_id, hk, s = 0;
+    // the piece: all work, and where this piece's share begins. The kv heads of a piece run
+    // side by side, so that whole rows of the cache are read together, and so do `side` row
+    // tiles of a head, which read the same.
+    int id, piece_id, hk, rt0, s = 0;
     int64_t at, end, base = 0, piece;
+    SeqWork sw;
     {
         CParams* p = params();
-        id = xcd_remap((int)blockIdx.x, p->pieces * p->hkv);
-        piece_id = uniform(id / p->hkv);
-        hk = id - piece_id * p->hkv;
+        id = xcd_remap((int)blockIdx.x, p->pieces * p->hkv * p->side);
+        const int col = uniform(id / p->side);
+        rt0 = id - col * p->side;
+        piece_id = uniform(col / p->hkv);
+        hk = col - piece_id * p->hkv;
         const int n = p->num_seqs;
         const SeqWork first = seq_work<ROWS, KT>(p, min(lane, n - 1));
         const int64_t sum0 = wave_scan64(lane < n ? first.work : 0, lane);
@@ -182,7 +227,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
             const SeqWork x = seq_work<ROWS, KT>(p, min(g0 + lane, n - 1));
             total += lane_value64(wave_scan64(g0 + lane < n ? x.work : 0, lane), 63);
         }
-        piece = max((int64_t)kMinPiece, (total + p->pieces - 1) / p->pieces);
+        piece = max((int64_t)kMinPiece, quotient(total + p->pieces - 1, p->pieces));
         at = piece_id * piece;
         end = min(total, at + piece);
         if (at >= end) {
@@ -190,32 +235,42 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
             return;
         }
         for (int g0 = 0; g0 < n; g0 += 64) {
-            int64_t sum = sum0, work = first.work;
+            int64_t sum = sum0;
+            sw = first;
             if (g0 > 0) {
-                work = seq_work<ROWS, KT>(p, min(g0 + lane, n - 1)).work;
-                sum = wave_scan64(g0 + lane < n ? work : 0, lane);
+                sw = seq_work<ROWS, KT>(p, min(g0 + lane, n - 1));
+                sum = wave_scan64(g0 + lane < n ? sw.work : 0, lane);
             }
             const uint64_t past = __ballot(g0 + lane < n && base + sum > at);
             if (past != 0) {
                 const int l = __builtin_ctzll(past);
                 s = g0 + l;
-                base += lane_value64(sum - work, l);
+                base += lane_value64(sum - sw.work, l);
+                sw.q0 = __builtin_amdgcn_readlane(sw.q0, l);
+                sw.n = __builtin_amdgcn_readlane(sw.n, l);
+                sw.len = __builtin_amdgcn_readlane(sw.len, l);
+                sw.tiles = __builtin_amdgcn_readlane(sw.tiles, l);
+                sw.work = lane_value64(sw.work, l);
                 break;
             }
             base += lane_value64(sum, 63);
         }
     }
 
-    // where this lane's rows of a 16-key block of K and of V lie: byte offsets of its direct loads
-    uint32_t off[NU > 1 ? 2 : 1][NI];
+    // Where this lane's part of a 16-row block lies: instruction j loads row 16 j / NI +
+    // lane / (64 NI / 16), at the chunk that the swizzle puts there (TileStager::lane_off), which is
+    // (its chunk of instruction 0) ^ (16 j / NI rows' part of the swizzle)
+    constexpr int LR = 64 * 16 / (2 * D);              // rows of an instruction
+    const uint32_t chunk0 = (uint32_t)((lane & (D / 8 - 1)) ^ row_swz<D>(lane / (D / 8))) * 16u;
+    uint32_t lane_row[NU > 1 ? 2 : 1];                 // byte offsets of the lane's row of instruction 0, in K and V
     {
         CParams* p = params();
-#pragma unroll
-        for (int i = 0; i < (NU > 1 ? 2 : 1); ++i) {
-            const bool key_side = NU > 1 ? i == 0 : w < NW / 2;
-            const uint32_t rs2 = (uint32_t)(2 * (key_side ? p->k_rs : p->v_rs));
-#pragma unroll
-            for (int j = 0; j < NI; ++j) off[i][j] = St::lane_off(j, lane, St::row_of(j, lane), rs2);
+        const uint32_t r = (uint32_t)(lane / (D / 8));
+        if (NU > 1) {
+            lane_row[0] = r * (uint32_t)(2 * p->k_rs);
+            lane_row[NU > 1] = r * (uint32_t)(2 * p->v_rs);
+        } else {
+            lane_row[0] = r * (uint32_t)(2 * (w < NW / 2 ? p->k_rs : p->v_rs));
         }
     }
     const uint32_t rbase = row_base<D>(l32, hi) + kw * NKB * 32 * 2 * D, tbase = TILE + tr_base<D>(lane) + kw * NKB * 32 * 2 * D;
@@ -224,19 +279,22 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
 
     while (at < end) {
         CParams* p = params();
-        if (s >= p->num_seqs) break;
-        const SeqWork sw = seq_work<ROWS, KT>(p, s);
         if (at >= base + sw.work) {                    // (this sequence is done, or has no queries)
             base += sw.work;
-            ++s;
+            if (++s >= p->num_seqs) break;
+            sw = seq_work<ROWS, KT>(p, s);
             continue;
         }
-        const int rt = uniform((int)((at - base) / sw.tiles));
-        const int t0 = uniform((int)(at - base - (int64_t)rt * sw.tiles));
+        const int round = uniform((int)quotient(at - base, sw.tiles)), rt = round * p->side + rt0;
+        const int t0 = uniform((int)(at - base - (int64_t)round * sw.tiles));
         const int t1 = uniform((int)min((int64_t)sw.tiles, t0 + (end - at)));
         const int len = uniform(sw.len), ctx = len - uniform(sw.n), n_rows = uniform(sw.n) * p->g, q0 = uniform(sw.q0);
         const bool whole = t0 == 0 && t1 == sw.tiles;
-        if (t0 == 0 && !whole) begun = int4{q0, n_rows, rt, (int)((at + sw.tiles - 1) / piece) - piece_id + 1};
+        if ((int64_t)rt * ROWS >= n_rows) {            // (the last round has fewer row tiles)
+            at += t1 - t0;
+            continue;
+        }
+        if (t0 == 0 && !whole) begun = int4{q0, n_rows, rt, (int)quotient(at + sw.tiles - 1, piece) - piece_id + 1};
         at += t1 - t0;
 
         // 16 keys of a tile at a time; past the last key, its block again, rows that repeat it
@@ -247,29 +305,54 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
         const int64_t k_rs = p->k_rs, v_rs = p->v_rs;
         const char* kh = reinterpret_cast<const char*>(p->k + (int64_t)hk * D);
         const char* vh = reinterpret_cast<const char*>(p->v + (int64_t)hk * D);
-        // block i of this wave's in tile `it`: whether of K, its first key, its place in a stage, its source
-        auto key_side = [&](int i) { return w + i * NW < KT / 16; };
-        auto first_key = [&](int it, int i) __attribute__((always_inline)) {
-            return min((t0 + it) * KT + 16 * ((w + i * NW) & (KT / 16 - 1)), (len - 1) & ~15);
+        // Cache rows of 64 blocks of 16 keys at a time (TPG tiles), a lane each, the next 64's
+        // lookups under way meanwhile.
+        constexpr int BPT = KT / 16, TPG = 64 / BPT;
+        auto block_key = [&](int g) { return min((t0 + g * TPG) * KT + 16 * lane, (len - 1) & ~15); };
+        auto block_col = [&](int key) { return page_log2 >= 0 ? key >> page_log2 : key / page_size; };
+        auto lookup = [&](int g) { return bt[min(block_col(block_key(g)), last_col)]; };
+        auto cache_row = [&](int pg, int g) {
+            const int key = block_key(g);
+            return min(max(pg, 0), num_pages - 1) * page_size + (key - block_col(key) * page_size);
         };
-        auto source = [&](int key, int i) __attribute__((always_inline)) {
-            const int col = uniform(page_log2 >= 0 ? key >> page_log2 : key / page_size);
-            const int pg = min(max(uniform(bt[min(col, last_col)]), 0), num_pages - 1);
-            const int64_t row = (int64_t)pg * page_size + (key - col * page_size);
+        int rows_now = 0, pages_next = 0;
+        if (n_tiles > 0) {
+            rows_now = cache_row(lookup(0), 0);
+            pages_next = lookup(1);
+        }
+        // block i of this wave's in tile `it`: whether of K, its first key, its source
+        auto key_side = [&](int i) { return w + i * NW < BPT; };
+        auto first_key = [&](int it, int i) __attribute__((always_inline)) {
+            return min((t0 + it) * KT + 16 * ((w + i * NW) & (BPT - 1)), (len - 1) & ~15);
+        };
+        auto source = [&](int it, int i) __attribute__((always_inline)) {
+            const int64_t row = __builtin_amdgcn_readlane(rows_now, it % TPG * BPT + ((w + i * NW) & (BPT - 1)));
             return uniform(key_side(i) ? kh + row * (2 * k_rs) : vh + row * (2 * v_rs));
+        };
+        auto next_rows = [&](int it) __attribute__((always_inline)) {      // before a tile's sources are taken
+            if (it % TPG == 0 && it > 0) {
+                rows_now = cache_row(pages_next, it / TPG);
+                pages_next = lookup(it / TPG + 1);
+            }
+        };
+        auto lane_off = [&](int i, int j) __attribute__((always_inline)) {
+            uint32_t c = chunk0;                       // (one add per use, not a register held per load)
+            asm volatile("" : "+v"(c));
+            return (c ^ (uint32_t)(row_swz<D>(j * LR) * 16)) + lane_row[NU > 1 ? (i >= NU / 2) : 0];
         };
         auto stage = [&](int it) __attribute__((always_inline)) {
             char* buf = smem + it % NBUF * STAGE;
+            next_rows(it);
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 const int key = first_key(it, i), rmax = len - 1 - key;
-                const char* src = source(key, i);
+                const char* src = source(it, i);
                 char* dst = buf + (w + i * NW) * NI * 1024;
+                const uint32_t rs2 = (uint32_t)(2 * (key_side(i) ? k_rs : v_rs));
                 if (rmax >= 15) {
 #pragma unroll
-                    for (int j = 0; j < NI; ++j) lds_dma16s(src, off[NU > 1 ? i / (NU > 1 ? NU / 2 : 1) : 0][j], dst + j * 1024);
+                    for (int j = 0; j < NI; ++j) lds_dma16s(src + j * LR * (int64_t)rs2, lane_off(i, j), dst + j * 1024);
                 } else {
-                    const uint32_t rs2 = (uint32_t)(2 * (key_side(i) ? k_rs : v_rs));
 #pragma unroll
                     for (int j = 0; j < NI; ++j)
                         lds_dma16s(src, St::lane_off(j, lane, min(St::row_of(j, lane), rmax), rs2), dst + j * 1024);
@@ -300,8 +383,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
         const float c2 = p->scale_log2;
 
         // sums: of the rounded weights (l_run) and of the weights (x_run)
+        if (threadIdx.x == 0) s_odd = 0;               // a value of V in the tree's tiles is not finite
         float m_run = kNegInf, l_run = 0.f, x_run = 0.f;
-        uint32_t odd = 0;                              // a value of V in the tree's tiles was not finite
         f32x16_t oacc[DB];
 #pragma unroll
         for (int db = 0; db < DB; ++db) oacc[db] = f32x16_t{};
@@ -322,9 +405,11 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
             auto products = [&](auto with_loads) __attribute__((always_inline)) {
                 const char* src[NU];
                 char* dst = smem + (it + AHEAD) % NBUF * STAGE + w * NI * 1024;
-                if (decltype(with_loads)::value)
+                if (decltype(with_loads)::value) {
+                    next_rows(it + AHEAD);
 #pragma unroll
-                    for (int i = 0; i < NU; ++i) src[i] = source(first_key(it + AHEAD, i), i);
+                    for (int i = 0; i < NU; ++i) src[i] = source(it + AHEAD, i);
+                }
                 u32x4_t ka[NS];
 #pragma unroll
                 for (int i = 0; i < 4 && i < NS; ++i) ka[i] = row_operand<D>(kb_, i / NKB, 32 * (i % NKB));
@@ -337,7 +422,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
                         constexpr int E = NS / LOADS;          // products per load
                         if (i % E == E - 1 && i / E < LOADS) {
                             const int x = i / E / NI, j = i / E % NI;
-                            lds_dma16s(src[x], off[NU > 1 ? x / (NU > 1 ? NU / 2 : 1) : 0][j], dst + (x * NW * NI + j) * 1024);
+                            lds_dma16s(src[x] + j * LR * (2 * (key_side(x) ? k_rs : v_rs)), lane_off(x, j),
+                                       dst + (x * NW * NI + j) * 1024);
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -390,22 +476,30 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
                     pf[c][j] = T::pack2(a, b);
                     l_run = dot2_ones<T>(pf[c][j], l_run);
                 }
+            if constexpr (MASKED) {
+                // this wave's share of the tile's V: what is not finite leaves the tile, and is
+                // added below to the rows that see it
+                char* vs = smem + it % NBUF * STAGE + TILE + w * (TILE / NW) + lane * 16;
+#pragma unroll
+                for (int i = 0; i < TILE / NW / 1024; ++i) {
+                    u32x4_t v = ld16(vs + i * 1024);
+                    u16x2_t top{};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, v[j] & 0x7fff7fffu));
+                    if (max(top[0], top[1]) >= kInf16<T>) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] &= finite_halves<T>(v[j]);
+                        st16(vs + i * 1024, v);
+                        s_odd = 1;
+                    }
+                }
+                __syncthreads();
+            }
 #pragma unroll
             for (int c = 0; c < NPC; ++c)
 #pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    u32x4_t v = tr_operand<D>(vtb, c, db);
-                    if constexpr (MASKED) {
-                        // what is not finite is left out here, and added below to the rows that see it
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t keep = finite_halves<T>(v[j]);
-                            odd |= ~keep;
-                            v[j] &= keep;
-                        }
-                    }
-                    oacc[db] = mfma32<T>(v, pf[c], oacc[db]);
-                }
+                for (int db = 0; db < DB; ++db) oacc[db] = mfma32<T>(tr_operand<D>(vtb, c, db), pf[c], oacc[db]);
         };
         if (AHEAD > 1 && n_tiles > 1) stage(1);
         // tiles that end before the tree
@@ -416,7 +510,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
 #pragma unroll 1
         for (; it < n_tiles; ++it) step(it, std::true_type{});
 
-        if (__any(odd != 0)) {
+        if (plain < n_tiles && uniform(s_odd) != 0) {
             // infinities and NaN of this wave's keys in the tree's tiles, one key after the
             // other, from the cache
             const uint32_t* words = s_mask[tok - tok0];
@@ -482,13 +576,18 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
                 }
             }
         }
-        // (NaN is not <= 0; rows that see nothing: 0 and -inf)
-        if (kw == 0 && row < n_rows) {
+        // (the row again, from the lane: nothing of it is held through the loops; NaN is not
+        // <= 0; rows that see nothing: 0 and -inf)
+        int l2 = l32;
+        asm volatile("" : "+v"(l2));
+        const int orow = rt * ROWS + 32 * rw + l2;
+        if (kw == 0 && orow < n_rows) {
             CParams* p2 = params();
+            const int otok = orow / p2->g, ohead = hk * p2->g + orow - otok * p2->g;
             const float inv = !(lt <= 0.f) ? 1.f / lt : 0.f;
             const float lse = !(xt <= 0.f) ? m_run * kLn2 + logf(xt) : kNegInf;
             if (whole) {
-                const int64_t rh = (int64_t)(q0 + tok) * p2->hq + head;
+                const int64_t rh = (int64_t)(q0 + otok) * p2->hq + ohead;
                 uint16_t* op = p2->o + rh * D;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
@@ -499,7 +598,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
                                     T::pack2(oacc[db][4 * rg + 2] * inv, oacc[db][4 * rg + 3] * inv)});
                 if (p2->lse != nullptr && hi == 0) p2->lse[rh] = lse;
             } else {
-                const int64_t pr = (int64_t)(2 * id + (t0 == 0 ? 1 : 0)) * ROWS + 32 * rw + l32;
+                const int64_t pr = (int64_t)(2 * id + (t0 == 0 ? 1 : 0)) * ROWS + 32 * rw + l2;
                 float* op = p2->part_o + pr * D;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
@@ -530,7 +629,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeKParams p) {
     const int row = d.z * ROWS + rr, n = d.w;
     if (n == 0 || row >= d.y) return;
     // piece z of the unit: the first one's second place, the others' first
-    auto place = [&](int z) { return ((int64_t)2 * (id + (int64_t)z * p.hkv) + (z == 0 ? 1 : 0)) * ROWS + rr; };
+    auto place = [&](int z) { return (2 * (id + (int64_t)z * p.hkv * p.side) + (z == 0 ? 1 : 0)) * ROWS + rr; };
     float m = kNegInf, sum = 0.f;
     fe_t acc{};
     for (int z0 = 0; z0 < n; z0 += U) {
@@ -559,7 +658,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeKParams p) {
         }
     }
     const float inv = !(sum <= 0.f) ? 1.f / sum : 0.f;
-    const int tok = row / p.g, head = id % p.hkv * p.g + row - tok * p.g;
+    const int tok = row / p.g, head = id / p.side % p.hkv * p.g + row - tok * p.g;
     const int64_t rh = (int64_t)(d.x + tok) * p.hq + head;
     uint32_t* out = reinterpret_cast<uint32_t*>(p.o + rh * D + NE * l32);
 #pragma unroll
@@ -572,7 +671,8 @@ hipError_t launch_rows(const TreeArgs& a, TreeKParams p, hipStream_t st) {
     constexpr int ROWS = 32 * RW;
     char* ws = (char*)a.workspace;
     p.pieces = a.plan.pieces;
-    const size_t grid = (size_t)p.pieces * p.hkv;
+    p.side = a.plan.side;
+    const size_t grid = (size_t)p.pieces * p.hkv * p.side;
     p.desc = (int4*)ws;
     p.part_lse = (float*)(ws + grid * sizeof(int4));
     p.part_o = p.part_lse + grid * 2 * ROWS;
@@ -600,9 +700,10 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
     p.scale_log2 = (g.scale == 0.f ? 1.f : fabsf(g.scale)) * kLog2e;
     p.q_and = g.scale == 0.f ? 0u : ~0u;
     p.q_xor = g.scale < 0.f ? 0x80008000u : 0u;
-    if (a.plan.rows == 32) return launch_rows<T, D, 4, 1, 128, 2>(a, p, st);
-    if (a.plan.rows == 64) return launch_rows<T, D, 4, 2, 64, 2>(a, p, st);
-    return launch_rows<T, D, 4, 4, 64, 2>(a, p, st);
+    if (a.plan.rows == 32) return launch_rows<T, D, A32>(a, p, st);
+    if (a.plan.rows == 64) return launch_rows<T, D, A64>(a, p, st);
+    if (a.plan.rows == 256) return launch_rows<T, D, A256>(a, p, st);
+    return launch_rows<T, D, A128>(a, p, st);
 }
 
 }  // namespace
@@ -610,14 +711,19 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
 TreePlan make_tree_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
     TreePlan plan;
     const int64_t rows = (int64_t)std::max(max_q, 1) * g.g;
-    plan.rows = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    const int kt = plan.rows == 32 ? 128 : 64;
+    plan.rows = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    const int kt = plan.rows == 32 ? K32 : plan.rows == 64 ? K64 : plan.rows == 128 ? K128 : 128;
+    // row tiles of a head side by side, where most sequences have that many
+    const int64_t most = (rows + plan.rows - 1) / plan.rows;
+    const int64_t usual = ((g.total_q * g.g + g.num_seqs - 1) / g.num_seqs + plan.rows - 1) / plan.rows;
+    plan.side = most <= 8 && 4 * usual >= 3 * most ? (int)most : 1;
     // as many pieces as the GPU holds workgroups for, or as there are tiles by the bounds
-    const int64_t full = std::max<int64_t>(1, (int64_t)cus * (plan.rows == 32 && g.d == 128 ? 1 : 2) / g.hkv);
-    const int64_t units = (int64_t)g.num_seqs * ((rows + plan.rows - 1) / plan.rows);
+    const int64_t held = (int64_t)cus * (plan.rows == 32 ? H32 : plan.rows == 64 ? (g.d == 64 ? LB64 : H64) : plan.rows == 128 ? (g.d == 64 ? LB64 : H128) : 1);
+    const int64_t full = std::max<int64_t>(1, held / ((int64_t)g.hkv * plan.side));
+    const int64_t units = (int64_t)g.num_seqs * ((most + plan.side - 1) / plan.side);
     const int64_t tiles = std::max<int64_t>(1, (max_kv + kt - 1) / kt);
     plan.pieces = (int)(units >= full ? full : std::min(full, units * tiles));
-    plan.bytes = (size_t)plan.pieces * g.hkv * (16 + 2 * (size_t)plan.rows * ((size_t)g.d + 1) * sizeof(float));
+    plan.bytes = (size_t)plan.pieces * g.hkv * plan.side * (16 + 2 * (size_t)plan.rows * ((size_t)g.d + 1) * sizeof(float));
     return plan;
 }
 
