@@ -59,6 +59,11 @@ namespace {
 
 constexpr int kMaskWords = kTreeMaxCols / 32 + 1;      // of a token's mask; the last one is 0
 constexpr int kMinPiece = 1;                           // shortest piece, in tiles
+// Beginning a unit after another one in a piece takes as long as this many tiles (the last
+// stores, a page lookup and the first tile's loads, one after the other: about 8 us where the GPU
+// streams, a tile of 32 KB per workgroup 3 us).
+template <int D, int KT>
+constexpr int kUnitCost = D * KT <= 4096 ? 4 : 3;
 
 struct TreeKParams {
     const uint16_t* q; const uint16_t* k; const uint16_t* v;
@@ -98,7 +103,7 @@ struct SeqWork {
     int q0, n, len, tiles, rounds;
     int64_t work;
 };
-template <int ROWS, int KT>
+template <int D, int ROWS, int KT>
 __device__ inline SeqWork seq_work(CParams* p, int s) {
     const SeqRange r = seq_range(p->cu_q, s, p->total_q);
     SeqWork w;
@@ -107,7 +112,7 @@ __device__ inline SeqWork seq_work(CParams* p, int s) {
     w.len = kv_length(p->cu_kv, s);
     w.tiles = max(1, (w.len + KT - 1) / KT);           // (without keys: rows of 0)
     w.rounds = ((w.n * p->g + ROWS - 1) / ROWS + p->side - 1) / p->side;
-    w.work = (int64_t)w.tiles * w.rounds;
+    w.work = (int64_t)(w.tiles + kUnitCost<D, KT>) * w.rounds;
     return w;
 }
 __device__ inline int64_t lane_value64(int64_t x, int l) {
@@ -220,11 +225,11 @@ __global__ __launch_bounds__(NW * 64, NW <= 4 && NBUF * KT * D * 4 <= 40 * 1024 
         piece_id = uniform(col / p->hkv);
         hk = col - piece_id * p->hkv;
         const int n = p->num_seqs;
-        const SeqWork first = seq_work<ROWS, KT>(p, min(lane, n - 1));
+        const SeqWork first = seq_work<D, ROWS, KT>(p, min(lane, n - 1));
         const int64_t sum0 = wave_scan64(lane < n ? first.work : 0, lane);
         int64_t total = lane_value64(sum0, 63);
         for (int g0 = 64; g0 < n; g0 += 64) {
-            const SeqWork x = seq_work<ROWS, KT>(p, min(g0 + lane, n - 1));
+            const SeqWork x = seq_work<D, ROWS, KT>(p, min(g0 + lane, n - 1));
             total += lane_value64(wave_scan64(g0 + lane < n ? x.work : 0, lane), 63);
         }
         piece = max((int64_t)kMinPiece, quotient(total + p->pieces - 1, p->pieces));
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(NW * 64, NW <= 4 && NBUF * KT * D * 4 <= 40 * 1024 
             int64_t sum = sum0;
             sw = first;
             if (g0 > 0) {
-                sw = seq_work<ROWS, KT>(p, min(g0 + lane, n - 1));
+                sw = seq_work<D, ROWS, KT>(p, min(g0 + lane, n - 1));
                 sum = wave_scan64(g0 + lane < n ? sw.work : 0, lane);
             }
             const uint64_t past = __ballot(g0 + lane < n && base + sum > at);
@@ -282,20 +287,22 @@ __global__ __launch_bounds__(NW * 64, NW <= 4 && NBUF * KT * D * 4 <= 40 * 1024 
         if (at >= base + sw.work) {                    // (this sequence is done, or has no queries)
             base += sw.work;
             if (++s >= p->num_seqs) break;
-            sw = seq_work<ROWS, KT>(p, s);
+            sw = seq_work<D, ROWS, KT>(p, s);
             continue;
         }
-        const int round = uniform((int)quotient(at - base, sw.tiles)), rt = round * p->side + rt0;
-        const int t0 = uniform((int)(at - base - (int64_t)round * sw.tiles));
-        const int t1 = uniform((int)min((int64_t)sw.tiles, t0 + (end - at)));
+        // (the line has kUnitCost places before a unit's tiles: a piece that begins a unit
+        // after another one gets fewer tiles)
+        const int len_v = sw.tiles + kUnitCost<D, KT>, round = uniform((int)quotient(at - base, len_v)), rt = round * p->side + rt0;
+        const int64_t unit_at = base + (int64_t)round * len_v + kUnitCost<D, KT>;     // the unit's first tile
+        const int t0 = uniform((int)max(at - unit_at, (int64_t)0));
+        const int t1 = uniform((int)(min(unit_at + sw.tiles, end) - unit_at));
         const int len = uniform(sw.len), ctx = len - uniform(sw.n), n_rows = uniform(sw.n) * p->g, q0 = uniform(sw.q0);
         const bool whole = t0 == 0 && t1 == sw.tiles;
-        if ((int64_t)rt * ROWS >= n_rows) {            // (the last round has fewer row tiles)
-            at += t1 - t0;
-            continue;
-        }
-        if (t0 == 0 && !whole) begun = int4{q0, n_rows, rt, (int)quotient(at + sw.tiles - 1, piece) - piece_id + 1};
-        at += t1 - t0;
+        at = min(unit_at + sw.tiles, end);
+        // (a piece that ends before the first tile; the last round has fewer row tiles)
+        if (t1 <= 0 || (int64_t)rt * ROWS >= n_rows) continue;
+        if (t0 == 0 && !whole)
+            begun = int4{q0, n_rows, rt, (int)quotient(unit_at + sw.tiles - 1, piece) - piece_id + 1};
 
         // 16 keys of a tile at a time; past the last key, its block again, rows that repeat it
         const int n_tiles = len > 0 ? t1 - t0 : 0;
@@ -618,7 +625,8 @@ __global__ __launch_bounds__(NW * 64, NW <= 4 && NBUF * KT * D * 4 <= 40 * 1024 
 // The rows of a unit that several pieces share: half a wave per row, its lanes over
 // the head dim, O = sum_z w_z O_z / sum_z w_z, w_z = exp(lse_z - max lse), in the
 // pieces' order. Bound by the latency of its loads: the rows of 8 pieces are under way
-// before their weights are known.
+// before their weights are known. (Two or four rows per half wave, for fewer workgroups: 2
+// and 4 us slower over 11 pieces.)
 template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeKParams p) {
     constexpr int NE = D / 32, U = 8;                  // columns of a lane, pieces at a time
