@@ -295,6 +295,7 @@ __global__ __launch_bounds__(kWaves * 64) void rope_kernel(RopeKParams p) {
 // weights' gradients are (e(j): the element of value j, -1: none).
 template <int N, typename E>
 __device__ inline void store_part(const RopeKParams& p, float* s_sum, const float (&acc)[2][N], E e, bool first, int w) {
+#pragma unroll
     for (int side = 0; side < 2; ++side) {
         for (int i = 0; i < kWaves; ++i) {             // (in the order of the waves)
             __syncthreads();
@@ -312,8 +313,9 @@ __device__ inline void store_part(const RopeKParams& p, float* s_sum, const floa
 }
 
 // Backward with norms, on the same units: dy and x in, dx out. A wave goes through
-// every (workgroups * kWaves)-th token, its share of dw in registers; one more
-// launch adds the workgroups' sums (no atomics: the same result every time).
+// every (workgroups * kWaves)-th token, the passes over its query heads, then over its
+// kv heads, the next pass's rows under way meanwhile; its share of dw stays in registers,
+// and one more launch adds the workgroups' sums (no atomics: the same result every time).
 template <typename T, bool INTER>
 __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
     __shared__ __attribute__((aligned(16))) float s_tab[kWaves][kMaxD];
@@ -329,33 +331,52 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
         s_w[side * kMaxD + i - side * p.d] = weight_at(p, side, i - side * p.d);
     }
     __syncthreads();
+    const int q_passes = (p.hq + hpw - 1) / hpw, passes = q_passes + (p.hkv + hpw - 1) / hpw;
+    struct Rows {
+        Row8<T> ga, gb, xa, xb;
+    };
+    auto head_of = [&](int pass) { return (pass < q_passes ? pass : pass - q_passes) * hpw + hl; };
+    auto load = [&](int64_t token, int pass, Rows& r) {
+        const int side = pass < q_passes ? 0 : 1, hd = head_of(pass);
+        r.ga.clear(); r.gb.clear(); r.xa.clear(); r.xb.clear();
+        if (unit && hd < (side == 0 ? p.hq : p.hkv)) {
+            const typename T::raw* g = (const typename T::raw*)p.in[side] + token * p.in_rs[side] + (int64_t)hd * p.d;
+            const typename T::raw* x = (const typename T::raw*)p.x[side] + token * p.x_rs[side] + (int64_t)hd * p.d;
+            r.ga.load(g + ea);
+            r.gb.load(g + eb);
+            r.xa.load(x + ea);
+            r.xb.load(x + eb);
+        }
+    };
     float dw[2][16] = {};
     const int64_t step = (int64_t)gridDim.x * kWaves;
-    for (int64_t token = (int64_t)blockIdx.x * kWaves + w; token < p.total; token += step) {
+    int64_t token = (int64_t)blockIdx.x * kWaves + w;
+    Rows now;
+    int pos = 0;
+    if (token < p.total) {
+        load(token, 0, now);
+        if (p.rot > 0) pos = p.positions[token];
+    }
+    while (token < p.total) {
         float cs[8], sn[8];
         if (p.rot > 0) {
             __builtin_amdgcn_wave_barrier();
-            wave_table(p, s_tab[w], p.positions[token], lane);
+            wave_table(p, s_tab[w], pos, lane);
             table_of(s_tab[w], u, p.rot, cs, sn);
+            pos = p.positions[min(token + step, p.total - 1)];
         }
-        for (int h0 = 0; h0 < p.heads; h0 += hpw) {
-            const int head = h0 + hl, side = head < p.hq ? 0 : 1, hd = head - side * p.hq;
-            const bool ok = unit && head < p.heads;
-            Row8<T> ga, gb, xa, xb;
-            ga.clear(); gb.clear(); xa.clear(); xb.clear();
-            if (ok) {
-                const typename T::raw* g = (const typename T::raw*)p.in[side] + token * p.in_rs[side] + (int64_t)hd * p.d;
-                const typename T::raw* x = (const typename T::raw*)p.x[side] + token * p.x_rs[side] + (int64_t)hd * p.d;
-                ga.load(g + ea);
-                gb.load(g + eb);
-                xa.load(x + ea);
-                xb.load(x + eb);
-            }
+#pragma unroll 1
+        for (int pass = 0; pass < passes; ++pass) {
+            const bool last = pass + 1 == passes;
+            const int64_t next = last ? token + step : token;
+            Rows then;
+            if (next < p.total) load(next, last ? 0 : pass + 1, then);
+            const int side = pass < q_passes ? 0 : 1, hd = head_of(pass);
             float va[8], vb[8], fa[8], fb[8];
-            ga.get(va);
-            gb.get(vb);
-            xa.get(fa);
-            xb.get(fb);
+            now.ga.get(va);
+            now.gb.get(vb);
+            now.xa.get(fa);
+            now.xb.get(fb);
             if (turns) rotate<INTER>(va, vb, cs, sn);
             const float* wt = s_w + side * kMaxD;
             float sum = 0.f, dot = 0.f;
@@ -373,23 +394,30 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
             }
             const float r = 1.f / sqrtf(fmaf(sum, p.inv_d, p.eps));
             const float m = dot * r * p.inv_d * r;                     // mean(w g xn) r
+            auto add = [&](float (&d)[16]) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    d[j] = fmaf(va[j], fa[j] * r, d[j]);
+                    d[8 + j] = fmaf(vb[j], fb[j] * r, d[8 + j]);
+                }
+            };
+            if (side == 0) add(dw[0]);
+            else add(dw[1]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float da = va[j] * (fa[j] * r), db = vb[j] * (fb[j] * r);
-                dw[0][j] += side == 0 ? da : 0.f;
-                dw[0][8 + j] += side == 0 ? db : 0.f;
-                dw[1][j] += side == 1 ? da : 0.f;
-                dw[1][8 + j] += side == 1 ? db : 0.f;
                 va[j] = r * fmaf(va[j], wa[j], -fa[j] * m);
                 vb[j] = r * fmaf(vb[j], wb[j], -fb[j] * m);
             }
-            if (!ok) continue;
-            ga.set(va);
-            gb.set(vb);
-            typename T::raw* y = (typename T::raw*)p.out[side] + token * p.out_rs[side] + (int64_t)hd * p.d;
-            ga.store(y + ea);
-            gb.store(y + eb);
+            if (unit && hd < (side == 0 ? p.hq : p.hkv)) {
+                now.ga.set(va);
+                now.gb.set(vb);
+                typename T::raw* y = (typename T::raw*)p.out[side] + token * p.out_rs[side] + (int64_t)hd * p.d;
+                now.ga.store(y + ea);
+                now.gb.store(y + eb);
+            }
+            now = then;
         }
+        token += step;
     }
     if (p.part == nullptr) return;
 #pragma unroll
@@ -499,24 +527,28 @@ __global__ __launch_bounds__(kWaves * 64) void rope_any_kernel(RopeKParams p, bo
         store_part<2 * NS>(p, s_sum, dw, [&](int j) { return j < NS ? ia[j] : ib[j - NS]; }, true, w);
 }
 
-// dw: the workgroups' sums, in their order within 16 interleaved runs, in 64 bits.
+// dw: the workgroups' sums, in their order within 64 interleaved runs and then by
+// halves, in 64 bits; 4 columns a workgroup, so that all loads are under way at once.
 __global__ __launch_bounds__(256) void rope_dw_kernel(const float* part, int n, int d, int w_code, void* dq, void* dk) {
-    __shared__ double s_sum[16][16];
-    const int c = threadIdx.x & 15, run = threadIdx.x >> 4, i = blockIdx.x * 16 + c;
+    __shared__ double s_sum[64][4];
+    const int c = threadIdx.x & 3, run = threadIdx.x >> 2, i = blockIdx.x * 4 + c;
     double sum = 0.;
     if (i < 2 * d) {
 #pragma unroll 8
-        for (int g = run; g < n; g += 16) sum += (double)part[(int64_t)g * 2 * d + i];
+        for (int g = run; g < n; g += 64) sum += (double)part[(int64_t)g * 2 * d + i];
     }
     s_sum[run][c] = sum;
-    __syncthreads();
+    for (int h = 32; h > 0; h >>= 1) {
+        __syncthreads();
+        if (run < h) s_sum[run][c] += s_sum[run + h][c];
+    }
     if (run != 0 || i >= 2 * d) return;
-    for (int k = 1; k < 16; ++k) sum += s_sum[k][c];
+    const float x = (float)s_sum[0][c];
     void* out = i < d ? dq : dk;
     const int e = i < d ? i : i - d;
     if (out == nullptr) return;
-    if (w_code == F32::code) ((float*)out)[e] = (float)sum;
-    else ((uint16_t*)out)[e] = w_code == BF16::code ? BF16::from_float((float)sum) : F16::from_float((float)sum);
+    if (w_code == F32::code) ((float*)out)[e] = x;
+    else ((uint16_t*)out)[e] = w_code == BF16::code ? BF16::from_float(x) : F16::from_float(x);
 }
 
 RopeKParams params(const RopeArgs& a) {
@@ -581,6 +613,9 @@ hipError_t launch_units(RopeKParams p, int passes, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Two passes per wave from 8192 passes on (2048 tokens of 32/8 heads, D = 128, bf16: 8.1 us, with
+// one 8.3; 16384 appended tokens with norms 84 against 87), one below, for the waves (1024
+// tokens 4.9 us, with two 5.0; 16 tokens with norms 3.3 against 4.1). More than two were slower.
 template <typename T, bool INTER, bool NORM, bool APPEND>
 hipError_t launch_passes(const RopeKParams& p, hipStream_t st) {
     const int hpw = 64 >> p.units_log2, passes = (p.heads + hpw - 1) / hpw;
@@ -617,7 +652,7 @@ hipError_t launch_typed(const RopeArgs& a, hipStream_t st) {
         if (e != hipSuccess) return e;
     }
     if (norm_bwd && (a.dw[0] != nullptr || a.dw[1] != nullptr)) {
-        hipLaunchKernelGGL(rope_dw_kernel, dim3((unsigned)((2 * a.d + 15) / 16)), dim3(256), 0, st, a.part,
+        hipLaunchKernelGGL(rope_dw_kernel, dim3((unsigned)((2 * a.d + 3) / 4)), dim3(256), 0, st, a.part,
                            a.total > 0 ? a.part_wgs : 0, a.d, a.w_dtype, a.dw[0], a.dw[1]);
     }
     return hipGetLastError();
@@ -625,8 +660,10 @@ hipError_t launch_typed(const RopeArgs& a, hipStream_t st) {
 
 }  // namespace
 
+// Two workgroups per CU, which its registers hold at every type, in one round (16384 tokens
+// of 32/8 heads, D = 128, bf16: 108 us; three per CU 114, four 133, six 126).
 int rope_part_wgs(int64_t total) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>((total + kWaves - 1) / kWaves, 1024));
+    return (int)std::max<int64_t>(1, std::min<int64_t>((total + kWaves - 1) / kWaves, 2 * (int64_t)device_cus()));
 }
 
 hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st) {

@@ -34,25 +34,6 @@
 #include "kernels.h"
 #include "../../include/mtlattn_capi.h"
 
-#ifndef LB64
-#define LB64 2
-#endif
-#ifndef A32
-#define A32 4, 1, 128, 2
-#define H32 1
-#define K32 128
-#endif
-#ifndef A64
-#define A64 4, 2, 64, 2
-#define H64 2
-#define K64 64
-#endif
-#ifndef A128
-#define A128 4, 4, 64, 2
-#define H128 2
-#define K128 64
-#endif
-#define A256 8, 8, 128, 2
 namespace mtlattn {
 
 namespace {
@@ -190,7 +171,7 @@ __device__ inline void load_masks(CParams* p, uint32_t (*s_mask)[kMaskWords], in
 }
 
 template <typename T, int D, int NW, int RW, int KT, int NBUF>
-__global__ __launch_bounds__(NW * 64, NW <= 4 && NBUF * KT * D * 4 <= 40 * 1024 ? LB64 : NW <= 4 && NBUF * KT * D * 4 <= 72 * 1024 ? 2 : 1) void tree_kernel(TreeKParams) {
+__global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 ? 2 : 1) void tree_kernel(TreeKParams) {
     constexpr int KW = NW / RW, ROWS = 32 * RW;
     constexpr int NKB = KT / 32 / KW;                  // 32-key blocks of a wave
     constexpr int NPC = 2 * NKB;                       // 16-key chunks of P
@@ -708,25 +689,33 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
     p.scale_log2 = (g.scale == 0.f ? 1.f : fabsf(g.scale)) * kLog2e;
     p.q_and = g.scale == 0.f ? 0u : ~0u;
     p.q_xor = g.scale < 0.f ? 0x80008000u : 0u;
-    if (a.plan.rows == 32) return launch_rows<T, D, A32>(a, p, st);
-    if (a.plan.rows == 64) return launch_rows<T, D, A64>(a, p, st);
-    if (a.plan.rows == 256) return launch_rows<T, D, A256>(a, p, st);
-    return launch_rows<T, D, A128>(a, p, st);
+    if (a.plan.rows == 32) return launch_rows<T, D, 4, 1, 128, 2>(a, p, st);
+    if (a.plan.rows == 64) return launch_rows<T, D, 4, 2, 64, 2>(a, p, st);
+    if (a.plan.rows == 128) return launch_rows<T, D, 4, 4, 64, 2>(a, p, st);
+    return launch_rows<T, D, 8, 8, 128, 2>(a, p, st);
 }
 
 }  // namespace
 
+// Rows of a workgroup: the fewest that hold a sequence's max_q * g rows of a kv head,
+// so that the others' matrix work is not done for nothing, up to 256 (4 sequences of 64 drafted
+// tokens, 64/8 heads, 32768 to 98304 keys: 570 us with 256 rows, 790 with 128, which read the
+// cache twice as often). At D = 64 a long stream takes 64 rows at least, whose two workgroups
+// on a CU overlap better (12 sequences of 512 to 16384 keys, 16 heads, 8 tokens 94 -> 87 us, 32 sequences of
+// 1024 to 16384, 32/8 heads, 4 tokens 134 -> 123; 4 of 100 to 2000, 16 heads, 16 tokens 16 -> 19, which keep 32).
 TreePlan make_tree_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
     TreePlan plan;
     const int64_t rows = (int64_t)std::max(max_q, 1) * g.g;
-    plan.rows = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    const int kt = plan.rows == 32 ? K32 : plan.rows == 64 ? K64 : plan.rows == 128 ? K128 : 128;
+    const bool stream = (int64_t)g.num_seqs * g.hkv * ((max_kv + 127) / 128) > 16 * (int64_t)cus;
+    plan.rows = rows <= 32 && !(g.d == 64 && stream) ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    const int kt = plan.rows == 32 || plan.rows == 256 ? 128 : 64;
     // row tiles of a head side by side, where most sequences have that many
     const int64_t most = (rows + plan.rows - 1) / plan.rows;
     const int64_t usual = ((g.total_q * g.g + g.num_seqs - 1) / g.num_seqs + plan.rows - 1) / plan.rows;
     plan.side = most <= 8 && 4 * usual >= 3 * most ? (int)most : 1;
-    // as many pieces as the GPU holds workgroups for, or as there are tiles by the bounds
-    const int64_t held = (int64_t)cus * (plan.rows == 32 ? H32 : plan.rows == 64 ? (g.d == 64 ? LB64 : H64) : plan.rows == 128 ? (g.d == 64 ? LB64 : H128) : 1);
+    // as many pieces as the GPU holds workgroups for (the ring of two tiles fills a CU's LDS at 128
+    // keys and D = 128, half of it otherwise), or as there are tiles by the bounds
+    const int64_t held = (int64_t)cus * (plan.rows == 256 || (plan.rows == 32 && g.d == 128) ? 1 : 2);
     const int64_t full = std::max<int64_t>(1, held / ((int64_t)g.hkv * plan.side));
     const int64_t units = (int64_t)g.num_seqs * ((most + plan.side - 1) / plan.side);
     const int64_t tiles = std::max<int64_t>(1, (max_kv + kt - 1) / kt);
