@@ -1204,7 +1204,6 @@ int mtlattn_rotary_bwd(const mtlattn_rotary* r, const void* q, int64_t q_row_str
     if (need > 0 && (uintptr_t)workspace % 4 != 0)
         return fail(MTLATTN_ERR_WORKSPACE, "rotary_bwd: the workspace must be 4-byte aligned");
     a.part = (float*)workspace;
-    a.part_wgs = rope_part_wgs(r->total);
     a.dw[0] = dq_weight;
     a.dw[1] = dk_weight;
     return launch_status(launch_rope(r->dtype, a, (hipStream_t)stream), "rotation backward");

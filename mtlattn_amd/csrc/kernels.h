@@ -219,8 +219,8 @@ struct Cache8Args {
 // to the rows of a paged cache (out[1], out[2] are the caches, out_rs their token
 // strides; hq == 0: no queries), by offsets as in Cache8Args; positions null: the
 // token's place in its sequence. backward: in = gradients of the rotated rows, out
-// = those of x; with norms x holds the rows, part room for part_wgs * 2 * d floats
-// and dw (nullable) the weights' gradients.
+// = those of x; with norms x holds the rows, part room for rope_part_wgs(total) * 2 * d
+// floats and dw (nullable) the weights' gradients.
 struct RopeArgs {
     const void* in[3]; int64_t in_rs[3];
     void* out[3]; int64_t out_rs[3];
@@ -236,10 +236,9 @@ struct RopeArgs {
     int64_t bt_stride;
     int num_seqs, page_size, num_pages;
     float* part;
-    int part_wgs;
     void* dw[2];
 };
-int rope_part_wgs(int64_t total);
+int rope_part_wgs(int64_t total);             // the most workgroups that leave sums in part
 
 // Attention of drafted tokens' trees over a 16-bit paged cache (launch_tree): rows of
 // 32 to 256 per workgroup, `side` workgroups with other rows side by side, `pieces` of the work, workspace bytes.

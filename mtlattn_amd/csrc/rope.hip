@@ -428,103 +428,141 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
     store_part<16>(p, s_sum, dw, [&](int j) { return unit ? (j < 8 ? ea + j : eb + j - 8) : -1; }, hl == 0, w);
 }
 
-// Any D up to 256, any even R, rows of any alignment: one wave per head of a token,
-// a lane per pair or passing element, one element at a time. About a third of
-// the other kernel's rate.
+// Any D up to 256, any even R, rows of any alignment: a wave takes kAnyHeads heads of a
+// token, one after the other, a lane per pair or passing element, one element at a time;
+// the angles of the lane's pairs once per token. About a third of the other kernel's
+// rate (16384 tokens of 32/8 heads, D = 128, bf16: 194 us, with norms 242, their backward
+// 474; on aligned rows 62, 76 and 119).
+constexpr int kAnyHeads = 8;
 template <typename T, bool BWD>
 __global__ __launch_bounds__(kWaves * 64) void rope_any_kernel(RopeKParams p, bool append) {
-    constexpr int NS = kMaxD / 64;                     // slots of a lane: pairs, then single elements
+    constexpr int NS = kMaxD / 64;                     // slots of a lane: pairs (the first NP at most), then single elements
+    constexpr int NP = NS / 2;
     __shared__ float s_sum[kMaxD];
     using raw = typename T::raw;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int pairs = p.rot / 2, slots = p.d - pairs;
-    int ia[NS], ib[NS];                                // elements of a slot (ib -1: a single one, ia -1: none)
+    const int pairs = p.rot / 2, slots = p.d - pairs, groups = (p.heads + kAnyHeads - 1) / kAnyHeads;
+    int ia[NS], ib[NP];                                // elements of a slot (ib -1: a single one, ia -1: none)
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
         const int t = lane + 64 * j;
         ia[j] = t >= slots ? -1 : t >= pairs ? t + pairs : p.interleaved ? 2 * t : t;
-        ib[j] = t >= pairs ? -1 : p.interleaved ? 2 * t + 1 : t + pairs;
+        if (j < NP) ib[j] = t >= pairs ? -1 : p.interleaved ? 2 * t + 1 : t + pairs;
     }
-    float dw[2][2 * NS] = {};
-    const int64_t step = (int64_t)gridDim.x * kWaves, rows = p.total * p.heads;
-    for (int64_t item = (int64_t)blockIdx.x * kWaves + w; item < rows; item += step) {
-        const int64_t token = item / p.heads;
-        const int head = (int)(item - token * p.heads);
-        const int part = head < p.hq ? 0 : head < p.hq + p.hkv ? 1 : 2;
-        const int hd = head - (part == 0 ? 0 : part == 1 ? p.hq : p.hq + p.hkv);
+    float wa[2][NS] = {}, wb[2][NP] = {};
+    if (p.norm) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                if (p.weight[side] == nullptr) continue;
+                if (ia[j] >= 0) wa[side][j] = weight_at(p, side, ia[j]);
+                if (j < NP && ib[j] >= 0) wb[side][j] = weight_at(p, side, ib[j]);
+            }
+    }
+    float dw[2][NS + NP] = {};
+    const int64_t step = (int64_t)gridDim.x * kWaves, items = p.total * groups;
+    for (int64_t item = (int64_t)blockIdx.x * kWaves + w; item < items; item += step) {
+        const int64_t token = item / groups;
+        const int head0 = (int)(item - token * groups) * kAnyHeads, head1 = min(head0 + kAnyHeads, p.heads);
         Place at{true, 0, 0};
         if (append) at = find_place(p, (int)token, lane);
-        const int64_t row = append && part > 0 ? at.row : token;
-        if (row < 0) continue;
-        const raw* in = (const raw*)p.in[part] + token * p.in_rs[part] + (int64_t)hd * p.d;
-        raw* y = (raw*)p.out[part] + row * p.out_rs[part] + (int64_t)hd * p.d;
-        if (part == 2 || !at.owned) {
+        float cs[NP], sn[NP];
+        if (p.rot > 0) {
+            const int pos = p.positions != nullptr ? p.positions[token] : at.pos;
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+                if (ib[j] >= 0) turn(pos, p.inv_freq[lane + 64 * j], p.scale, p.sign, cs[j], sn[j]);
+        }
+#pragma unroll 2
+        for (int head = head0; head < head1; ++head) {
+            const int part = head < p.hq ? 0 : head < p.hq + p.hkv ? 1 : 2;
+            const int hd = head - (part == 0 ? 0 : part == 1 ? p.hq : p.hq + p.hkv);
+            const int64_t row = append && part > 0 ? at.row : token;
+            if (row < 0) continue;
+            const raw* in = (const raw*)p.in[part] + token * p.in_rs[part] + (int64_t)hd * p.d;
+            raw* y = (raw*)p.out[part] + row * p.out_rs[part] + (int64_t)hd * p.d;
+            const raw* xr = BWD ? (const raw*)p.x[part] + token * p.x_rs[part] + (int64_t)hd * p.d : nullptr;
+            raw ra[NS] = {}, rb[NP] = {}, xa[NS] = {}, xb[NP] = {};
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
-                if (ia[j] >= 0) y[ia[j]] = part == 2 ? in[ia[j]] : raw(0);
-                if (ib[j] >= 0) y[ib[j]] = part == 2 ? in[ib[j]] : raw(0);
+                if (ia[j] >= 0) ra[j] = in[ia[j]];
+                if (j < NP && ib[j] >= 0) rb[j] = in[ib[j]];
+                if (BWD && ia[j] >= 0) xa[j] = xr[ia[j]];
+                if (BWD && j < NP && ib[j] >= 0) xb[j] = xr[ib[j]];
             }
-            continue;
-        }
-        const int pos = p.rot == 0 ? 0 : p.positions != nullptr ? p.positions[token] : at.pos;
-        const raw* xr = BWD ? (const raw*)p.x[part] + token * p.x_rs[part] + (int64_t)hd * p.d : nullptr;
-        float va[NS], vb[NS], fa[NS], fb[NS], wa[NS], wb[NS];
-        float sum = 0.f;
+            if (part == 2 || !at.owned) {
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            va[j] = ia[j] >= 0 ? T::to_float(in[ia[j]]) : 0.f;
-            vb[j] = ib[j] >= 0 ? T::to_float(in[ib[j]]) : 0.f;
-            fa[j] = fb[j] = wa[j] = wb[j] = 0.f;
-            if (p.norm) {
-                if (ia[j] >= 0) wa[j] = weight_at(p, part, ia[j]);
-                if (ib[j] >= 0) wb[j] = weight_at(p, part, ib[j]);
-                fa[j] = BWD ? (ia[j] >= 0 ? T::to_float(xr[ia[j]]) : 0.f) : va[j];
-                fb[j] = BWD ? (ib[j] >= 0 ? T::to_float(xr[ib[j]]) : 0.f) : vb[j];
-                sum = fmaf(fa[j], fa[j], fmaf(fb[j], fb[j], sum));
+                for (int j = 0; j < NS; ++j) {
+                    if (ia[j] >= 0) y[ia[j]] = part == 2 ? ra[j] : raw(0);
+                    if (j < NP && ib[j] >= 0) y[ib[j]] = part == 2 ? rb[j] : raw(0);
+                }
+                continue;
             }
-        }
-        const float r = p.norm ? 1.f / sqrtf(fmaf(wave_sum(sum), p.inv_d, p.eps)) : 1.f;
-        if (!BWD && p.norm) {
+            float va[NS], vb[NP], fa[NS], fb[NP], sum = 0.f, r = 1.f;
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
-                va[j] *= r * wa[j];
-                vb[j] *= r * wb[j];
+                va[j] = T::to_float(ra[j]);
+                fa[j] = BWD ? T::to_float(xa[j]) : va[j];
+                sum = fmaf(fa[j], fa[j], sum);
+                if (j < NP) {
+                    vb[j] = T::to_float(rb[j]);
+                    fb[j] = BWD ? T::to_float(xb[j]) : vb[j];
+                    sum = fmaf(fb[j], fb[j], sum);
+                }
             }
-        }
+            if (p.norm) r = 1.f / sqrtf(fmaf(wave_sum(sum), p.inv_d, p.eps));
+            // (every path of a side in registers: the index is a constant)
+            auto w_a = [&](int j) { return part == 0 ? wa[0][j] : wa[1][j]; };
+            auto w_b = [&](int j) { return part == 0 ? wb[0][j] : wb[1][j]; };
+            if (!BWD && p.norm) {
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            if (ib[j] < 0) continue;
-            float c, s;
-            turn(pos, p.inv_freq[lane + 64 * j], p.scale, p.sign, c, s);
-            const float a = va[j], b = vb[j];
-            va[j] = fmaf(a, c, -b * s);
-            vb[j] = fmaf(b, c, a * s);
-        }
-        if (BWD) {
-            float dot = 0.f;
+                for (int j = 0; j < NS; ++j) {
+                    va[j] *= r * w_a(j);
+                    if (j < NP) vb[j] *= r * w_b(j);
+                }
+            }
 #pragma unroll
-            for (int j = 0; j < NS; ++j) dot = fmaf(va[j] * wa[j], fa[j], fmaf(vb[j] * wb[j], fb[j], dot));
-            const float m = wave_sum(dot) * r * p.inv_d * r;
+            for (int j = 0; j < NP; ++j) {
+                if (ib[j] < 0) continue;
+                const float a = va[j], b = vb[j];
+                va[j] = fmaf(a, cs[j], -b * sn[j]);
+                vb[j] = fmaf(b, cs[j], a * sn[j]);
+            }
+            if (BWD) {
+                float dot = 0.f;
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    dot = fmaf(va[j] * w_a(j), fa[j], dot);
+                    if (j < NP) dot = fmaf(vb[j] * w_b(j), fb[j], dot);
+                }
+                const float m = wave_sum(dot) * r * p.inv_d * r;
+                auto add = [&](float (&d)[NS + NP]) {
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        d[j] = fmaf(va[j], fa[j] * r, d[j]);
+                        if (j < NP) d[NS + j] = fmaf(vb[j], fb[j] * r, d[NS + j]);
+                    }
+                };
+                if (part == 0) add(dw[0]);
+                else add(dw[1]);
+#pragma unroll
+                for (int j = 0; j < NS; ++j) {
+                    va[j] = r * fmaf(va[j], w_a(j), -fa[j] * m);
+                    if (j < NP) vb[j] = r * fmaf(vb[j], w_b(j), -fb[j] * m);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
-                const float da = va[j] * (fa[j] * r), db = vb[j] * (fb[j] * r);
-                dw[0][j] += part == 0 ? da : 0.f;
-                dw[0][NS + j] += part == 0 ? db : 0.f;
-                dw[1][j] += part == 1 ? da : 0.f;
-                dw[1][NS + j] += part == 1 ? db : 0.f;
-                va[j] = r * fmaf(va[j], wa[j], -fa[j] * m);
-                vb[j] = r * fmaf(vb[j], wb[j], -fb[j] * m);
+                // (what passes without a norm keeps its bits)
+                const bool pair = j < NP && ib[j] >= 0;
+                if (ia[j] >= 0) y[ia[j]] = !pair && !p.norm ? ra[j] : T::from_float(va[j]);
+                if (pair) y[ib[j]] = T::from_float(vb[j]);
             }
-        }
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            // (what passes without a norm keeps its bits)
-            if (ia[j] >= 0) y[ia[j]] = ib[j] < 0 && !p.norm ? in[ia[j]] : T::from_float(va[j]);
-            if (ib[j] >= 0) y[ib[j]] = T::from_float(vb[j]);
         }
     }
     if (BWD && p.part != nullptr)
-        store_part<2 * NS>(p, s_sum, dw, [&](int j) { return j < NS ? ia[j] : ib[j - NS]; }, true, w);
+        store_part<NS + NP>(p, s_sum, dw, [&](int j) { return j < NS ? ia[j] : ib[j - NS]; }, true, w);
 }
 
 // dw: the workgroups' sums, in their order within 64 interleaved runs and then by
@@ -591,6 +629,17 @@ RopeKParams params(const RopeArgs& a) {
     return p;
 }
 
+// Workgroups of the backward with norms, in one round: two per CU of the unit kernel, which its
+// registers hold at every type (16384 tokens of 32/8 heads, D = 128, bf16: 108 us; three per
+// CU 114, four 133, six 126), five of the other one.
+int unit_part_wgs(int64_t total) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>((total + kWaves - 1) / kWaves, 2 * (int64_t)device_cus()));
+}
+int any_part_wgs(int64_t total, int heads) {
+    const int64_t items = total * ((heads + kAnyHeads - 1) / kAnyHeads);
+    return (int)std::max<int64_t>(1, std::min<int64_t>((items + kWaves - 1) / kWaves, 5 * (int64_t)device_cus()));
+}
+
 // Rows that the unit kernels take: 16-byte aligned, D and R multiples of 16.
 bool whole_units(const RopeArgs& a, int es) {
     if (a.d % 16 != 0 || a.rot % 16 != 0) return false;
@@ -626,16 +675,17 @@ hipError_t launch_passes(const RopeKParams& p, hipStream_t st) {
 template <typename T>
 hipError_t launch_typed(const RopeArgs& a, hipStream_t st) {
     RopeKParams p = params(a);
-    const bool norm_bwd = a.backward && p.norm;
-    const int es = sizeof(typename T::raw);
+    const bool norm_bwd = a.backward && p.norm, units = whole_units(a, sizeof(typename T::raw));
+    const int part_wgs = units ? unit_part_wgs(a.total) : any_part_wgs(a.total, p.heads);
     if (a.total > 0) {
-        if (!whole_units(a, es)) {
-            const int64_t wgs = norm_bwd ? a.part_wgs : std::min<int64_t>((a.total * p.heads + kWaves - 1) / kWaves, 1 << 20);
+        if (!units) {
+            const int64_t items = a.total * ((p.heads + kAnyHeads - 1) / kAnyHeads);
+            const int64_t wgs = norm_bwd ? part_wgs : std::min<int64_t>((items + kWaves - 1) / kWaves, 1 << 20);
             if (norm_bwd) hipLaunchKernelGGL((rope_any_kernel<T, true>), dim3((unsigned)wgs), dim3(kWaves * 64), 0, st, p, false);
             else hipLaunchKernelGGL((rope_any_kernel<T, false>), dim3((unsigned)wgs), dim3(kWaves * 64), 0, st, p, a.append);
         } else if (norm_bwd) {
-            if (a.interleaved) hipLaunchKernelGGL((rope_bwd_kernel<T, true>), dim3(a.part_wgs), dim3(kWaves * 64), 0, st, p);
-            else hipLaunchKernelGGL((rope_bwd_kernel<T, false>), dim3(a.part_wgs), dim3(kWaves * 64), 0, st, p);
+            if (a.interleaved) hipLaunchKernelGGL((rope_bwd_kernel<T, true>), dim3(part_wgs), dim3(kWaves * 64), 0, st, p);
+            else hipLaunchKernelGGL((rope_bwd_kernel<T, false>), dim3(part_wgs), dim3(kWaves * 64), 0, st, p);
         } else {
             hipError_t e;
             if (a.append) {
@@ -653,18 +703,14 @@ hipError_t launch_typed(const RopeArgs& a, hipStream_t st) {
     }
     if (norm_bwd && (a.dw[0] != nullptr || a.dw[1] != nullptr)) {
         hipLaunchKernelGGL(rope_dw_kernel, dim3((unsigned)((2 * a.d + 3) / 4)), dim3(256), 0, st, a.part,
-                           a.total > 0 ? a.part_wgs : 0, a.d, a.w_dtype, a.dw[0], a.dw[1]);
+                           a.total > 0 ? part_wgs : 0, a.d, a.w_dtype, a.dw[0], a.dw[1]);
     }
     return hipGetLastError();
 }
 
 }  // namespace
 
-// Two workgroups per CU, which its registers hold at every type, in one round (16384 tokens
-// of 32/8 heads, D = 128, bf16: 108 us; three per CU 114, four 133, six 126).
-int rope_part_wgs(int64_t total) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>((total + kWaves - 1) / kWaves, 2 * (int64_t)device_cus()));
-}
+int rope_part_wgs(int64_t total) { return any_part_wgs(total, 1 << 17); }
 
 hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st) {
     if (dtype == MTLATTN_DTYPE_BF16) return launch_typed<BF16>(a, st);
