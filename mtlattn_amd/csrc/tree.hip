@@ -41,10 +41,10 @@ namespace {
 constexpr int kMaskWords = kTreeMaxCols / 32 + 1;      // of a token's mask; the last one is 0
 constexpr int kMinPiece = 1;                           // shortest piece, in tiles
 // Beginning a unit after another one in a piece takes as long as this many tiles (the last
-// stores, a page lookup and the first tile's loads, one after the other: about 8 us where the GPU
-// streams, a tile of 32 KB per workgroup 3 us).
-template <int D, int KT>
-constexpr int kUnitCost = D * KT <= 4096 ? 4 : 3;
+// stores, a page lookup and the first tile's loads, one after the other, where the GPU streams:
+// 16 sequences of 8 to 32 drafted tokens over 128 to 4096 keys, 32/8 heads, D = 128: 46.3 us
+// without, 43.3 with 4; 12 of 512 to 16384 keys, 16 heads, D = 64: 93 and 88).
+constexpr int kUnitCost = 4;
 
 struct TreeKParams {
     const uint16_t* q; const uint16_t* k; const uint16_t* v;
@@ -93,7 +93,7 @@ __device__ inline SeqWork seq_work(CParams* p, int s) {
     w.len = kv_length(p->cu_kv, s);
     w.tiles = max(1, (w.len + KT - 1) / KT);           // (without keys: rows of 0)
     w.rounds = ((w.n * p->g + ROWS - 1) / ROWS + p->side - 1) / p->side;
-    w.work = (int64_t)(w.tiles + kUnitCost<D, KT>) * w.rounds;
+    w.work = (int64_t)(w.tiles + kUnitCost) * w.rounds;
     return w;
 }
 __device__ inline int64_t lane_value64(int64_t x, int l) {
@@ -273,8 +273,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
         }
         // (the line has kUnitCost places before a unit's tiles: a piece that begins a unit
         // after another one gets fewer tiles)
-        const int len_v = sw.tiles + kUnitCost<D, KT>, round = uniform((int)quotient(at - base, len_v)), rt = round * p->side + rt0;
-        const int64_t unit_at = base + (int64_t)round * len_v + kUnitCost<D, KT>;     // the unit's first tile
+        const int len_v = sw.tiles + kUnitCost, round = uniform((int)quotient(at - base, len_v)), rt = round * p->side + rt0;
+        const int64_t unit_at = base + (int64_t)round * len_v + kUnitCost;     // the unit's first tile
         const int t0 = uniform((int)max(at - unit_at, (int64_t)0));
         const int t1 = uniform((int)(min(unit_at + sw.tiles, end) - unit_at));
         const int len = uniform(sw.len), ctx = len - uniform(sw.n), n_rows = uniform(sw.n) * p->g, q0 = uniform(sw.q0);
@@ -484,10 +484,18 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
                 }
                 __syncthreads();
             }
+            // (the operand reads four products ahead)
+            constexpr int NV = NPC * DB;
+            u32x4_t va[NV];
 #pragma unroll
-            for (int c = 0; c < NPC; ++c)
+            for (int i = 0; i < 4; ++i) va[i] = tr_operand<D>(vtb, i / DB, i % DB);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int db = 0; db < DB; ++db) oacc[db] = mfma32<T>(tr_operand<D>(vtb, c, db), pf[c], oacc[db]);
+            for (int i = 0; i < NV; ++i) {
+                oacc[i % DB] = mfma32<T>(va[i], pf[i / DB], oacc[i % DB]);
+                if (i + 4 < NV) va[i + 4] = tr_operand<D>(vtb, (i + 4) / DB, (i + 4) % DB);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         if (AHEAD > 1 && n_tiles > 1) stage(1);
         // tiles that end before the tree
