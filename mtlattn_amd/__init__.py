@@ -311,9 +311,10 @@ def paged_tree_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_ta
     max_seqlen_q: the longest tree (any number; it shapes the launch, and so
     does max_seqlen_kv). scale defaults to 1/sqrt(D).
 
-    Rows that see nothing are 0 (LSE -inf). Nothing of a key that a row does
-    not see reaches it, infinities and NaN included. Forward only; the same
-    from run to run. Returns [Mq, Hq, D]."""
+    Rows that see nothing are 0 (LSE -inf); rows of no sequence are not
+    written. Nothing of a key that a row does not see reaches it, infinities
+    and NaN included. Forward only; the same from run to run. Returns
+    [Mq, Hq, D]."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return _C.paged_tree_decode(q, k_cache, v_cache, cu_seqlens_q.int(), cu_seqlens_kv.int(), block_table.int(),
@@ -338,6 +339,7 @@ class _RotaryFn(torch.autograd.Function):
         return _C.rotary(q, k, positions, inv_freq, interleaved, scale, q_weight, k_weight, eps)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, inv_freq, *rows = ctx.saved_tensors
         q, k, q_weight, k_weight = rows if ctx.normed else (dq, dk, None, None)
@@ -358,7 +360,9 @@ def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=Non
     q_weight, k_weight: [D] (fp32 or q's dtype), both or neither: heads are
     first divided by sqrt(mean(x^2) + eps) and multiplied by the weight.
     Angles are formed in 64 bits, everything else in fp32, rounded once to
-    q's dtype. Returns (q, k), contiguous."""
+    q's dtype. inv_freq is a constant. Returns (q, k), contiguous."""
+    if inv_freq.requires_grad:
+        raise NotImplementedError("mtlattn: differentiable frequencies (inv_freq.requires_grad) are not supported")
     args = (positions.int(), inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         if (q_weight is None) != (k_weight is None):

@@ -185,6 +185,8 @@ def test_python_refuses():
     q, k = torch.zeros(3, 2, 8), torch.zeros(3, 1, 8)
     with pytest.raises(RuntimeError, match="GPU"):
         mtlattn.rotary(q, k, torch.arange(3), torch.ones(4))
+    with pytest.raises(NotImplementedError, match="inv_freq"):
+        mtlattn.rotary(q, k, torch.arange(3), torch.ones(4, requires_grad=True))
     with pytest.raises(ValueError, match="together"):
         mtlattn.rotary(q.requires_grad_(), k, torch.arange(3), torch.ones(4), q_weight=torch.ones(8))
     with pytest.raises(RuntimeError, match="GPU"):

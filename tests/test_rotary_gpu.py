@@ -160,6 +160,27 @@ def test_one_output_alone(mt):
     assert bool(torch.isfinite(ql.grad).all()) and float(ql.grad.abs().max()) > 0 and float(w[0].grad.abs().max()) > 0
 
 
+def test_gradients_of_gradients_are_refused(mt):
+    g = torch.Generator().manual_seed(18)
+    q, k, _ = [t.cuda().requires_grad_() for t in rows(5, 4, 2, 64, F32, g)]
+    a, b = mt.rotary(q, k, torch.arange(5).cuda(), frequencies(64).cuda())
+    d, = torch.autograd.grad(a.square().sum() + b.sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        d.sum().backward()
+
+
+def test_rows_changed_before_the_backward_are_noticed(mt):
+    """Without norms the backward does not need the rows; with them a changed row raises."""
+    g = torch.Generator().manual_seed(19)
+    q, k, _ = [t.cuda() for t in rows(5, 4, 2, 64, F32, g)]
+    w = [x.cuda().requires_grad_() for x in weights(64, F32, g)]
+    f, pos = frequencies(64).cuda(), torch.arange(5).cuda()
+    a, _ = mt.rotary(q, k, pos, f, q_weight=w[0], k_weight=w[1])
+    q.mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        a.sum().backward()
+
+
 def test_no_rows(mt):
     f = frequencies(64).cuda()
     q = torch.empty(0, 4, 64, dtype=BF16, device="cuda", requires_grad=True)
@@ -360,6 +381,31 @@ def test_append_bad_offsets_stay_inside(mt):
     out = mt.paged_cache_append(k, v, caches[0], caches[1], cu, cu_kv, table, q=q, inv_freq=frequencies(64).cuda())
     torch.cuda.synchronize()
     assert bool(torch.isfinite(out.float()).all()) and bool(torch.isfinite(caches.float()).all())
+
+
+def test_append_rows_before_the_first_sequence(mt):
+    """Offsets that begin past row 0: the rows before them belong to nobody."""
+    g = torch.Generator().manual_seed(20)
+    q, k, v = rows(9, 4, 2, 64, BF16, g)
+    f = frequencies(64)
+    cu, kl, page = [2, 5, 8], [10, 3], 16
+    table = torch.tensor([[2], [0]], dtype=torch.int32)
+    caches = torch.zeros(2, 3, page, 2, 64, dtype=BF16, device="cuda")
+    out = mt.paged_cache_append(k.cuda(), v.cuda(), *caches, torch.tensor(cu).cuda(), torch.tensor([4, 14, 17]).cuda(),
+                                table.cuda(), q=q.cuda(), inv_freq=f.cuda())
+    pos = torch.tensor([0, 0, 7, 8, 9, 0, 1, 2, 0], dtype=torch.int32)
+    ref = [oracle.forward(x, pos, f) for x in (q, k)]
+    bounds = [forward_bound(x, r, f, False, 1.0, None, EPS, BF16) for x, r in zip((q, k), ref)]
+    mine = torch.tensor([False] * 2 + [True] * 6 + [False])
+    check(out[mine.cuda()], ref[0][mine], bounds[0][mine])
+    assert bool((out[~mine.cuda()] == 0).all())
+    flat = [c.flatten(0, 1).cpu() for c in caches]
+    at = torch.tensor([2 * page + 7, 2 * page + 8, 2 * page + 9, 0, 1, 2])
+    check(flat[0][at], ref[1][mine], bounds[1][mine])
+    assert torch.equal(flat[1][at], v[mine])
+    rest = torch.ones(3 * page, dtype=torch.bool)
+    rest[at] = False
+    assert all(bool((c[rest] == 0).all()) for c in flat)
 
 
 def test_append_refusals(mt):

@@ -82,6 +82,35 @@ def test_more_queries_than_tokens(mt):
     c.check(*c.run(mt))
 
 
+def test_more_tokens_than_a_mask_has_columns(mt):
+    """300 drafted tokens: those past the 256th column are seen by none."""
+    g = torch.Generator().manual_seed(17)
+    c = Case([300, 2], [333, 40], 4, 2, 64, 16, BF16, g, cols=256)
+    c.check(*c.run(mt))
+
+
+def test_rows_before_the_first_sequence(mt):
+    """Offsets that begin past row 0: the rows before them are left as they were."""
+    g = torch.Generator().manual_seed(18)
+    c = Case([3, 0, 6], [3, 0, 120], 4, 2, 64, 16, BF16, g, behind=2)
+    q = torch.cat((torch.full((2, 4, 64), math.nan).to(BF16), c.q))
+    mask = torch.cat((torch.zeros(2, c.cols, dtype=torch.bool), c.mask))
+    lse = torch.full((q.shape[0], 4), 7.0, device="cuda")
+    out = mt.paged_tree_decode(q.cuda(), c.k.cuda(), c.v.cuda(), cu_of(c.ql, "cuda") + 2, cu_of(c.kl, "cuda") + 5,
+                               c.table.cuda(), mask.cuda(), 6, 120, c.scale, lse)
+    assert bool((lse[:2] == 7.0).all())
+    c.check(out[2:], lse[2:])
+
+
+def test_one_mask_for_all_tokens(mt):
+    """A mask broadcast over the rows (a prefix mask)."""
+    g = torch.Generator().manual_seed(19)
+    c = Case([4, 4], [90, 4], 4, 2, 64, 16, F16, g)
+    row = torch.tensor([[True, True, False, True]])
+    c.mask = row.expand(8, 4)
+    c.check(*c.run(mt, mask=row.cuda().expand(8, 4)))
+
+
 def test_bounds_shape_the_launch_alone(mt):
     g = torch.Generator().manual_seed(4)
     c = Case([40, 3, 9], [900, 3, 77], 8, 2, 128, 16, BF16, g)
