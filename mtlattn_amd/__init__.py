@@ -324,29 +324,6 @@ def paged_tree_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_ta
 # ---- position rotation ----
 
 
-class _RotaryFn(torch.autograd.Function):
-    """Autograd node for rotary. Without norms the backward is the rotation
-    back and needs nothing of the forward; with them it recomputes the norms
-    from q and k."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, q_weight, k_weight, eps):
-        ctx.args = (interleaved, scale)
-        ctx.eps = eps
-        ctx.normed = q_weight is not None
-        rows = (q, k, q_weight, k_weight) if ctx.normed else ()
-        ctx.save_for_backward(positions, inv_freq, *rows)
-        return _C.rotary(q, k, positions, inv_freq, interleaved, scale, q_weight, k_weight, eps)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk):
-        positions, inv_freq, *rows = ctx.saved_tensors
-        q, k, q_weight, k_weight = rows if ctx.normed else (dq, dk, None, None)
-        dq, dk, dqw, dkw = _C.rotary_bwd(q, k, dq, dk, positions, inv_freq, *ctx.args, q_weight, k_weight, ctx.eps)
-        return dq, dk, None, None, None, None, dqw, dkw, None
-
-
 def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=None, k_weight=None, eps=1e-6):
     """Rotate queries and keys to their positions, with their per-head norms
     in the same pass (no reference counterpart). Differentiable in q, k and
@@ -367,7 +344,7 @@ def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=Non
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         if (q_weight is None) != (k_weight is None):
             raise ValueError("mtlattn: q_weight and k_weight go together")
-        return _RotaryFn.apply(q, k, *args)
+        return _C.rotary_grad(q, k, *args)
     return _C.rotary(q, k, *args)
 
 

@@ -9,6 +9,8 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <tuple>
 #include <vector>
@@ -641,6 +643,75 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::
     return {dq, dk, dqw, dkw};
 }
 
+// The autograd node of rotary, in C++: a Python one's backward takes the interpreter's lock
+// on the engine's thread (64 tokens, forward and gradients: 85 us, 72 here, of which the engine takes 45). Without norms the
+// backward is the rotation back and needs nothing of the forward; with them it recomputes the
+// norms from q and k.
+struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                                                  const at::Tensor& k, const at::Tensor& positions,
+                                                  const at::Tensor& inv_freq, bool interleaved, double scale,
+                                                  const c10::optional<at::Tensor>& q_weight,
+                                                  const c10::optional<at::Tensor>& k_weight, double eps) {
+        const bool normed = q_weight.has_value();
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["eps"] = eps;
+        if (normed) ctx->save_for_backward({positions, inv_freq, q, k, *q_weight, *k_weight});
+        else ctx->save_for_backward({positions, inv_freq});
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [qo, ko] = rotary(q, k, positions, inv_freq, interleaved, scale, q_weight, k_weight, eps);
+        return {qo, ko};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const bool normed = saved.size() > 2;
+        const at::Tensor &dq = grads[0], &dk = grads[1];
+        c10::optional<at::Tensor> qw, kw;
+        if (normed) {
+            qw = saved[4];
+            kw = saved[5];
+        }
+        torch::autograd::variable_list out(9);
+        const bool again = at::GradMode::is_enabled();
+        {
+            at::AutoGradMode off(false);
+            auto [gq, gk, gqw, gkw] = rotary_bwd(normed ? saved[2] : dq, normed ? saved[3] : dk, dq, dk, saved[0], saved[1],
+                                                 ctx->saved_data["interleaved"].toBool(),
+                                                 ctx->saved_data["scale"].toDouble(), qw, kw,
+                                                 ctx->saved_data["eps"].toDouble());
+            out[0] = gq;
+            out[1] = gk;
+            if (gqw) out[6] = *gqw;
+            if (gkw) out[7] = *gkw;
+        }
+        if (again) {                    // (gradients of these would be wrong without a word: they raise)
+            torch::autograd::variable_list some;
+            for (auto& t : out)
+                if (t.defined()) some.push_back(t.detach().set_requires_grad(true));
+            const auto node = std::make_shared<torch::autograd::DelayedError>(
+                "mtlattn: rotary is once_differentiable: gradients of its gradients are not supported", (int)some.size());
+            some = (*node)(std::move(some));
+            size_t i = 0;
+            for (auto& t : out)
+                if (t.defined()) t = some[i++];
+        }
+        return out;
+    }
+};
+
+// _C.rotary_grad: rotary as a differentiable operation of q, k and the weights.
+std::tuple<at::Tensor, at::Tensor> rotary_grad(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                                               const at::Tensor& inv_freq, bool interleaved, double scale,
+                                               c10::optional<at::Tensor> q_weight, c10::optional<at::Tensor> k_weight,
+                                               double eps) {
+    TORCH_CHECK(q_weight.has_value() == k_weight.has_value(), "mtlattn: q_weight and k_weight go together");
+    auto out = RotaryFunction::apply(q, k, positions, inv_freq, interleaved, scale, q_weight, k_weight, eps);
+    return {out[0], out[1]};
+}
+
 // _C.paged_cache_append: rows k, v [M, Hkv, D] into a 16-bit paged cache, k (and q, whose
 // rows are returned) normed and rotated on the way.
 c10::optional<at::Tensor> paged_cache_append(const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& k_cache,
@@ -945,6 +1016,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("cu_seqlens"),
           py::arg("cu_seqlens_kv"), py::arg("block_table"), py::arg("total"), py::arg("dtype"));
     m.def("rotary", &rotary, "q and k with their heads normed and rotated", py::arg("q"), py::arg("k"),
+          py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0,
+          py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6);
+    m.def("rotary_grad", &rotary_grad, "rotary, differentiable in q, k and the weights", py::arg("q"), py::arg("k"),
           py::arg("positions"), py::arg("inv_freq"), py::arg("interleaved") = false, py::arg("scale") = 1.0,
           py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6);
     m.def("rotary_bwd", &rotary_bwd, "gradients of rotary", py::arg("q"), py::arg("k"), py::arg("dq_out"),
