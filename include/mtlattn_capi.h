@@ -489,10 +489,10 @@ int mtlattn_rotary_bwd(const mtlattn_rotary* r,
  * not used. dtype fp16 or bf16, any page_size >= 1.
  * Rows whose logical position is negative, or whose table column or page does not
  * exist, are not written to the cache (their q is still turned); q_out rows of no
- * sequence are 0. Nothing else of the cache changes. Cache rows that
- * get tokens must stand once in the block tables. q_out may be q; otherwise
- * caches, q_out and the rows must not share memory (K and V side by side in the token rows
- * of one buffer do not); such calls are refused. No workspace; deterministic.
+ * sequence are 0. Nothing else of the cache changes. Cache rows that get tokens must
+ * stand once in the block tables. q_out may be q; otherwise caches, q_out and the rows
+ * must not share memory (K and V side by side in the token rows of one buffer do not);
+ * such calls are refused. No workspace; deterministic.
  */
 int mtlattn_cache_append(const mtlattn_rotary* r,
                          const void* q, int64_t q_row_stride,
@@ -515,8 +515,8 @@ int mtlattn_cache_append(const mtlattn_rotary* r,
  * token j iff tree_mask's byte j of the query's row is not 0 (j < tree_cols; itself
  * included only if the mask says so).
  *   out[row] = sum_j softmax_j(p->scale * q k_j) v_j over the seen keys, lse as for the
- *   forward; rows that see no key: 0 and -inf. Keys that a row does not see do not reach it, whatever
- *   their values.
+ *   forward; rows that see no key: 0 and -inf. Keys that a row does not see do not reach
+ *   it, whatever their values.
  *   p            : dtype fp16/bf16, D in {64, 128}, cu_seqlens_kv the logical lengths
  *                  (prefix sums); total_kv, causal, window and bias are not read.
  *                  max_seqlen_q shapes the launch only, and so does max_seqlen_kv

@@ -240,8 +240,9 @@ struct RopeArgs {
 };
 int rope_part_wgs(int64_t total);             // the most workgroups that leave sums in part
 
-// Attention of drafted tokens' trees over a 16-bit paged cache (launch_tree): rows of
-// 32 to 256 per workgroup, `side` workgroups with other rows side by side, `pieces` of the work, workspace bytes.
+// Attention of drafted tokens' trees over a 16-bit paged cache (launch_tree): rows (32
+// to 256) of a workgroup, `side` workgroups with other rows side by side, `pieces` of
+// the work, workspace bytes.
 constexpr int kTreeMaxCols = 256;              // columns of the mask
 struct TreePlan {
     int rows = 128, side = 1, pieces = 1;

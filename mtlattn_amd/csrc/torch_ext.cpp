@@ -643,10 +643,10 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::
     return {dq, dk, dqw, dkw};
 }
 
-// The autograd node of rotary, in C++: a Python one's backward takes the interpreter's lock
-// on the engine's thread (64 tokens, forward and gradients: 85 us, 72 here, of which the engine takes 45). Without norms the
-// backward is the rotation back and needs nothing of the forward; with them it recomputes the
-// norms from q and k.
+// The autograd node of rotary, in C++: a Python one's backward takes the interpreter's
+// lock on the engine's thread (64 tokens, forward and gradients: 85 us with that, 72
+// here, of which the engine takes 45). Without norms the backward is the rotation back
+// and needs nothing of the forward; with them it recomputes the norms from q and k.
 struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
                                                   const at::Tensor& k, const at::Tensor& positions,

@@ -6,23 +6,30 @@
 //   S[i, j] = scale * q_i . k_j,  P = softmax over the seen j,  O_i = sum_j P[i, j] v_j
 //
 // With few rows (drafted tokens times the heads of a GQA group) the cache's stream
-// bounds it, with many the matrix cores do.
+// bounds it, with many the matrix cores and their softmax do. Measured, bf16, D = 128:
+// 64 sequences of 2 to 8 drafted tokens over 1024 to 16384 keys, 32/8 heads, 415 us,
+// 5.4 TB/s; 4 of 64 over 32768 to 98304, 64/8 heads, 500 us, 1.05 PFLOP/s; one of 16
+// over 700, 14 us.
 //   * A unit of work is up to ROWS = 32 RW of the rows n * g that share a kv head,
-//     against all keys of the sequence, in tiles of KT. All units' tiles are numbered in one line, cut
-//     into equal pieces, one per workgroup that the GPU holds, from the offsets on
-//     the device (no host read): a piece may end one unit and begin the next. Units
-//     inside one piece are written directly; of the others each piece leaves
-//     normalised fp32 rows and their LSEs, two at most (of the unit that an earlier
-//     piece began, of the one that begins here and goes on), for the merge kernel.
-//   * 4 waves share the tiles in LDS: RW of them take other rows, KW = 4 / RW other
+//     against all keys of the sequence, in tiles of KT. All units' tiles are numbered in
+//     one line, cut into equal pieces, from the offsets on the device (no host read): a
+//     piece may end one unit and begin the next. Units inside one piece are written
+//     directly; of the others each piece leaves normalised fp32 rows and their LSEs, two
+//     at most (of the unit that an earlier piece began, of the one that begins here and
+//     goes on), for the merge kernel. A workgroup takes a piece for one kv head; those of
+//     all heads run side by side.
+//   * NW waves share the tiles in LDS: RW of them take other rows, KW = NW / RW other
 //     keys of a tile (their results meet in LDS at the end of the unit), so that few
 //     rows still keep four waves at the stream.
-//   * K and V go from the pages into LDS by direct loads, 16 keys (one page, one
-//     lookup) at a time per wave, one tile ahead. Products and softmax are those of
-//     the flash forward (fwd.hip): S^T = K Q^T, O^T += V^T P^T on 32x32x16 matrix
-//     instructions, softmax statistics and sums in fp32, P rounded to the type of q
-//     for the second product (half a step of each weight: less than the output's own
-//     rounding; the row sum adds the rounded weights).
+//   * K and V go from the pages into a ring of two tiles in LDS by direct loads, 16 keys
+//     (one page) at a time per wave, whose rows were looked up 64 blocks of 16 keys at a
+//     time (one lookup per tile, in front of its loads, cost 20% of a stream). Products
+//     and softmax are those of the flash forward (fwd.hip): S^T = K Q^T, O^T += V^T P^T
+//     on 32x32x16 matrix instructions, operands read four ahead (V's so: 563 -> 507 us on
+//     the long trees), softmax statistics and sums in fp32, P rounded to the type of q
+//     for the second product (half a step of each weight, about the output's own
+//     rounding; all of its bits would take twice the products), whose result is divided
+//     by the sum of the rounded weights; the LSE has the sum of the weights themselves.
 //   * Keys before the tree are seen by every row: their tiles have no masks. The
 //     tree's tiles take 32 bits per row and 32 keys, and there nothing of a key that
 //     a row does not see reaches it, infinities and NaN of V included (a product with 0
@@ -39,7 +46,6 @@ namespace mtlattn {
 namespace {
 
 constexpr int kMaskWords = kTreeMaxCols / 32 + 1;      // of a token's mask; the last one is 0
-constexpr int kMinPiece = 1;                           // shortest piece, in tiles
 // Beginning a unit after another one in a piece takes as long as this many tiles (the last
 // stores, a page lookup and the first tile's loads, one after the other, where the GPU streams:
 // 16 sequences of 8 to 32 drafted tokens over 128 to 4096 keys, 32/8 heads, D = 128: 46.3 us
@@ -170,8 +176,8 @@ __device__ inline void load_masks(CParams* p, uint32_t (*s_mask)[kMaskWords], in
     }
 }
 
-template <typename T, int D, int NW, int RW, int KT, int NBUF>
-__global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 ? 2 : 1) void tree_kernel(TreeKParams) {
+template <typename T, int D, int NW, int RW, int KT>
+__global__ __launch_bounds__(NW * 64, NW == 4 && KT * D <= 8192 ? 2 : 1) void tree_kernel(TreeKParams) {
     constexpr int KW = NW / RW, ROWS = 32 * RW;
     constexpr int NKB = KT / 32 / KW;                  // 32-key blocks of a wave
     constexpr int NPC = 2 * NKB;                       // 16-key chunks of P
@@ -179,13 +185,13 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
     constexpr int TILE = KT * D * 2, STAGE = 2 * TILE;
     constexpr int NI = 16 * D * 2 / 1024;              // direct loads of 16 rows
     constexpr int NU = 2 * KT / 16 / NW;               // 16-row blocks of K or V that a wave stages
-    constexpr int AHEAD = NBUF - 1, LOADS = NU * NI, NS = NKB * DC;
+    constexpr int LOADS = NU * NI, NS = NKB * DC;      // of a wave and tile: direct loads, products of S
     constexpr int kShare = DB * 4096 + 3 * 256;        // bytes of a wave's O, maxima and sums
     constexpr bool SPREAD = LOADS <= NS;               // loads between the products
     using St = TileStager<D, 16, 1>;
-    static_assert(KT % (32 * KW) == 0 && 2 * KT % (16 * NW) == 0, "a tile's keys over the waves");
-    static_assert((KW - 1) * RW * kShare <= NBUF * STAGE, "the waves' results meet in the ring");
-    __shared__ __attribute__((aligned(1024))) char smem[NBUF * STAGE];
+    static_assert(KT % (32 * KW) == 0 && KT % (16 * NW) == 0, "a tile's keys over the waves");
+    static_assert((KW - 1) * RW * kShare <= 2 * STAGE, "the waves' results meet in the ring");
+    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];
     __shared__ uint32_t s_mask[ROWS][kMaskWords];
     __shared__ int s_odd;
 
@@ -213,7 +219,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
             const SeqWork x = seq_work<D, ROWS, KT>(p, min(g0 + lane, n - 1));
             total += lane_value64(wave_scan64(g0 + lane < n ? x.work : 0, lane), 63);
         }
-        piece = max((int64_t)kMinPiece, quotient(total + p->pieces - 1, p->pieces));
+        piece = max((int64_t)1, quotient(total + p->pieces - 1, p->pieces));
         at = piece_id * piece;
         end = min(total, at + piece);
         if (at >= end) {
@@ -243,22 +249,13 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
         }
     }
 
-    // Where this lane's part of a 16-row block lies: instruction j loads row 16 j / NI +
-    // lane / (64 NI / 16), at the chunk that the swizzle puts there (TileStager::lane_off), which is
-    // (its chunk of instruction 0) ^ (16 j / NI rows' part of the swizzle)
+    // Where this lane's part of a 16-row block lies: instruction j loads row LR j + lane / (D / 8), at
+    // the chunk that the swizzle puts there (TileStager::lane_off), which is its chunk of
+    // instruction 0 with the swizzle of LR j rows on top
     constexpr int LR = 64 * 16 / (2 * D);              // rows of an instruction
     const uint32_t chunk0 = (uint32_t)((lane & (D / 8 - 1)) ^ row_swz<D>(lane / (D / 8))) * 16u;
-    uint32_t lane_row[NU > 1 ? 2 : 1];                 // byte offsets of the lane's row of instruction 0, in K and V
-    {
-        CParams* p = params();
-        const uint32_t r = (uint32_t)(lane / (D / 8));
-        if (NU > 1) {
-            lane_row[0] = r * (uint32_t)(2 * p->k_rs);
-            lane_row[NU > 1] = r * (uint32_t)(2 * p->v_rs);
-        } else {
-            lane_row[0] = r * (uint32_t)(2 * (w < NW / 2 ? p->k_rs : p->v_rs));
-        }
-    }
+    const uint32_t lane_krow = (uint32_t)(lane / (D / 8)) * (uint32_t)(2 * params()->k_rs);   // bytes, in K and in V
+    const uint32_t lane_vrow = (uint32_t)(lane / (D / 8)) * (uint32_t)(2 * params()->v_rs);
     const uint32_t rbase = row_base<D>(l32, hi) + kw * NKB * 32 * 2 * D, tbase = TILE + tr_base<D>(lane) + kw * NKB * 32 * 2 * D;
     constexpr float kRescale = std::is_same<T, F16>::value ? 15.f : 32.f;     // (as in the flash forward)
     int4 begun{0, 0, 0, 0};
@@ -308,8 +305,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
             rows_now = cache_row(lookup(0), 0);
             pages_next = lookup(1);
         }
-        // block i of this wave's in tile `it`: whether of K, its first key, its source
-        auto key_side = [&](int i) { return w + i * NW < BPT; };
+        // block i of this wave's in tile `it`, first those of K, then those of V: its first key, its source
+        auto key_side = [](int i) { return i < NU / 2; };
         auto first_key = [&](int it, int i) __attribute__((always_inline)) {
             return min((t0 + it) * KT + 16 * ((w + i * NW) & (BPT - 1)), (len - 1) & ~15);
         };
@@ -326,10 +323,10 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
         auto lane_off = [&](int i, int j) __attribute__((always_inline)) {
             uint32_t c = chunk0;                       // (one add per use, not a register held per load)
             asm volatile("" : "+v"(c));
-            return (c ^ (uint32_t)(row_swz<D>(j * LR) * 16)) + lane_row[NU > 1 ? (i >= NU / 2) : 0];
+            return (c ^ (uint32_t)(row_swz<D>(j * LR) * 16)) + (key_side(i) ? lane_krow : lane_vrow);
         };
         auto stage = [&](int it) __attribute__((always_inline)) {
-            char* buf = smem + it % NBUF * STAGE;
+            char* buf = smem + it % 2 * STAGE;
             next_rows(it);
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
@@ -378,25 +375,25 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
         for (int db = 0; db < DB; ++db) oacc[db] = f32x16_t{};
         auto step = [&](int it, auto masked) __attribute__((always_inline)) {
             constexpr bool MASKED = decltype(masked)::value;
-            if (AHEAD > 1 && it + 1 < n_tiles) wait_vmcnt<LOADS>(); else wait_vmcnt<0>();
+            wait_vmcnt<0>();
             __syncthreads();
             // (a tile that ends past the last key is staged at once, with its rows clamped)
-            const bool more = it + AHEAD < n_tiles;
-            const bool spread = SPREAD && !MASKED && more && (t0 + it + AHEAD + 1) * KT <= len;
-            if (more && !spread) stage(it + AHEAD);
-            const char* kb_ = opaque(smem + it % NBUF * STAGE + rbase);
-            const char* vtb = opaque(smem + it % NBUF * STAGE + tbase);
+            const bool more = it + 1 < n_tiles;
+            const bool spread = SPREAD && !MASKED && more && (t0 + it + 2) * KT <= len;
+            if (more && !spread) stage(it + 1);
+            const char* kb_ = opaque(smem + it % 2 * STAGE + rbase);
+            const char* vtb = opaque(smem + it % 2 * STAGE + tbase);
             f32x16_t sacc[NKB];
 #pragma unroll
             for (int kb = 0; kb < NKB; ++kb) sacc[kb] = f32x16_t{};
             __builtin_amdgcn_s_setprio(1);
             auto products = [&](auto with_loads) __attribute__((always_inline)) {
                 const char* src[NU];
-                char* dst = smem + (it + AHEAD) % NBUF * STAGE + w * NI * 1024;
+                char* dst = smem + (it + 1) % 2 * STAGE + w * NI * 1024;
                 if (decltype(with_loads)::value) {
-                    next_rows(it + AHEAD);
+                    next_rows(it + 1);
 #pragma unroll
-                    for (int i = 0; i < NU; ++i) src[i] = source(it + AHEAD, i);
+                    for (int i = 0; i < NU; ++i) src[i] = source(it + 1, i);
                 }
                 u32x4_t ka[NS];
 #pragma unroll
@@ -467,7 +464,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
             if constexpr (MASKED) {
                 // this wave's share of the tile's V: what is not finite leaves the tile, and is
                 // added below to the rows that see it
-                char* vs = smem + it % NBUF * STAGE + TILE + w * (TILE / NW) + lane * 16;
+                char* vs = smem + it % 2 * STAGE + TILE + w * (TILE / NW) + lane * 16;
 #pragma unroll
                 for (int i = 0; i < TILE / NW / 1024; ++i) {
                     u32x4_t v = ld16(vs + i * 1024);
@@ -497,7 +494,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && NBUF * KT * D * 4 <= 72 * 1024 
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        if (AHEAD > 1 && n_tiles > 1) stage(1);
         // tiles that end before the tree
         const int plain = min(n_tiles, max(0, ctx / KT - t0));
         int it = 0;
@@ -663,7 +659,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeKParams p) {
     if (p.lse != nullptr && l32 == 0) p.lse[rh] = !(sum <= 0.f) ? m + logf(sum) : kNegInf;
 }
 
-template <typename T, int D, int NW, int RW, int KT, int NBUF>
+template <typename T, int D, int NW, int RW, int KT>
 hipError_t launch_rows(const TreeArgs& a, TreeKParams p, hipStream_t st) {
     constexpr int ROWS = 32 * RW;
     char* ws = (char*)a.workspace;
@@ -673,7 +669,7 @@ hipError_t launch_rows(const TreeArgs& a, TreeKParams p, hipStream_t st) {
     p.desc = (int4*)ws;
     p.part_lse = (float*)(ws + grid * sizeof(int4));
     p.part_o = p.part_lse + grid * 2 * ROWS;
-    hipLaunchKernelGGL((tree_kernel<T, D, NW, RW, KT, NBUF>), dim3((unsigned)grid), dim3(NW * 64), 0, st, p);
+    hipLaunchKernelGGL((tree_kernel<T, D, NW, RW, KT>), dim3((unsigned)grid), dim3(NW * 64), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((tree_merge_kernel<T, D, ROWS>), dim3((unsigned)grid, ROWS / 8), dim3(256), 0, st, p);
@@ -697,10 +693,10 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
     p.scale_log2 = (g.scale == 0.f ? 1.f : fabsf(g.scale)) * kLog2e;
     p.q_and = g.scale == 0.f ? 0u : ~0u;
     p.q_xor = g.scale < 0.f ? 0x80008000u : 0u;
-    if (a.plan.rows == 32) return launch_rows<T, D, 4, 1, 128, 2>(a, p, st);
-    if (a.plan.rows == 64) return launch_rows<T, D, 4, 2, 64, 2>(a, p, st);
-    if (a.plan.rows == 128) return launch_rows<T, D, 4, 4, 64, 2>(a, p, st);
-    return launch_rows<T, D, 8, 8, 128, 2>(a, p, st);
+    if (a.plan.rows == 32) return launch_rows<T, D, 4, 1, 128>(a, p, st);
+    if (a.plan.rows == 64) return launch_rows<T, D, 4, 2, 64>(a, p, st);
+    if (a.plan.rows == 128) return launch_rows<T, D, 4, 4, 64>(a, p, st);
+    return launch_rows<T, D, 8, 8, 128>(a, p, st);
 }
 
 }  // namespace
@@ -708,9 +704,10 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
 // Rows of a workgroup: the fewest that hold a sequence's max_q * g rows of a kv head,
 // so that the others' matrix work is not done for nothing, up to 256 (4 sequences of 64 drafted
 // tokens, 64/8 heads, 32768 to 98304 keys: 570 us with 256 rows, 790 with 128, which read the
-// cache twice as often). At D = 64 a long stream takes 64 rows at least, whose two workgroups
-// on a CU overlap better (12 sequences of 512 to 16384 keys, 16 heads, 8 tokens 94 -> 87 us, 32 sequences of
-// 1024 to 16384, 32/8 heads, 4 tokens 134 -> 123; 4 of 100 to 2000, 16 heads, 16 tokens 16 -> 19, which keep 32).
+// cache twice as often). At D = 64 a long stream takes 64 rows at least, whose two
+// workgroups on a CU overlap better (12 sequences of 512 to 16384 keys, 16 heads, 8
+// tokens: 94 us with 32 rows, 87 with 64; 32 of 1024 to 16384, 32/8 heads, 4 tokens: 134
+// and 123; 4 of 100 to 2000, 16 heads, 16 tokens, which keep 32: 16 and 19).
 TreePlan make_tree_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
     TreePlan plan;
     const int64_t rows = (int64_t)std::max(max_q, 1) * g.g;

@@ -259,6 +259,24 @@ def test_far_pages(mt):
     assert torch.equal(out, c.run(mt)[0])
 
 
+def test_the_longest_sequence(mt):
+    """2^31 - 2^16 logical tokens, in two pages again and again: equal keys and values of
+    +-1, whose sums stay exact, over work that passes 2^24 tiles."""
+    n = 2 ** 31 - 2 ** 16
+    k = torch.ones(3, 64, 1, 64, dtype=BF16, device="cuda")
+    v = torch.where(torch.arange(64, device="cuda") % 3 == 0, 1.0, -1.0).to(BF16).expand(3, 64, 1, 64).contiguous()
+    q = torch.ones(1, 1, 64, dtype=BF16, device="cuda")
+    lse = torch.empty(1, 1, device="cuda")
+    mask = torch.ones(1, 1, dtype=torch.bool, device="cuda")
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    ck = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    table = 1 + torch.arange(n // 64, dtype=torch.int32, device="cuda")[None] % 2
+    out = mt.paged_tree_decode(q, k, v, cu, ck, table, mask, 1, n, 0.125, lse)
+    assert torch.equal(out[0, 0], v[0, 0, 0])
+    # (64 products of 0.125; the logarithm in fp32)
+    assert abs(float(lse) - (8.0 + math.log(n))) <= 4 * 2.0 ** -23 * 32
+
+
 def test_bad_pages_are_clamped(mt):
     """Pages and columns that do not exist read the nearest ones that do, as in
     paged_decode."""
