@@ -337,7 +337,10 @@ def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=Non
     q_weight, k_weight: [D] (fp32 or q's dtype), both or neither: heads are
     first divided by sqrt(mean(x^2) + eps) and multiplied by the weight.
     Angles are formed in 64 bits, everything else in fp32, rounded once to
-    q's dtype. inv_freq is a constant. Returns (q, k), contiguous."""
+    q's dtype. inv_freq is a constant. Gradients are the same from run to
+    run. Forward and backward may be captured into a graph together (by
+    torch.autograd.grad, with no eager graph of the same leaves alive: torch
+    would wait for that graph's stream). Returns (q, k), contiguous."""
     if inv_freq.requires_grad:
         raise NotImplementedError("mtlattn: differentiable frequencies (inv_freq.requires_grad) are not supported")
     args = (positions.int(), inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))

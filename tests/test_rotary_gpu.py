@@ -530,6 +530,40 @@ def test_graph_of_forward_and_backward(mt):
         assert all(torch.equal(a, b) for a, b in zip(outs, eager)), i
 
 
+def test_graph_of_a_training_step(mt):
+    """The differentiable operation and its gradients captured together, replayed with
+    new values."""
+    g = torch.Generator().manual_seed(17)
+    m, d = 70, 128
+    data = [t.cuda() for t in (*rows(m, 4, 2, d, BF16, g)[:2], *weights(d, F32, g))]
+    dys = [torch.randn_like(t) for t in data[:2]]
+    pos, f = torch.arange(m, dtype=torch.int32).cuda(), frequencies(d).cuda()
+
+    def step(q, k, wq, wk):
+        out = mt.rotary(q, k, pos, f, q_weight=wq, k_weight=wk)
+        return [t.detach() for t in (*out, *torch.autograd.grad(out, (q, k, wq, wk), dys))]
+
+    leaves = [t.clone().requires_grad_() for t in data]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(*leaves)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*leaves)
+    for i in range(5):
+        for t, leaf in zip(data, leaves):
+            t.copy_(torch.randn(t.shape, generator=g).to(t.dtype))
+            leaf.data.copy_(t)
+        for t in dys:
+            t.copy_(torch.randn(t.shape, generator=g).to(BF16))
+        graph.replay()
+        want = step(*[t.clone().requires_grad_() for t in data])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
 def test_two_streams(mt):
     g = torch.Generator().manual_seed(16)
     f = frequencies(64).cuda()
