@@ -271,6 +271,11 @@ __device__ inline void lds_dma16s(const void* sbase, uint32_t voff, const char* 
     const uint32_t a = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(sbase), "{m0}"(a) : "memory");
 }
+// The same of data that nothing reads again soon: it displaces nothing in the caches.
+__device__ inline void lds_dma16s_once(const void* sbase, uint32_t voff, const char* lds) {
+    const uint32_t a = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(voff), "s"(sbase), "{m0}"(a) : "memory");
+}
 
 // Stages rows [row0, row0 + ROWS) of a [*, D] 16-bit matrix (row stride rs
 // elements) into a swizzled LDS tile with global_load_lds_dwordx4: each
