@@ -9,8 +9,8 @@
 //   dx = r (w g - xn mean(w g xn)),  dw = sum over rows of g xn,  xn = x r.
 //
 // All of it is bound by HBM: a value read, a value written (bf16, 32/8 heads, D = 128: 32768
-// tokens 118 us, 5.7 TB/s; 16384 with norms 66 us, 5.1, their backward 109 us, 4.6; 16384
-// appended with norms 83 us, 4.8; a step of 16 tokens 3 us, its launch). Angles are formed in
+// tokens 116 us, 5.8 TB/s; 16384 with norms 66 us, 5.1, their backward 107 us, 4.7; 16384
+// appended with norms 75 us, 5.3; a step of 16 tokens 3 us, its launch). Angles are formed in
 // 64 bits (in turns, so that the reduction is exact; positions reach millions) and
 // their cosines and sines in 32, once per token and frequency: a wave takes one
 // token, a lane one frequency of it, and the heads of the token share them through
@@ -68,12 +68,20 @@ __device__ inline void turn(int pos, float f, float scale, float sign, float& c,
     s *= scale * sign;
 }
 
-// Eight neighbouring values of a row, as they are stored.
+// Eight neighbouring values of a row, as they are stored. FAR: past the caches, which
+// keep what they hold (values that nothing reads again soon).
 template <typename T>
 struct Row8 {
     u32x4_t x;
-    __device__ inline void load(const typename T::raw* p) { x = ld16(p); }
-    __device__ inline void store(typename T::raw* p) const { st16(p, x); }
+    template <bool FAR = false>
+    __device__ inline void load(const typename T::raw* p) {
+        x = FAR ? __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p)) : ld16(p);
+    }
+    template <bool FAR = false>
+    __device__ inline void store(typename T::raw* p) const {
+        if (FAR) __builtin_nontemporal_store(x, reinterpret_cast<u32x4_t*>(p));
+        else st16(p, x);
+    }
     __device__ inline void get(float* f) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -90,13 +98,22 @@ struct Row8 {
 template <>
 struct Row8<F32> {
     f32x4_t x, y;
+    template <bool FAR = false>
     __device__ inline void load(const float* p) {
-        x = *reinterpret_cast<const f32x4_t*>(p);
-        y = *reinterpret_cast<const f32x4_t*>(p + 4);
+        const f32x4_t* f = reinterpret_cast<const f32x4_t*>(p);
+        x = FAR ? __builtin_nontemporal_load(f) : f[0];
+        y = FAR ? __builtin_nontemporal_load(f + 1) : f[1];
     }
+    template <bool FAR = false>
     __device__ inline void store(float* p) const {
-        *reinterpret_cast<f32x4_t*>(p) = x;
-        *reinterpret_cast<f32x4_t*>(p + 4) = y;
+        f32x4_t* f = reinterpret_cast<f32x4_t*>(p);
+        if (FAR) {
+            __builtin_nontemporal_store(x, f);
+            __builtin_nontemporal_store(y, f + 1);
+        } else {
+            f[0] = x;
+            f[1] = y;
+        }
     }
     __device__ inline void get(float* f) const {
 #pragma unroll
@@ -203,9 +220,15 @@ __device__ inline void table_of(const float* tab, int u, int rot, float* cs, flo
 // Forward (and, without norms, backward: sign = -1), or an append. D and R are
 // multiples of 16, rows 16-byte aligned. A lane holds 16 values of a head (its
 // unit: both members of 8 pairs), 2^units_log2 lanes a head; a wave takes PP passes
-// over its token's heads, whose loads are all under way before the angles.
+// over its token's heads, whose loads are all under way before the angles. Rows come past
+// the caches (16384 tokens of 32/8 heads, D = 128, bf16, not in them: 65 -> 58 us), but
+// those that the backward reads again; an append's go past them too (32 sequences of
+// 1024 new tokens 155 -> 142 us, with a paged decode of them 180 -> 170; 16 of 512 41 ->
+// 38, 50 -> 52), a rotation's do not, which the attention reads (32768 tokens 118 -> 110
+// us alone, but with the attention 407 -> 412).
 template <typename T, bool INTER, bool NORM, bool APPEND, int PP>
 __global__ __launch_bounds__(kWaves * 64) void rope_kernel(RopeKParams p) {
+    constexpr bool FAR_IN = APPEND || !NORM;
     __shared__ __attribute__((aligned(16))) float s_tab[kWaves][kMaxD];
     __shared__ __attribute__((aligned(16))) float s_w[NORM ? 2 * kMaxD : 4];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -235,8 +258,8 @@ __global__ __launch_bounds__(kWaves * 64) void rope_kernel(RopeKParams p) {
         }
         const typename T::raw* x =
             (const typename T::raw*)p.in[part[i]] + token * p.in_rs[part[i]] + (int64_t)hd[i] * p.d;
-        xa[i].load(x + ea);
-        xb[i].load(x + eb);
+        xa[i].template load<FAR_IN>(x + ea);
+        xb[i].template load<FAR_IN>(x + eb);
     }
     Place at{true, 0, 0};
     if (APPEND) at = find_place(p, (int)token, lane);
@@ -288,51 +311,50 @@ __global__ __launch_bounds__(kWaves * 64) void rope_kernel(RopeKParams p) {
             }
         }
         typename T::raw* y = (typename T::raw*)p.out[part[i]] + row * p.out_rs[part[i]] + (int64_t)hd[i] * p.d;
-        xa[i].store(y + ea);
-        xb[i].store(y + eb);
+        xa[i].template store<APPEND>(y + ea);
+        xb[i].template store<APPEND>(y + eb);
     }
 }
 
-// The sums of a workgroup's waves: acc holds, per lane, what its elements of the
-// weights' gradients are (e(j): the element of value j, -1: none).
+// The sums of a workgroup's waves, in their order: acc holds, per lane, what its elements
+// of the weights' gradients are (e(j): the element of value j, -1: none).
 template <int N, typename E>
-__device__ inline void store_part(const RopeKParams& p, float* s_sum, const float (&acc)[2][N], E e, bool first, int w) {
+__device__ inline void store_part(const RopeKParams& p, float (*s_sum)[2][kMaxD], const float (&acc)[2][N], E e, bool first,
+                                  int w) {
+    if (first) {
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-        for (int i = 0; i < kWaves; ++i) {             // (in the order of the waves)
-            __syncthreads();
-            if (i == w && first)
+        for (int side = 0; side < 2; ++side)
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const int at = e(j);
-                    if (at >= 0) s_sum[at] = i == 0 ? acc[side][j] : s_sum[at] + acc[side][j];
-                }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < p.d; i += kWaves * 64)
-            p.part[((int64_t)blockIdx.x * 2 + side) * p.d + i] = s_sum[i];
+            for (int j = 0; j < N; ++j)
+                if (e(j) >= 0) s_sum[w][side][e(j)] = acc[side][j];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * p.d; i += kWaves * 64) {
+        const int side = i >= p.d ? 1 : 0;
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) sum += s_sum[k][side][i - side * p.d];
+        p.part[(int64_t)blockIdx.x * 2 * p.d + i] = sum;
     }
 }
 
 // Backward with norms, on the same units: dy and x in, dx out. A wave goes through
 // every (workgroups * kWaves)-th token, the passes over its query heads, then over its
-// kv heads, the next pass's rows under way meanwhile; its share of dw stays in registers,
-// and one more launch adds the workgroups' sums (no atomics: the same result every time).
+// kv heads, the next pass's rows under way meanwhile (the next two: 120 us against 112);
+// its share of dw stays in registers, and one more launch adds the workgroups' sums (no
+// atomics: the same result every time). With few tokens the waves of a token share its
+// passes. Rows come and go past the caches (16384 tokens 116 -> 110 us, the same with the
+// matrix product that takes them).
 template <typename T, bool INTER>
 __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
     __shared__ __attribute__((aligned(16))) float s_tab[kWaves][kMaxD];
     __shared__ __attribute__((aligned(16))) float s_w[2 * kMaxD];
-    __shared__ float s_sum[kMaxD];
+    __shared__ float s_sum[kWaves][2][kMaxD];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int u = lane & ((1 << p.units_log2) - 1), hl = lane >> p.units_log2, hpw = 64 >> p.units_log2;
     const bool unit = 16 * u < p.d, turns = 16 * u < p.rot;
     int ea, eb;
     unit_chunks<INTER>(u, p.rot, ea, eb);
-    for (int i = threadIdx.x; i < 2 * p.d; i += kWaves * 64) {
-        const int side = i >= p.d ? 1 : 0;
-        s_w[side * kMaxD + i - side * p.d] = weight_at(p, side, i - side * p.d);
-    }
-    __syncthreads();
     const int q_passes = (p.hq + hpw - 1) / hpw, passes = q_passes + (p.hkv + hpw - 1) / hpw;
     struct Rows {
         Row8<T> ga, gb, xa, xb;
@@ -344,21 +366,27 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
         if (unit && hd < (side == 0 ? p.hq : p.hkv)) {
             const typename T::raw* g = (const typename T::raw*)p.in[side] + token * p.in_rs[side] + (int64_t)hd * p.d;
             const typename T::raw* x = (const typename T::raw*)p.x[side] + token * p.x_rs[side] + (int64_t)hd * p.d;
-            r.ga.load(g + ea);
-            r.gb.load(g + eb);
-            r.xa.load(x + ea);
-            r.xb.load(x + eb);
+            r.ga.template load<true>(g + ea);
+            r.gb.template load<true>(g + eb);
+            r.xa.template load<true>(x + ea);
+            r.xb.template load<true>(x + eb);
         }
     };
     float dw[2][16] = {};
-    const int64_t step = (int64_t)gridDim.x * kWaves;
-    int64_t token = (int64_t)blockIdx.x * kWaves + w;
+    const int64_t wave = (int64_t)blockIdx.x * kWaves + w, step = (int64_t)gridDim.x * kWaves / p.slices;
+    const int slice = (int)(wave % p.slices), first = slice * passes / p.slices, end = (slice + 1) * passes / p.slices;
+    int64_t token = wave / p.slices;
     Rows now;
     int pos = 0;
     if (token < p.total) {
-        load(token, 0, now);
+        load(token, first, now);
         if (p.rot > 0) pos = p.positions[token];
     }
+    for (int i = threadIdx.x; i < 2 * p.d; i += kWaves * 64) {
+        const int side = i >= p.d ? 1 : 0;
+        s_w[side * kMaxD + i - side * p.d] = weight_at(p, side, i - side * p.d);
+    }
+    __syncthreads();
     while (token < p.total) {
         float cs[8], sn[8];
         if (p.rot > 0) {
@@ -368,11 +396,11 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
             pos = p.positions[min(token + step, p.total - 1)];
         }
 #pragma unroll 1
-        for (int pass = 0; pass < passes; ++pass) {
-            const bool last = pass + 1 == passes;
+        for (int pass = first; pass < end; ++pass) {
+            const bool last = pass + 1 == end;
             const int64_t next = last ? token + step : token;
             Rows then;
-            if (next < p.total) load(next, last ? 0 : pass + 1, then);
+            if (next < p.total) load(next, last ? first : pass + 1, then);
             const int side = pass < q_passes ? 0 : 1, hd = head_of(pass);
             float va[8], vb[8], fa[8], fb[8];
             now.ga.get(va);
@@ -414,8 +442,8 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
                 now.ga.set(va);
                 now.gb.set(vb);
                 typename T::raw* y = (typename T::raw*)p.out[side] + token * p.out_rs[side] + (int64_t)hd * p.d;
-                now.ga.store(y + ea);
-                now.gb.store(y + eb);
+                now.ga.template store<true>(y + ea);
+                now.gb.template store<true>(y + eb);
             }
             now = then;
         }
@@ -432,14 +460,14 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
 // Any D up to 256, any even R, rows of any alignment: a wave takes kAnyHeads heads of a
 // token, one after the other, a lane per pair or passing element, one element at a time;
 // the angles of the lane's pairs once per token. About a third of the other kernel's
-// rate (16384 tokens of 32/8 heads, D = 128, bf16: 194 us, with norms 242, their backward
-// 474; on aligned rows 62, 76 and 119).
+// rate (16384 tokens of 32/8 heads, D = 128, bf16: 195 us, with norms 244, their backward
+// 377; on aligned rows 55, 74 and 107).
 constexpr int kAnyHeads = 8;
 template <typename T, bool BWD>
-__global__ __launch_bounds__(kWaves * 64) void rope_any_kernel(RopeKParams p, bool append) {
+__global__ __launch_bounds__(kWaves * 64, BWD ? 5 : 1) void rope_any_kernel(RopeKParams p, bool append) {
     constexpr int NS = kMaxD / 64;                     // slots of a lane: pairs (the first NP at most), then single elements
     constexpr int NP = NS / 2;
-    __shared__ float s_sum[kMaxD];
+    __shared__ float s_sum[kWaves][2][kMaxD];
     using raw = typename T::raw;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int pairs = p.rot / 2, slots = p.d - pairs, groups = (p.heads + kAnyHeads - 1) / kAnyHeads;
@@ -631,10 +659,16 @@ RopeKParams params(const RopeArgs& a) {
 }
 
 // Workgroups of the backward with norms, in one round: two per CU of the unit kernel, which its
-// registers hold at every type (16384 tokens of 32/8 heads, D = 128, bf16: 108 us; three per
-// CU 114, four 133, six 126), five of the other one.
-int unit_part_wgs(int64_t total) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>((total + kWaves - 1) / kWaves, 2 * (int64_t)device_cus()));
+// registers hold at every type (16384 tokens of 32/8 heads, D = 128, bf16: 107 us; three per
+// CU 6% slower, four or six 17 to 23%), five of the other one.
+int unit_part_wgs(int64_t total, int slices) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>((total * slices + kWaves - 1) / kWaves, 2 * (int64_t)device_cus()));
+}
+// Waves that share a token's passes: 2 or 4 where the workgroups above have the waves (512
+// tokens of 32/8 heads, D = 128, bf16: 17 us, with one each 21; 8 or 16 the same).
+int bwd_slices(int64_t total) {
+    const int64_t waves = 2 * (int64_t)device_cus() * kWaves;
+    return 4 * total <= waves ? 4 : 2 * total <= waves ? 2 : 1;
 }
 int any_part_wgs(int64_t total, int heads) {
     const int64_t items = total * ((heads + kAnyHeads - 1) / kAnyHeads);
@@ -676,8 +710,10 @@ hipError_t launch_passes(const RopeKParams& p, hipStream_t st) {
 template <typename T>
 hipError_t launch_typed(const RopeArgs& a, hipStream_t st) {
     RopeKParams p = params(a);
-    const bool norm_bwd = a.backward && p.norm, units = whole_units(a, sizeof(typename T::raw));
-    const int part_wgs = units ? unit_part_wgs(a.total) : any_part_wgs(a.total, p.heads);
+    const bool norm_bwd = a.backward && p.norm;
+    if (norm_bwd) p.slices = bwd_slices(a.total);
+    const bool units = whole_units(a, sizeof(typename T::raw));
+    const int part_wgs = units ? unit_part_wgs(a.total, p.slices) : any_part_wgs(a.total, p.heads);
     if (a.total > 0) {
         if (!units) {
             const int64_t items = a.total * ((p.heads + kAnyHeads - 1) / kAnyHeads);
