@@ -240,7 +240,7 @@ struct RopeArgs {
 };
 int rope_part_wgs(int64_t total);             // the most workgroups that leave sums in part
 
-// Attention of drafted tokens' trees over a 16-bit paged cache (launch_tree): rows (32
+// Attention of drafted tokens' trees over a 16-bit paged cache (launch_tree): rows (64
 // to 256) of a workgroup, `side` workgroups with other rows side by side, `pieces` of
 // the work, workspace bytes.
 constexpr int kTreeMaxCols = 256;              // columns of the mask

@@ -7,8 +7,8 @@
 //
 // With few rows (drafted tokens times the heads of a GQA group) the cache's stream
 // bounds it, with many the matrix cores and their softmax do. Measured, bf16, D = 128:
-// 64 sequences of 2 to 8 drafted tokens over 1024 to 16384 keys, 32/8 heads, 415 us,
-// 5.4 TB/s; 4 of 64 over 32768 to 98304, 64/8 heads, 500 us, 1.05 PFLOP/s; one of 16
+// 64 sequences of 2 to 8 drafted tokens over 1024 to 16384 keys, 32/8 heads, 377 us,
+// 5.9 TB/s; 4 of 64 over 32768 to 98304, 64/8 heads, 500 us, 1.05 PFLOP/s; one of 16
 // over 700, 14 us.
 //   * A unit of work is up to ROWS = 32 RW of the rows n * g that share a kv head,
 //     against all keys of the sequence, in tiles of KT. All units' tiles are numbered in
@@ -20,7 +20,7 @@
 //     all heads run side by side.
 //   * NW waves share the tiles in LDS: RW of them take other rows, KW = NW / RW other
 //     keys of a tile (their results meet in LDS at the end of the unit), so that few
-//     rows still keep four waves at the stream.
+//     rows still keep four waves at the stream, two workgroups a CU.
 //   * K and V go from the pages into a ring of two tiles in LDS by direct loads, 16 keys
 //     (one page) at a time per wave, whose rows were looked up 64 blocks of 16 keys at a
 //     time (one lookup per tile, in front of its loads, cost 20% of a stream). The loads
@@ -179,7 +179,7 @@ __device__ inline void load_masks(CParams* p, uint32_t (*s_mask)[kMaskWords], in
 }
 
 template <typename T, int D, int NW, int RW, int KT>
-__global__ __launch_bounds__(NW * 64, NW == 4 && KT * D <= 8192 ? 2 : 1) void tree_kernel(TreeKParams) {
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKParams) {
     constexpr int KW = NW / RW, ROWS = 32 * RW;
     constexpr int NKB = KT / 32 / KW;                  // 32-key blocks of a wave
     constexpr int NPC = 2 * NKB;                       // 16-key chunks of P
@@ -695,7 +695,6 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
     p.scale_log2 = (g.scale == 0.f ? 1.f : fabsf(g.scale)) * kLog2e;
     p.q_and = g.scale == 0.f ? 0u : ~0u;
     p.q_xor = g.scale < 0.f ? 0x80008000u : 0u;
-    if (a.plan.rows == 32) return launch_rows<T, D, 4, 1, 128>(a, p, st);
     if (a.plan.rows == 64) return launch_rows<T, D, 4, 2, 64>(a, p, st);
     if (a.plan.rows == 128) return launch_rows<T, D, 4, 4, 64>(a, p, st);
     return launch_rows<T, D, 8, 8, 128>(a, p, st);
@@ -704,25 +703,23 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
 }  // namespace
 
 // Rows of a workgroup: the fewest that hold a sequence's max_q * g rows of a kv head,
-// so that the others' matrix work is not done for nothing, up to 256 (4 sequences of 64 drafted
-// tokens, 64/8 heads, 32768 to 98304 keys: 570 us with 256 rows, 790 with 128, which read the
-// cache twice as often). At D = 64 a long stream takes 64 rows at least, whose two
-// workgroups on a CU overlap better (12 sequences of 512 to 16384 keys, 16 heads, 8
-// tokens: 94 us with 32 rows, 87 with 64; 32 of 1024 to 16384, 32/8 heads, 4 tokens: 134
-// and 123; 4 of 100 to 2000, 16 heads, 16 tokens, which keep 32: 16 and 19).
+// so that the others' matrix work is not done for nothing, from 64 up to 256 (4 sequences
+// of 64 drafted tokens, 64/8 heads, 32768 to 98304 keys: 570 us with 256 rows, 790 with
+// 128, which read the cache twice as often). 32 rows against 128-key tiles, one workgroup
+// a CU, are 1% faster over long streams (64 sequences of 1024 to 16384 keys, 4 tokens,
+// 32/8 heads: 388 us against 392) and slower over all others, and all of D = 64 (one of
+// 500 17.5 against 14.3; 16 of 128 to 4096 35.6 against 30.8): there are none.
 TreePlan make_tree_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
     TreePlan plan;
     const int64_t rows = (int64_t)std::max(max_q, 1) * g.g;
-    const bool stream = (int64_t)g.num_seqs * g.hkv * ((max_kv + 127) / 128) > 16 * (int64_t)cus;
-    plan.rows = rows <= 32 && !(g.d == 64 && stream) ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    const int kt = plan.rows == 32 || plan.rows == 256 ? 128 : 64;
+    plan.rows = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    const int kt = plan.rows == 256 ? 128 : 64;
     // row tiles of a head side by side, where most sequences have that many
     const int64_t most = (rows + plan.rows - 1) / plan.rows;
     const int64_t usual = ((g.total_q * g.g + g.num_seqs - 1) / g.num_seqs + plan.rows - 1) / plan.rows;
     plan.side = most <= 8 && 4 * usual >= 3 * most ? (int)most : 1;
-    // as many pieces as the GPU holds workgroups for (the ring of two tiles fills a CU's LDS at 128
-    // keys and D = 128, half of it otherwise), or as there are tiles by the bounds
-    const int64_t held = (int64_t)cus * (plan.rows == 256 || (plan.rows == 32 && g.d == 128) ? 1 : 2);
+    // as many pieces as the GPU holds workgroups for, or as there are tiles by the bounds
+    const int64_t held = (int64_t)cus * (plan.rows == 256 ? 1 : 2);
     const int64_t full = std::max<int64_t>(1, held / ((int64_t)g.hkv * plan.side));
     const int64_t units = (int64_t)g.num_seqs * ((most + plan.side - 1) / plan.side);
     const int64_t tiles = std::max<int64_t>(1, (max_kv + kt - 1) / kt);
