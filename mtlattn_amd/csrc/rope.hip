@@ -9,8 +9,8 @@
 //   dx = r (w g - xn mean(w g xn)),  dw = sum over rows of g xn,  xn = x r.
 //
 // All of it is bound by HBM: a value read, a value written (bf16, 32/8 heads, D = 128: 32768
-// tokens 116 us, 5.8 TB/s; 16384 with norms 66 us, 5.1, their backward 107 us, 4.7; 16384
-// appended with norms 75 us, 5.3; a step of 16 tokens 3 us, its launch). Angles are formed in
+// tokens 116 us, 5.8 TB/s; 16384 with norms 66 us, 5.1, their backward 101 us, 5.0; 16384
+// appended with norms 74 us, 5.4; a step of 16 tokens 3 us, its launch). Angles are formed in
 // 64 bits (in turns, so that the reduction is exact; positions reach millions) and
 // their cosines and sines in 32, once per token and frequency: a wave takes one
 // token, a lane one frequency of it, and the heads of the token share them through
