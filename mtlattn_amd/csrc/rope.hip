@@ -9,7 +9,7 @@
 //   dx = r (w g - xn mean(w g xn)),  dw = sum over rows of g xn,  xn = x r.
 //
 // All of it is bound by HBM: a value read, a value written (bf16, 32/8 heads, D = 128: 32768
-// tokens 116 us, 5.8 TB/s; 16384 with norms 66 us, 5.1, their backward 101 us, 5.0; 16384
+// tokens 116 us, 5.8 TB/s; 16384 with norms 66 us, 5.1, their backward 98 us, 5.1; 16384
 // appended with norms 74 us, 5.4; a step of 16 tokens 3 us, its launch). Angles are formed in
 // 64 bits (in turns, so that the reduction is exact; positions reach millions) and
 // their cosines and sines in 32, once per token and frequency: a wave takes one
@@ -344,7 +344,8 @@ __device__ inline void store_part(const RopeKParams& p, float (*s_sum)[2][kMaxD]
 // its share of dw stays in registers, and one more launch adds the workgroups' sums (no
 // atomics: the same result every time). With few tokens the waves of a token share its
 // passes. Rows come and go past the caches (16384 tokens 116 -> 110 us, the same with the
-// matrix product that takes them).
+// matrix product that takes them). All lane moves of dw's sums are under way together (one
+// value's after another's: 4 us more at every size).
 template <typename T, bool INTER>
 __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
     __shared__ __attribute__((aligned(16))) float s_tab[kWaves][kMaxD];
@@ -449,11 +450,11 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
         }
         token += step;
     }
+    for (int o = 1 << p.units_log2; o < 64; o <<= 1)   // (all values' moves under way together)
 #pragma unroll
-    for (int side = 0; side < 2; ++side)
+        for (int side = 0; side < 2; ++side)
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            for (int o = 1 << p.units_log2; o < 64; o <<= 1) dw[side][j] += __shfl_xor(dw[side][j], o);
+            for (int j = 0; j < 16; ++j) dw[side][j] += __shfl_xor(dw[side][j], o);
     store_part<16>(p, s_sum, dw, [&](int j) { return unit ? (j < 8 ? ea + j : eb + j - 8) : -1; }, hl == 0, w);
 }
 
@@ -659,13 +660,14 @@ RopeKParams params(const RopeArgs& a) {
 }
 
 // Workgroups of the backward with norms, in one round: two per CU of the unit kernel, which its
-// registers hold at every type (16384 tokens of 32/8 heads, D = 128, bf16: 107 us; three per
+// registers hold at every type (16384 tokens of 32/8 heads, D = 128, bf16: 103 us; three per
 // CU 6% slower, four or six 17 to 23%), five of the other one.
 int unit_part_wgs(int64_t total, int slices) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((total * slices + kWaves - 1) / kWaves, 2 * (int64_t)device_cus()));
 }
-// Waves that share a token's passes: 2 or 4 where the workgroups above have the waves (512
-// tokens of 32/8 heads, D = 128, bf16: 17 us, with one each 21; 8 or 16 the same).
+// Waves that share a token's passes: 2 or 4 where the workgroups above have the waves (16
+// tokens of 32/8 heads, D = 128, bf16: 8.9 us with the sums, with one each 13.1; 512: 12.7
+// and 14.6; 8 waves the same from 64 tokens on).
 int bwd_slices(int64_t total) {
     const int64_t waves = 2 * (int64_t)device_cus() * kWaves;
     return 4 * total <= waves ? 4 : 2 * total <= waves ? 2 : 1;

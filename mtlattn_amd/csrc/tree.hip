@@ -50,8 +50,8 @@ namespace {
 constexpr int kMaskWords = kTreeMaxCols / 32 + 1;      // of a token's mask; the last one is 0
 // Beginning a unit after another one in a piece takes as long as this many tiles (the last
 // stores, a page lookup and the first tile's loads, one after the other, where the GPU streams:
-// 16 sequences of 8 to 32 drafted tokens over 128 to 4096 keys, 32/8 heads, D = 128: 46.3 us
-// without, 43.3 with 4; 12 of 512 to 16384 keys, 16 heads, D = 64: 93 and 88).
+// 16 sequences of 8 to 32 drafted tokens over 128 to 4096 keys, 32/8 heads, D = 128: 45.2 us
+// without, 43.6 with 4, 44.7 with 7; 12 of 512 to 16384 keys, 16 heads, D = 64: 85, 79, 78).
 constexpr int kUnitCost = 4;
 
 struct TreeKParams {

@@ -111,6 +111,26 @@ def test_many_rows(mt):
     assert all(torch.equal(a, b) for a, b in zip(grads, twice))
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(1, 1, 16), (1, 1, 256), (24, 8, 128), (7, 3, 64)])
+@pytest.mark.parametrize("m", [3, 511, 512, 513, 1023, 1025])
+def test_gradients_of_few_tokens(mt, m, hq, hkv, d):
+    """Four, two or one of the backward's waves share a token's heads, which may be
+    fewer than the waves."""
+    g = torch.Generator().manual_seed(m + d)
+    parts = rows(m, hq, hkv, d, BF16, g)[:2]
+    w = weights(d, F32, g)
+    pos, f = torch.randint(0, 4096, (m,), generator=g, dtype=torch.int32), frequencies(d)
+    leaves = [t.cuda().requires_grad_() for t in (*parts, *w)]
+    dys = [torch.randn(t.shape, generator=g).to(BF16) for t in parts]
+    out = mt.rotary(*leaves[:2], pos.cuda(), f.cuda(), q_weight=leaves[2], k_weight=leaves[3])
+    grads = torch.autograd.grad(out, leaves, [t.cuda() for t in dys])
+    for i, h in enumerate((hq, hkv)):
+        back = oracle.backward(dys[i], parts[i], pos, f, weight=w[i])
+        bounds = backward_bound(dys[i], parts[i], back, f, False, 1.0, w[i], EPS, BF16, m * h)
+        check(grads[i], back[0], bounds[0])
+        check(grads[2 + i], back[1], bounds[1])
+
+
 @pytest.mark.parametrize("d,rot", [(64, 64), (24, 12)])
 def test_far_and_negative_positions(mt, d, rot):
     """Angles of up to 2^31 radians; their product in 64 bits is off by up to
