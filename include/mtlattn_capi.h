@@ -516,7 +516,8 @@ int mtlattn_cache_append(const mtlattn_rotary* r,
  * included only if the mask says so).
  *   out[row] = sum_j softmax_j(p->scale * q k_j) v_j over the seen keys, lse as for the
  *   forward; rows that see no key: 0 and -inf. Keys that a row does not see do not reach
- *   it, whatever their values.
+ *   it, whatever their values. Scores, softmax and sums are fp32; the weights multiply V
+ *   with 16 bits (bf16: two bf16 numbers each) or 22 (fp16); the result is rounded once.
  *   p            : dtype fp16/bf16, D in {64, 128}, cu_seqlens_kv the logical lengths
  *                  (prefix sums); total_kv, causal, window and bias are not read.
  *                  max_seqlen_q shapes the launch only, and so does max_seqlen_kv

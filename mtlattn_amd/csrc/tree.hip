@@ -7,9 +7,9 @@
 //
 // With few rows (drafted tokens times the heads of a GQA group) the cache's stream
 // bounds it, with many the matrix cores and their softmax do. Measured, bf16, D = 128:
-// 64 sequences of 2 to 8 drafted tokens over 1024 to 16384 keys, 32/8 heads, 377 us,
-// 5.9 TB/s; 4 of 64 over 32768 to 98304, 64/8 heads, 500 us, 1.05 PFLOP/s; one of 16
-// over 700, 14 us.
+// 64 sequences of 2 to 8 drafted tokens over 1024 to 16384 keys, 32/8 heads, 380 us,
+// 5.9 TB/s; 4 of 64 over 32768 to 98304, 64/8 heads, 688 us, where the matrix cores
+// run at 1.15 PFLOP/s; one of 16 over 700, 15 us.
 //   * A unit of work is up to ROWS = 32 RW of the rows n * g that share a kv head,
 //     against all keys of the sequence, in tiles of KT. All units' tiles are numbered in
 //     one line, cut into equal pieces, from the offsets on the device (no host read): a
@@ -28,10 +28,13 @@
 //     nothing else displaced since the last call 33 -> 36, displaced 39 -> 37). Products
 //     and softmax are those of the flash forward (fwd.hip): S^T = K Q^T, O^T += V^T P^T
 //     on 32x32x16 matrix instructions, operands read four ahead (V's so: 563 -> 507 us on
-//     the long trees), softmax statistics and sums in fp32, P rounded to the type of q
-//     for the second product (half a step of each weight, about the output's own
-//     rounding; all of its bits would take twice the products), whose result is divided
-//     by the sum of the rounded weights; the LSE has the sum of the weights themselves.
+//     the long trees), softmax statistics and sums in fp32.
+//   * P enters the second product as the sum of two numbers of q's type, itself rounded
+//     and what that left: 16 bits of it in bf16, 22 in fp16, far below the rounding of the
+//     result. (Rounded once, results were off by 2.1-2.3e-3 of their norm in bf16 where
+//     1.7e-3 is their own rounding. Its second part takes half as many products again,
+//     which the streams hide, 377 -> 380 us; few rows 43 -> 45; the long trees, at the matrix
+//     cores' rate, 512 -> 688.) A third part would be below what fp32 scores are off by.
 //   * Keys before the tree are seen by every row: their tiles have no masks. The
 //     tree's tiles take 32 bits per row and 32 keys, and there nothing of a key that
 //     a row does not see reaches it, infinities and NaN of V included (a product with 0
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
     constexpr int NI = 16 * D * 2 / 1024;              // direct loads of 16 rows
     constexpr int NU = 2 * KT / 16 / NW;               // 16-row blocks of K or V that a wave stages
     constexpr int LOADS = NU * NI, NS = NKB * DC;      // of a wave and tile: direct loads, products of S
-    constexpr int kShare = DB * 4096 + 3 * 256;        // bytes of a wave's O, maxima and sums
+    constexpr int kShare = DB * 4096 + 2 * 256;        // bytes of a wave's O, maxima and sums
     constexpr bool SPREAD = LOADS <= NS;               // loads between the products
     using St = TileStager<D, 16, 1>;
     static_assert(KT % (32 * KW) == 0 && KT % (16 * NW) == 0, "a tile's keys over the waves");
@@ -369,9 +372,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
         }
         const float c2 = p->scale_log2;
 
-        // sums: of the rounded weights (l_run) and of the weights (x_run)
         if (threadIdx.x == 0) s_odd = 0;               // a value of V in the tree's tiles is not finite
-        float m_run = kNegInf, l_run = 0.f, x_run = 0.f;
+        float m_run = kNegInf, l_run = 0.f;
         f32x16_t oacc[DB];
 #pragma unroll
         for (int db = 0; db < DB; ++db) oacc[db] = f32x16_t{};
@@ -445,13 +447,12 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
             if (__any(m_new != m_run)) {
                 const float corr = __builtin_amdgcn_exp2f(m_run - (m_new == kNegInf ? 0.f : m_new));
                 l_run *= corr;
-                x_run *= corr;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) oacc[db] *= corr;
             }
             m_run = m_new;
             const float m_use = m_run == kNegInf ? 0.f : m_run;
-            u32x4_t pf[NPC];
+            u32x4_t pf[NPC], pl[NPC];                  // the weights rounded, and what that left of them
 #pragma unroll
             for (int c = 0; c < NPC; ++c)
 #pragma unroll
@@ -459,9 +460,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
                     const int r = 8 * (c & 1) + 2 * j;
                     const float a = __builtin_amdgcn_exp2f(fmaf(sacc[c >> 1][r], c2, -m_use));
                     const float b = __builtin_amdgcn_exp2f(fmaf(sacc[c >> 1][r + 1], c2, -m_use));
-                    x_run += a + b;
+                    l_run += a + b;
                     pf[c][j] = T::pack2(a, b);
-                    l_run = dot2_ones<T>(pf[c][j], l_run);
+                    pl[c][j] = T::pack2(a - lo16<T>(pf[c][j]), b - hi16<T>(pf[c][j]));
                 }
             if constexpr (MASKED) {
                 // this wave's share of the tile's V: what is not finite leaves the tile, and is
@@ -492,6 +493,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 oacc[i % DB] = mfma32<T>(va[i], pf[i / DB], oacc[i % DB]);
+                oacc[i % DB] = mfma32<T>(va[i], pl[i / DB], oacc[i % DB]);
                 if (i + 4 < NV) va[i + 4] = tr_operand<D>(vtb, (i + 4) / DB, (i + 4) % DB);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -504,33 +506,67 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
 #pragma unroll 1
         for (; it < n_tiles; ++it) step(it, std::true_type{});
 
-        if (plain < n_tiles && uniform(s_odd) != 0) {
-            // infinities and NaN of this wave's keys in the tree's tiles, one key after the
-            // other, from the cache
+        // Where a seen value of V is not finite, the column is what such values add up to (an
+        // infinity times the two parts of a weight can be NaN): this wave's keys, from the
+        // cache, 64 at a time, those with such a value one after the other. In the tree's
+        // tiles where V was found to have one, before them where a sum is not finite (of rows
+        // with a weight that is NaN every column is).
+        float lt = pair_sum(l_run), off = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) off = fmaf(oacc[db][r], 0.f, off);
+        const bool odd = plain < n_tiles && uniform(s_odd) != 0, before = __any(off != off && lt == lt);
+        if (odd || before) {
             const uint32_t* words = s_mask[tok - tok0];
-#pragma unroll 1
-            for (int key = (t0 + plain) * KT; key < min(len, t1 * KT); ++key) {
-                if (key / 32 % (KT / 32) / NKB != kw) continue;
-                const int node = key - ctx;
-                const bool see = node < 0 || (node < kTreeMaxCols && (words[node >> 5] >> (node & 31) & 1u) != 0);
+            const int last = min(len, t1 * KT);
+            auto value_row = [&](int key) {
                 const int col = page_log2 >= 0 ? key >> page_log2 : key / page_size;
                 const int pg = min(max(bt[min(col, last_col)], 0), num_pages - 1);
-                const char* vp = vh + ((int64_t)pg * page_size + (key - col * page_size)) * (2 * v_rs) + 8 * hi;
+                return vh + ((int64_t)pg * page_size + (key - col * page_size)) * (2 * v_rs);
+            };
+            f32x16_t x[DB];
 #pragma unroll
-                for (int db = 0; db < DB; ++db)
+            for (int db = 0; db < DB; ++db) x[db] = f32x16_t{};
+#pragma unroll 1
+            for (int key0 = before ? t0 * KT : (t0 + plain) * KT; key0 < last; key0 += 64) {
+                const int mine = min(key0 + lane, last - 1);
+                const char* vp = value_row(mine);
+                u16x2_t top{};
+#pragma unroll 4
+                for (int i = 0; i < D / 8; ++i) {
+                    const u32x4_t v = ld16(vp + 16 * i);
 #pragma unroll
-                    for (int rg = 0; rg < 4; ++rg) {
-                        const u32x2_t x = ld8(vp + 2 * (32 * db + 8 * rg));
+                    for (int j = 0; j < 4; ++j)
+                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, v[j] & 0x7fff7fffu));
+                }
+                uint64_t todo = __ballot(key0 + lane < last && max(top[0], top[1]) >= kInf16<T> &&
+                                         mine / 32 % (KT / 32) / NKB == kw);
+#pragma unroll 1
+                for (; todo != 0; todo &= todo - 1) {
+                    const int key = key0 + __builtin_ctzll(todo), node = key - ctx;
+                    const bool see = node < 0 || (node < kTreeMaxCols && (words[node >> 5] >> (node & 31) & 1u) != 0);
+                    const char* kp = value_row(key) + 8 * hi;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float f = (e & 1) ? hi16<T>(x[e >> 1]) : lo16<T>(x[e >> 1]);
-                            if (see && !(fabsf(f) < kPosInf)) oacc[db][4 * rg + e] += f;
+                    for (int db = 0; db < DB; ++db)
+#pragma unroll
+                        for (int rg = 0; rg < 4; ++rg) {
+                            const u32x2_t y = ld8(kp + 2 * (32 * db + 8 * rg));
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float f = (e & 1) ? hi16<T>(y[e >> 1]) : lo16<T>(y[e >> 1]);
+                                if (see && !(fabsf(f) < kPosInf)) x[db][4 * rg + e] += f;
+                            }
                         }
-                    }
+                }
             }
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!(fabsf(x[db][r]) < kPosInf)) oacc[db][r] = x[db][r];
         }
 
-        float lt = pair_sum(l_run), xt = pair_sum(x_run);
         if (KW > 1) {
             // the waves of other keys leave theirs in the ring, lane by lane
             __syncthreads();
@@ -545,7 +581,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
                 float* sums = reinterpret_cast<float*>(own + DB * 4096) + lane;
                 sums[0] = m_run;
                 sums[64] = lt;
-                sums[128] = xt;
             }
             __syncthreads();
             if (kw == 0) {
@@ -556,7 +591,6 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
                     const float m = nan_max(sums[0], m_run), mu = m == kNegInf ? 0.f : m;
                     const float a = __builtin_amdgcn_exp2f(m_run - mu), b = __builtin_amdgcn_exp2f(sums[0] - mu);
                     lt = lt * a + sums[64] * b;
-                    xt = xt * a + sums[128] * b;
                     m_run = m;
 #pragma unroll
                     for (int db = 0; db < DB; ++db)
@@ -579,7 +613,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : 1) void tree_kernel(TreeKPar
             CParams* p2 = params();
             const int otok = orow / p2->g, ohead = hk * p2->g + orow - otok * p2->g;
             const float inv = !(lt <= 0.f) ? 1.f / lt : 0.f;
-            const float lse = !(xt <= 0.f) ? m_run * kLn2 + logf(xt) : kNegInf;
+            const float lse = !(lt <= 0.f) ? m_run * kLn2 + logf(lt) : kNegInf;
             if (whole) {
                 const int64_t rh = (int64_t)(q0 + otok) * p2->hq + ohead;
                 uint16_t* op = p2->o + rh * D;
