@@ -423,7 +423,10 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
                 sum += __shfl_xor(sum, o);
                 dot += __shfl_xor(dot, o);
             }
-            const float r = 1.f / sqrtf(fmaf(sum, p.inv_d, p.eps));
+            // (lanes without a head hold zeros: their r could be infinite, and the sums of dw take
+            // every lane)
+            const bool there = unit && hd < (side == 0 ? p.hq : p.hkv);
+            const float r = there ? 1.f / sqrtf(fmaf(sum, p.inv_d, p.eps)) : 0.f;
             const float m = dot * r * p.inv_d * r;                     // mean(w g xn) r
             auto add = [&](float (&d)[16]) {
 #pragma unroll
@@ -439,7 +442,7 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
                 va[j] = r * fmaf(va[j], wa[j], -fa[j] * m);
                 vb[j] = r * fmaf(vb[j], wb[j], -fb[j] * m);
             }
-            if (unit && hd < (side == 0 ? p.hq : p.hkv)) {
+            if (there) {
                 now.ga.set(va);
                 now.gb.set(vb);
                 typename T::raw* y = (typename T::raw*)p.out[side] + token * p.out_rs[side] + (int64_t)hd * p.d;
