@@ -438,7 +438,7 @@ typedef struct mtlattn_rotary {
     int32_t rotary_dim;       /* even, 0 (no rotation) .. D */
     int32_t interleaved;      /* 0 / 1 */
     float scale;
-    float eps;
+    float eps;                /* finite, >= 0 (not read without weights) */
     int64_t total;            /* rows */
     const int32_t* positions;      /* device int32 [total] */
     const float* inv_freq;         /* device fp32 [rotary_dim / 2] */

@@ -336,7 +336,8 @@ def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=Non
     of a head are rotated, pairs (i, i + R / 2), or (2 i, 2 i + 1) where
     interleaved; the others pass. scale multiplies what is rotated.
     q_weight, k_weight: [D] (fp32 or q's dtype), both or neither: heads are
-    first divided by sqrt(mean(x^2) + eps) and multiplied by the weight.
+    first divided by sqrt(mean(x^2) + eps), eps >= 0, and multiplied by the
+    weight.
     Angles are formed in 64 bits, everything else in fp32, rounded once to
     q's dtype. inv_freq is a constant. Gradients are the same from run to
     run. Forward and backward may be captured into a graph together (by

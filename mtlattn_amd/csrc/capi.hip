@@ -425,6 +425,8 @@ int check_rotary(const mtlattn_rotary* r, bool append, const char* what) {
     if ((r->q_weight != nullptr || r->k_weight != nullptr) && r->weight_dtype != MTLATTN_DTYPE_F32 &&
         r->weight_dtype != r->dtype)
         return fail(MTLATTN_ERR_INVALID, "%s: weights must be fp32 or of the rows' type", what);
+    if ((r->q_weight != nullptr || r->k_weight != nullptr) && !(r->eps >= 0.f && r->eps < INFINITY))
+        return fail(MTLATTN_ERR_INVALID, "%s: eps must be finite and not negative", what);
     if (r->num_heads_q > 0 && (r->q_weight == nullptr) != (r->k_weight == nullptr))
         return fail(MTLATTN_ERR_INVALID, "%s: q_weight and k_weight go together", what);
     return MTLATTN_OK;
