@@ -363,7 +363,8 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_len
     times factor^(dim / (dim - 2)), so that the slowest pair turns factor
     times slower and the fastest as before; "yarn": pairs that turn fewer
     than beta_slow times over original_length as "linear", more than
-    beta_fast times as trained, a linear blend in between, and a scale of
+    beta_fast times as trained, a linear blend over the pairs in between
+    (between where those turns lie, past the last pair too), and a scale of
     0.1 ln(factor) + 1 (others: 1). Computed in 64 bits, returned in fp32 on
     `device`."""
     dim = int(dim)
@@ -388,8 +389,10 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_len
         # the pair (as a real number) that turns `turns` times over the trained length
         def pair(turns):
             return dim * math.log(original_length / (2 * math.pi * turns)) / (2 * math.log(base))
-        low = min(max(math.floor(pair(beta_fast)), 0), dim // 2 - 1)
-        high = min(max(math.ceil(pair(beta_slow)), 0), dim // 2 - 1)
+        # (the blend may end past the last pair, which then still turns more than beta_slow times;
+        # dim - 1 is where the published form ends it at the latest)
+        low = max(math.floor(pair(beta_fast)), 0)
+        high = min(max(math.ceil(pair(beta_slow)), 0), dim - 1)
         slow = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
         freq = freq * (1.0 - slow) + freq / factor * slow
         if factor > 1:
