@@ -38,7 +38,7 @@ struct RopeKParams {
     float scale, eps, inv_d, sign;      // sign: -1 rotates back
     int interleaved, norm;
     int hq, hkv, heads, d, rot;
-    int64_t total;
+    int64_t total, wg0;                 // rows; forward: workgroups of the launches before this one
     int units_log2, slices;             // lanes of a head (log2), waves that share a token's heads
     // append: the cache rows of k and v
     const int* cu; const int* cu_kv; const int* block_table;
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kWaves * 64) void rope_kernel(RopeKParams p) {
     __shared__ __attribute__((aligned(16))) float s_tab[kWaves][kMaxD];
     __shared__ __attribute__((aligned(16))) float s_w[NORM ? 2 * kMaxD : 4];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * kWaves + w;
+    const int64_t item = (p.wg0 + blockIdx.x) * kWaves + w;
     const int64_t tok = item / p.slices;
     const bool active = tok < p.total;
     const int64_t token = active ? tok : p.total - 1;
@@ -697,9 +697,14 @@ template <typename T, bool INTER, bool NORM, bool APPEND, int PP>
 hipError_t launch_units(RopeKParams p, int passes, hipStream_t st) {
     p.slices = (passes + PP - 1) / PP;
     const int64_t wgs = (p.total * p.slices + kWaves - 1) / kWaves;
-    if (wgs > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((rope_kernel<T, INTER, NORM, APPEND, PP>), dim3((unsigned)wgs), dim3(kWaves * 64), 0, st, p);
-    return hipGetLastError();
+    constexpr int64_t kMost = (int64_t(1) << 32) / (kWaves * 64) - 1;  // (a grid has fewer than 2^32 threads)
+    for (; p.wg0 < wgs; p.wg0 += kMost) {
+        hipLaunchKernelGGL((rope_kernel<T, INTER, NORM, APPEND, PP>), dim3((unsigned)std::min(wgs - p.wg0, kMost)),
+                           dim3(kWaves * 64), 0, st, p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // Two passes per wave from 8192 passes on (2048 tokens of 32/8 heads, D = 128, bf16: 8.1 us, with

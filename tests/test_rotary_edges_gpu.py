@@ -46,3 +46,33 @@ def test_norms_without_an_epsilon(mt, eps, interleaved, hq, hkv, d, rot):
             bounds = backward_bound(dy[i], x[i], back, f, interleaved, 1.0, w[i], eps, dtype, m * h)
             check(grads[i], back[0], bounds[0], "dx")
             check(grads[2 + i], back[1], bounds[1], "dw")
+
+
+def test_more_rows_than_a_grid_has_threads(mt):
+    """2^26 + 5 tokens of a head of 16 elements, a wave each: past the 2^32 threads of a grid.
+    The same bits as in two calls, and the rows about the borders by the oracle."""
+    m, d = (1 << 26) + 5, 16
+    half = 40_000_000
+    pos = torch.arange(m, dtype=torch.int32, device="cuda") % 5003
+    f = frequencies(d)
+    x = [torch.randn(m, 1, d, device="cuda", dtype=BF16, generator=torch.Generator("cuda").manual_seed(i)) for i in range(2)]
+    out = mt.rotary(*x, pos, f.cuda())
+    parts = [mt.rotary(*[t[a] for t in x], pos[a], f.cuda()) for a in (slice(0, half), slice(half, m))]
+    for i in range(2):
+        assert torch.equal(out[i][:half], parts[0][i]) and torch.equal(out[i][half:], parts[1][i])
+    last = 4 * ((1 << 24) - 1)                      # the first row of the second launch
+    rows = torch.tensor([0, 1, half, last - 1, last, last + 1, m - 1])
+    xs = x[0][rows.cuda()].cpu()
+    ref = oracle.forward(xs, pos.cpu()[rows], f)
+    check(out[0][rows.cuda()], ref, forward_bound(xs, ref, f, False, 1.0, None, 0.0, BF16))
+    # the same rows appended, from the last page to the first
+    del out, parts
+    page = 1 << 20
+    pages = -(-m // page)
+    caches = [torch.zeros(pages, page, 1, d, dtype=BF16, device="cuda") for _ in range(2)]
+    cu = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    mt.paged_cache_append(*x, *caches, cu, cu, table)
+    for t, c in zip(x, caches):
+        assert torch.equal(c.flip(0).flatten(0, 1)[:m], t)
+        assert not c.flip(0).flatten(0, 1)[m:].any()
