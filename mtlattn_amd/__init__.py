@@ -279,7 +279,7 @@ def paged_cache_append(k, v, k_cache, v_cache, cu_seqlens, cu_seqlens_kv, block_
     the norms, as for rotary; without inv_freq nothing is rotated, without
     weights nothing normed, and with neither k is copied. positions: int [M],
     by default each token's place in its sequence (drafted tokens of a tree
-    take their depths). q: [M, Hq, D], normed and rotated likewise.
+    take their context's length plus their depth in the tree). q: [M, Hq, D], normed and rotated likewise.
     Returns q's rows (None without q); rows of no sequence are 0.
 
     Rows without a place (a table column or page that does not exist, more
@@ -301,8 +301,8 @@ def paged_tree_decode(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_kv, block_ta
 
     q: [Mq, Hq, D]: sequence s's rows cu_seqlens_q[s]..cu_seqlens_q[s+1] are
     its drafted tokens, which are its last logical tokens; their keys and
-    values are in the cache already (paged_cache_append, with the tokens'
-    depths as positions). tree_mask: bool [Mq, T], T <= 256: a query sees
+    values are in the cache already (paged_cache_append, with the length of
+    their context plus their depth in the tree as positions). tree_mask: bool [Mq, T], T <= 256: a query sees
     every key before the drafted tokens, and of those token j of its sequence
     iff tree_mask[row, j] (itself too only if the mask says so; columns past
     the sequence's tokens are not read, tokens past T are seen by none).

@@ -76,3 +76,62 @@ def test_more_rows_than_a_grid_has_threads(mt):
     for t, c in zip(x, caches):
         assert torch.equal(c.flip(0).flatten(0, 1)[:m], t)
         assert not c.flip(0).flatten(0, 1)[m:].any()
+
+
+def test_positions_of_a_tree_count_from_the_sequence_s_beginning(mt):
+    """Drafted tokens behind a context, their positions as documented (context length +
+    depth): each sees its path as if that had been appended alone, token after token."""
+    g = torch.Generator().manual_seed(21)
+    hq, hkv, d, page = 4, 2, 64, 16
+    contexts, parents = [21, 0, 40], [-1, 0, 0, 1, 2, -1]
+    n = len(parents)
+    paths = []
+    for j, p in enumerate(parents):
+        paths.append((paths[p] if p >= 0 else []) + [j])
+    depth = torch.tensor([len(p) - 1 for p in paths] * len(contexts), dtype=torch.int32, device="cuda")
+    mask = torch.zeros(n, n, dtype=torch.bool)
+    for j, p in enumerate(paths):
+        mask[j, p] = True
+    f = frequencies(d).cuda()
+    old = [[torch.randn(c, hkv, d, generator=g).to(BF16).cuda() for _ in range(2)] for c in contexts]
+    q, k, v = [torch.randn(n * len(contexts), h, d, generator=g).to(BF16).cuda() for h in (hq, hkv, hkv)]
+
+    def cu(lens):
+        return torch.tensor([0] + lens, dtype=torch.int32, device="cuda").cumsum(0).int()
+
+    def caches(b):
+        table = torch.randperm(4 * b, generator=g).view(b, 4).to(torch.int32).cuda()
+        return [torch.zeros(4 * b, page, hkv, d, dtype=BF16, device="cuda") for _ in range(2)] + [table]
+
+    kc, vc, table = caches(len(contexts))
+    mt.paged_cache_append(torch.cat([x[0] for x in old]), torch.cat([x[1] for x in old]), kc, vc, cu(contexts),
+                          cu(contexts), table, inv_freq=f)
+    cu_q, cu_kv = cu([n] * len(contexts)), cu([c + n for c in contexts])
+    drafted = cu_q.diff()
+    context = (cu_kv.diff() - drafted).repeat_interleave(drafted)
+    qr = mt.paged_cache_append(k, v, kc, vc, cu_q, cu_kv, table, q=q, positions=context + depth, inv_freq=f)
+    out = mt.paged_tree_decode(qr, kc, vc, cu_q, cu_kv, table, mask.repeat(len(contexts), 1).cuda(), n,
+                               max(contexts) + n)
+    for s, c in enumerate(contexts):
+        for j, path in enumerate(paths):
+            at = torch.tensor(path, device="cuda") + s * n
+            one_k, one_v, one = caches(1)
+            keys, values = torch.cat((old[s][0], k[at])), torch.cat((old[s][1], v[at]))
+            m = [c + len(path)]
+            rows = torch.zeros(m[0], hq, d, dtype=BF16, device="cuda")
+            rows[-1] = q[s * n + j]
+            turned = mt.paged_cache_append(keys, values, one_k, one_v, cu(m), cu(m), one, q=rows, inv_freq=f)
+            assert torch.equal(turned[-1], qr[s * n + j])
+            # the definition over the rotated rows, in 64 bits
+            p = torch.arange(m[0])
+            kk = one_k.flatten(0, 1)[one[0].cpu()[p // page].long() * page + p % page].double().cpu()
+            vv = values.double().cpu()
+            qq = turned[-1].double().cpu()
+            for h in range(hq):
+                w = torch.softmax((kk[:, h // 2] * qq[h]).sum(-1) / 8.0, 0)
+                ref, size = (w[:, None] * vv[:, h // 2]).sum(0), (w[:, None] * vv[:, h // 2].abs()).sum(0)
+                # scores: 72 U of sum |q k| / 8; two parts of a weight 2^-16, exp2 2^-18, sums 2 U a key; one rounding
+                far = float((kk[:, h // 2].abs() * qq[h].abs()).sum(-1).max()) / 8.0
+                rel = 2.02 * 72 * 2.0 ** -24 * far + 2.0 ** -18 + 2.0 ** -15 + 2 * m[0] * 2.0 ** -24
+                err = (out[s * n + j, h].double().cpu() - ref).abs()
+                assert bool((err <= rel * size + 2.0 ** -8 * ref.abs() + 2.0 ** -25).all()), (s, j, h)
