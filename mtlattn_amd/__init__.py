@@ -262,6 +262,13 @@ def paged_cache_read(k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_seqlens_
                                block_table.int(), int(total), dtype)
 
 
+def _int_positions(positions):
+    if positions.is_floating_point() or positions.is_complex():
+        raise ValueError(f"mtlattn: positions must be integers (got {positions.dtype}); a factor on positions belongs "
+                         "to the frequencies (rotary_frequencies)")
+    return positions.int()
+
+
 def paged_cache_append(k, v, k_cache, v_cache, cu_seqlens, cu_seqlens_kv, block_table, q=None, positions=None,
                        inv_freq=None, interleaved=False, scale=1.0, q_weight=None, k_weight=None, eps=1e-6):
     """Append new K/V rows to the 16-bit paged cache that paged_decode and
@@ -277,8 +284,8 @@ def paged_cache_append(k, v, k_cache, v_cache, cu_seqlens, cu_seqlens_kv, block_
 
     inv_freq, interleaved, scale, q_weight, k_weight, eps: the rotation and
     the norms, as for rotary; without inv_freq nothing is rotated, without
-    weights nothing normed, and with neither k is copied. positions: int [M],
-    by default each token's place in its sequence (drafted tokens of a tree
+    weights nothing normed, and with neither k is copied. positions: integers
+    [M] of 32 bits, by default each token's place in its sequence (drafted tokens of a tree
     take their context's length plus their depth in the tree). q: [M, Hq, D], normed and rotated likewise.
     Returns q's rows (None without q); rows of no sequence are 0.
 
@@ -289,7 +296,7 @@ def paged_cache_append(k, v, k_cache, v_cache, cu_seqlens, cu_seqlens_kv, block_
     q, k and v (caches that are slices of one tensor's token rows do not).
     Not differentiable."""
     if positions is not None:
-        positions = positions.int()
+        positions = _int_positions(positions)
     return _C.paged_cache_append(k, v, k_cache, v_cache, cu_seqlens.int(), cu_seqlens_kv.int(), block_table.int(), q,
                                  positions, inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))
 
@@ -331,7 +338,7 @@ def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=Non
     the weights.
 
     q: [M, Hq, D]; k: [M, Hkv, D] (fp32/fp16/bf16, row-strided views allowed,
-    D <= 256). positions: int [M]. inv_freq: fp32 [R / 2], the angle of a
+    D <= 256). positions: integers [M] in the range of 32 bits. inv_freq: fp32 [R / 2], the angle of a
     pair per position, R <= D (see rotary_frequencies): the first R elements
     of a head are rotated, pairs (i, i + R / 2), or (2 i, 2 i + 1) where
     interleaved; the others pass. scale multiplies what is rotated.
@@ -345,7 +352,7 @@ def rotary(q, k, positions, inv_freq, interleaved=False, scale=1.0, q_weight=Non
     would wait for that graph's stream). Returns (q, k), contiguous."""
     if inv_freq.requires_grad:
         raise NotImplementedError("mtlattn: differentiable frequencies (inv_freq.requires_grad) are not supported")
-    args = (positions.int(), inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))
+    args = (_int_positions(positions), inv_freq, bool(interleaved), float(scale), q_weight, k_weight, float(eps))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         if (q_weight is None) != (k_weight is None):
             raise ValueError("mtlattn: q_weight and k_weight go together")

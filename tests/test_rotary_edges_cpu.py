@@ -5,6 +5,7 @@ import ctypes
 import math
 
 import pytest
+import torch
 
 import mtlattn
 
@@ -48,3 +49,18 @@ def test_yarn_blends_over_the_turns_of_the_trained_length(dim, base, length, fac
         want = base ** (-2 * i / dim) * ((1 - slow) + slow / factor)
         assert math.isclose(float(f[i]), want, rel_tol=1e-7), (i, slow)
     assert math.isclose(min(max((dim // 2 - 1 - ends[0]) / (ends[1] - ends[0]), 0.0), 1.0), last)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.complex64])
+def test_positions_that_are_no_integers_are_refused(dtype):
+    """Positions divided by a factor would lose their fractions: the factor belongs to the
+    frequencies."""
+    x, f = torch.zeros(3, 2, 8), torch.ones(4)
+    pos, cu = torch.arange(3).to(dtype) / 2, torch.tensor([0, 3], dtype=torch.int32)
+    for train in (False, True):
+        with pytest.raises(ValueError, match="mtlattn: positions must be integers"):
+            mtlattn.rotary(x.detach().requires_grad_(train), x, pos, f)
+    cache = torch.zeros(2, 16, 2, 8)
+    with pytest.raises(ValueError, match="mtlattn: positions must be integers"):
+        mtlattn.paged_cache_append(x, x, cache, cache, cu, cu, torch.zeros(1, 2, dtype=torch.int32), positions=pos,
+                                   inv_freq=f)
