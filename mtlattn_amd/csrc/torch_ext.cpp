@@ -596,11 +596,21 @@ at::Tensor gradient_rows(const at::Tensor& t) {
     return inner ? laid_out(t) : t.contiguous();
 }
 
+// Tangents of forward-mode differentiation, which no entry carries on.
+void check_no_tangents(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& q_weight,
+                       const c10::optional<at::Tensor>& k_weight) {
+    auto has = [](const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); };
+    TORCH_CHECK_NOT_IMPLEMENTED(!has(q) && !has(k) && !(defined(q_weight) && has(*q_weight)) &&
+                                    !(defined(k_weight) && has(*k_weight)),
+                                "mtlattn: rotary has no forward-mode derivative (its inputs have tangents)");
+}
+
 // _C.rotary: q and k with their heads normed and rotated.
 std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& positions,
                                           const at::Tensor& inv_freq, bool interleaved, double scale,
                                           c10::optional<at::Tensor> q_weight, c10::optional<at::Tensor> k_weight,
                                           double eps) {
+    check_no_tangents(q_, k_, q_weight, k_weight);
     check_rotated(q_, k_);
     const c10::OptionalDeviceGuard guard(q_.device());
     const auto q = laid_out(q_), k = laid_out(k_);

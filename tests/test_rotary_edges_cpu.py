@@ -6,6 +6,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import mtlattn
 
@@ -64,3 +65,16 @@ def test_positions_that_are_no_integers_are_refused(dtype):
     with pytest.raises(ValueError, match="mtlattn: positions must be integers"):
         mtlattn.paged_cache_append(x, x, cache, cache, cu, cu, torch.zeros(1, 2, dtype=torch.int32), positions=pos,
                                    inv_freq=f)
+
+
+def test_tangents_of_forward_mode_are_refused():
+    """In q, k or a weight, with and without gradients of the other mode."""
+    f, pos = torch.ones(4), torch.arange(3)
+    for which in range(4):
+        for train in (False, True):
+            x = [torch.randn(3, 2, 8), torch.randn(3, 1, 8), torch.randn(8), torch.randn(8)]
+            x = [t.requires_grad_(train) for t in x]
+            with forward_ad.dual_level():
+                x[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+                with pytest.raises(NotImplementedError, match="mtlattn: .*tangents"):
+                    mtlattn.rotary(x[0], x[1], pos, f, q_weight=x[2], k_weight=x[3])
