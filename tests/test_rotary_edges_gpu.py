@@ -135,3 +135,35 @@ def test_positions_of_a_tree_count_from_the_sequence_s_beginning(mt):
                 rel = 2.02 * 72 * 2.0 ** -24 * far + 2.0 ** -18 + 2.0 ** -15 + 2 * m[0] * 2.0 ** -24
                 err = (out[s * n + j, h].double().cpu() - ref).abs()
                 assert bool((err <= rel * size + 2.0 ** -8 * ref.abs() + 2.0 ** -25).all()), (s, j, h)
+
+
+@pytest.mark.parametrize("cu,cu_kv", [([-4, 7, 5, 30], [0, 9, 3, 2 ** 31 - 1]), ([0, 12, 3, 12], [0, 20, 21, 30]),
+                                      ([9, 2, 2, 40], [5, 0, 17, 40]), ([-9, -3, -1, 6], [-7, 3, 4, 9])])
+def test_bad_offsets_write_placed_rows_alone(mt, cu, cu_kv):
+    """Offsets that are not rising, negative or past the rows: what changes in the cache are rows
+    that a table names for one of its sequence's last tokens, each holding a new row."""
+    g = torch.Generator().manual_seed(13)
+    page, m = 16, 12
+    q, k, v = [torch.randn(m, h, 64, generator=g).to(BF16) for h in (4, 2, 2)]
+    caches = torch.full((2, 7, page, 2, 64), -77.0, dtype=BF16, device="cuda")
+    table = torch.tensor([[0, 1], [2, 3], [4, 6]], dtype=torch.int32)
+    kw = dict(q=q.cuda(), inv_freq=frequencies(64).cuda())
+    out = mt.paged_cache_append(k.cuda(), v.cuda(), caches[0], caches[1],
+                                *[torch.tensor(x, dtype=torch.int32, device="cuda") for x in (cu, cu_kv)], table.cuda(), **kw)
+    assert bool(torch.isfinite(out.float()).all())
+    at = caches.cpu().flatten(1, 2)
+    changed = (at != -77.0).flatten(2).any(2)
+    allowed = set()
+    for s in range(3):
+        a = min(max(cu[s], 0), m)
+        n, length = max(min(cu[s + 1], m) - a, 0), max(cu_kv[s + 1] - cu_kv[s], 0)
+        for pos in range(max(length - n, 0), length):
+            if pos // page < 2:
+                allowed.add(int(table[s, pos // page]) * page + pos % page)
+            else:
+                break
+    for side in range(2):
+        assert set(changed[side].nonzero()[:, 0].tolist()) <= allowed
+    assert torch.equal(changed[0], changed[1]) and int(changed[0].sum()) <= m
+    for row in changed[1].nonzero()[:, 0].tolist():
+        assert bool((v.flatten(1) == at[1, row].flatten()).all(1).any())
