@@ -220,15 +220,14 @@ __device__ inline void table_of(const float* tab, int u, int rot, float* cs, flo
 // Forward (and, without norms, backward: sign = -1), or an append. D and R are
 // multiples of 16, rows 16-byte aligned. A lane holds 16 values of a head (its
 // unit: both members of 8 pairs), 2^units_log2 lanes a head; a wave takes PP passes
-// over its token's heads, whose loads are all under way before the angles. Rows come past
-// the caches (16384 tokens of 32/8 heads, D = 128, bf16, not in them: 65 -> 58 us), but
-// those that the backward reads again; an append's go past them too (32 sequences of
-// 1024 new tokens 155 -> 142 us, with a paged decode of them 180 -> 170; 16 of 512 41 ->
-// 38, 50 -> 52), a rotation's do not, which the attention reads (32768 tokens 118 -> 110
-// us alone, but with the attention 407 -> 412).
-template <typename T, bool INTER, bool NORM, bool APPEND, int PP>
+// over its token's heads, whose loads are all under way before the angles. An append's
+// rows go past the caches both ways (32 sequences of 1024 new tokens 155 -> 142 us, with a
+// paged decode of them 180 -> 170; 16 of 512 41 -> 38, 50 -> 52). A rotation's are left in
+// them, for the attention (32768 tokens 118 -> 110 us past them, but with the attention
+// 407 -> 412), and come past them where FAR_IN says so (past_caches), but with
+// norms, whose rows the backward reads again.
+template <typename T, bool INTER, bool NORM, bool APPEND, int PP, bool FAR_IN>
 __global__ __launch_bounds__(kWaves * 64) void rope_kernel(RopeKParams p) {
-    constexpr bool FAR_IN = APPEND || !NORM;
     __shared__ __attribute__((aligned(16))) float s_tab[kWaves][kMaxD];
     __shared__ __attribute__((aligned(16))) float s_w[NORM ? 2 * kMaxD : 4];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -343,11 +342,14 @@ __device__ inline void store_part(const RopeKParams& p, float (*s_sum)[2][kMaxD]
 // kv heads, the next pass's rows under way meanwhile (the next two: 120 us against 112);
 // its share of dw stays in registers, and one more launch adds the workgroups' sums (no
 // atomics: the same result every time). With few tokens the waves of a token share its
-// passes. Rows come and go past the caches (16384 tokens 116 -> 110 us, the same with the
-// matrix product that takes them). All lane moves of dw's sums are under way together (one
-// value's after another's: 4 us more at every size).
+// passes. Rows of 16 bits come and go past the caches (16384 tokens of 32/8 heads, D = 128: 104
+// -> 92 us, all displaced 112 -> 100; 2048: 21 -> 24, displaced 30 -> 23; 16384 of 16/16, D = 64:
+// 47 -> 49, 56 -> 51); those of fp32 do not, whose neighbouring 16 bytes are two loads, so that
+// a line would come twice (16384 of 16/16, D = 80: 176 us past them, 117 not). All lane moves
+// of dw's sums are under way together (one value's after another's: 4 us more at every size).
 template <typename T, bool INTER>
 __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
+    constexpr bool FAR = T::code != F32::code;
     __shared__ __attribute__((aligned(16))) float s_tab[kWaves][kMaxD];
     __shared__ __attribute__((aligned(16))) float s_w[2 * kMaxD];
     __shared__ float s_sum[kWaves][2][kMaxD];
@@ -367,10 +369,10 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
         if (unit && hd < (side == 0 ? p.hq : p.hkv)) {
             const typename T::raw* g = (const typename T::raw*)p.in[side] + token * p.in_rs[side] + (int64_t)hd * p.d;
             const typename T::raw* x = (const typename T::raw*)p.x[side] + token * p.x_rs[side] + (int64_t)hd * p.d;
-            r.ga.template load<true>(g + ea);
-            r.gb.template load<true>(g + eb);
-            r.xa.template load<true>(x + ea);
-            r.xb.template load<true>(x + eb);
+            r.ga.template load<FAR>(g + ea);
+            r.gb.template load<FAR>(g + eb);
+            r.xa.template load<FAR>(x + ea);
+            r.xb.template load<FAR>(x + eb);
         }
     };
     float dw[2][16] = {};
@@ -446,8 +448,8 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
                 now.ga.set(va);
                 now.gb.set(vb);
                 typename T::raw* y = (typename T::raw*)p.out[side] + token * p.out_rs[side] + (int64_t)hd * p.d;
-                now.ga.template store<true>(y + ea);
-                now.gb.template store<true>(y + eb);
+                now.ga.template store<FAR>(y + ea);
+                now.gb.template store<FAR>(y + eb);
             }
             now = then;
         }
@@ -693,18 +695,29 @@ bool whole_units(const RopeArgs& a, int es) {
     return true;
 }
 
-template <typename T, bool INTER, bool NORM, bool APPEND, int PP>
+template <typename T, bool INTER, bool NORM, bool APPEND, int PP, bool FAR_IN>
 hipError_t launch_units(RopeKParams p, int passes, hipStream_t st) {
     p.slices = (passes + PP - 1) / PP;
     const int64_t wgs = (p.total * p.slices + kWaves - 1) / kWaves;
     constexpr int64_t kMost = (int64_t(1) << 32) / (kWaves * 64) - 1;  // (a grid has fewer than 2^32 threads)
     for (; p.wg0 < wgs; p.wg0 += kMost) {
-        hipLaunchKernelGGL((rope_kernel<T, INTER, NORM, APPEND, PP>), dim3((unsigned)std::min(wgs - p.wg0, kMost)),
+        hipLaunchKernelGGL((rope_kernel<T, INTER, NORM, APPEND, PP, FAR_IN>), dim3((unsigned)std::min(wgs - p.wg0, kMost)),
                            dim3(kWaves * 64), 0, st, p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
+}
+
+// Rows in of a rotation without norms come past the caches where they and the rows out are
+// more than the last cache holds (256 MiB), rows of 16 bits only. Just written by another
+// kernel and with that one, bf16, 32/8 heads, D = 128: 16384 tokens (336 MB) 129 -> 123 us,
+// displaced 71 -> 66 alone; 12288 (252 MB) 88 -> 92, 4096 30.8 -> 31.4, 16384 of 16/16, D = 80
+// (168 MB) 36 -> 41, though displaced rows would gain there too (8192 41 -> 38). fp32: a line
+// would come twice (see the backward; 16384 of 16/16, D = 80 80 -> 99, of 32/8, D = 128 122 -> 130).
+bool past_caches(const RopeKParams& p, int es) {
+    constexpr double kLastCache = 256.0 * (1 << 20);
+    return 2.0 * (double)p.total * (p.hq + p.hkv) * p.d * es > kLastCache;
 }
 
 // Two passes per wave from 8192 passes on (2048 tokens of 32/8 heads, D = 128, bf16: 8.1 us, with
@@ -713,8 +726,11 @@ hipError_t launch_units(RopeKParams p, int passes, hipStream_t st) {
 template <typename T, bool INTER, bool NORM, bool APPEND>
 hipError_t launch_passes(const RopeKParams& p, hipStream_t st) {
     const int hpw = 64 >> p.units_log2, passes = (p.heads + hpw - 1) / hpw;
-    if (p.total * passes <= 8192) return launch_units<T, INTER, NORM, APPEND, 1>(p, passes, st);
-    return launch_units<T, INTER, NORM, APPEND, 2>(p, passes, st);
+    if constexpr (!NORM && !APPEND && T::code != F32::code) {
+        if (past_caches(p, sizeof(typename T::raw))) return launch_units<T, INTER, NORM, APPEND, 2, true>(p, passes, st);
+    }
+    if (p.total * passes <= 8192) return launch_units<T, INTER, NORM, APPEND, 1, APPEND>(p, passes, st);
+    return launch_units<T, INTER, NORM, APPEND, 2, APPEND>(p, passes, st);
 }
 
 template <typename T>
