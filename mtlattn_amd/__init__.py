@@ -263,6 +263,8 @@ def paged_cache_read(k_cache, v_cache, k_scale, v_scale, cu_seqlens, cu_seqlens_
 
 
 def _int_positions(positions):
+    if positions.dtype is torch.int32:
+        return positions
     if positions.is_floating_point() or positions.is_complex():
         raise ValueError(f"mtlattn: positions must be integers (got {positions.dtype}); a factor on positions belongs "
                          "to the frequencies (rotary_frequencies)")
