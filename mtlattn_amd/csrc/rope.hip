@@ -9,8 +9,8 @@
 //   dx = r (w g - xn mean(w g xn)),  dw = sum over rows of g xn,  xn = x r.
 //
 // All of it is bound by HBM: a value read, a value written (bf16, 32/8 heads, D = 128: 32768
-// tokens 116 us, 5.8 TB/s; 16384 with norms 66 us, 5.1, their backward 98 us, 5.1; 16384
-// appended with norms 74 us, 5.4; a step of 16 tokens 3 us, its launch). Angles are formed in
+// tokens 116 us, 5.8 TB/s; 16384 with norms 66-72 us, 4.7-5.1, their backward 92-101, 5.0-5.5;
+// 16384 appended with norms 75 us, 5.3; a step of 16 tokens 3 us, its launch). Angles are formed in
 // 64 bits (in turns, so that the reduction is exact; positions reach millions) and
 // their cosines and sines in 32, once per token and frequency: a wave takes one
 // token, a lane one frequency of it, and the heads of the token share them through
@@ -466,8 +466,8 @@ __global__ __launch_bounds__(kWaves * 64) void rope_bwd_kernel(RopeKParams p) {
 // Any D up to 256, any even R, rows of any alignment: a wave takes kAnyHeads heads of a
 // token, one after the other, a lane per pair or passing element, one element at a time;
 // the angles of the lane's pairs once per token. About a third of the other kernel's
-// rate (16384 tokens of 32/8 heads, D = 128, bf16: 195 us, with norms 244, their backward
-// 377; on aligned rows 55, 74 and 107).
+// rate (16384 tokens of 32/8 heads, D = 128, bf16: 194 us, with norms 250, their backward
+// 379; on aligned rows 58, 75 and 98).
 constexpr int kAnyHeads = 8;
 template <typename T, bool BWD>
 __global__ __launch_bounds__(kWaves * 64, BWD ? 5 : 1) void rope_any_kernel(RopeKParams p, bool append) {
@@ -665,14 +665,15 @@ RopeKParams params(const RopeArgs& a) {
 }
 
 // Workgroups of the backward with norms, in one round: two per CU of the unit kernel, which its
-// registers hold at every type (16384 tokens of 32/8 heads, D = 128, bf16: 103 us; three per
-// CU 6% slower, four or six 17 to 23%), five of the other one.
+// registers hold at every type, five of the other one. 32/8 heads, D = 128, us: 16384 tokens
+// bf16 103, fp16 102, fp32 192; three per CU 98, 111, 210 (registers of bf16 alone hold those),
+// four 108 in bf16; 4096 tokens bf16 33.6, fp16 34.3; three 34.5, 37.
 int unit_part_wgs(int64_t total, int slices) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((total * slices + kWaves - 1) / kWaves, 2 * (int64_t)device_cus()));
 }
 // Waves that share a token's passes: 2 or 4 where the workgroups above have the waves (16
-// tokens of 32/8 heads, D = 128, bf16: 8.9 us with the sums, with one each 13.1; 512: 12.7
-// and 14.6; 8 waves the same from 64 tokens on).
+// tokens of 32/8 heads, D = 128, bf16: 9.6 us with the sums, with one each 13.8; 512: 13.2
+// and 15.2; 8 waves the same from 64 tokens on).
 int bwd_slices(int64_t total) {
     const int64_t waves = 2 * (int64_t)device_cus() * kWaves;
     return 4 * total <= waves ? 4 : 2 * total <= waves ? 2 : 1;
@@ -720,9 +721,9 @@ bool past_caches(const RopeKParams& p, int es) {
     return 2.0 * (double)p.total * (p.hq + p.hkv) * p.d * es > kLastCache;
 }
 
-// Two passes per wave from 8192 passes on (2048 tokens of 32/8 heads, D = 128, bf16: 8.1 us, with
-// one 8.3; 16384 appended tokens with norms 84 against 87), one below, for the waves (1024
-// tokens 4.9 us, with two 5.0; 16 tokens with norms 3.3 against 4.1). More than two were slower.
+// Two passes per wave from 8192 passes on (2048 tokens of 32/8 heads, D = 128, bf16: 10.0 us, with
+// one 11.0; 16384 appended tokens with norms 76 against 83), one below, for the waves (1024
+// with norms 7.6 us, with two 7.9; 16 3.7 against 4.5). More than two were slower.
 template <typename T, bool INTER, bool NORM, bool APPEND>
 hipError_t launch_passes(const RopeKParams& p, hipStream_t st) {
     const int hpw = 64 >> p.units_log2, passes = (p.heads + hpw - 1) / hpw;

@@ -9,7 +9,8 @@
 // bounds it, with many the matrix cores and their softmax do. Measured, bf16, D = 128:
 // 64 sequences of 2 to 8 drafted tokens over 1024 to 16384 keys, 32/8 heads, 380 us,
 // 5.9 TB/s; 4 of 64 over 32768 to 98304, 64/8 heads, 688 us, where the matrix cores
-// run at 1.15 PFLOP/s; one of 16 over 700, 15 us.
+// run at 1.15 PFLOP/s, 63% of their cycles at the 1.74 GHz that the GPU then holds; one of
+// 16 over 700, 15 us.
 //   * A unit of work is up to ROWS = 32 RW of the rows n * g that share a kv head,
 //     against all keys of the sequence, in tiles of KT. All units' tiles are numbered in
 //     one line, cut into equal pieces, from the offsets on the device (no host read): a
@@ -24,11 +25,10 @@
 //   * K and V go from the pages into a ring of two tiles in LDS by direct loads, 16 keys
 //     (one page) at a time per wave, whose rows were looked up 64 blocks of 16 keys at a
 //     time (one lookup per tile, in front of its loads, cost 20% of a stream). The loads
-//     leave nothing in the caches (the 64 sequences 415 -> 374 us; 113 MB of cache that
-//     nothing else displaced since the last call 33 -> 36, displaced 39 -> 37). Products
+//     leave nothing in the caches (the 64 sequences 418 -> 381 us; 119 MB of cache that
+//     nothing else displaced since the last call 45 -> 50, displaced 49 -> 47). Products
 //     and softmax are those of the flash forward (fwd.hip): S^T = K Q^T, O^T += V^T P^T
-//     on 32x32x16 matrix instructions, operands read four ahead (V's so: 563 -> 507 us on
-//     the long trees), softmax statistics and sums in fp32.
+//     on 32x32x16 matrix instructions, operands read four ahead (two the same), softmax statistics and sums in fp32.
 //   * P enters the second product as the sum of two numbers of q's type, itself rounded
 //     and what that left: 16 bits of it in bf16, 22 in fp16, far below the rounding of the
 //     result. (Rounded once, results were off by 2.1-2.3e-3 of their norm in bf16 where
@@ -53,8 +53,9 @@ namespace {
 constexpr int kMaskWords = kTreeMaxCols / 32 + 1;      // of a token's mask; the last one is 0
 // Beginning a unit after another one in a piece takes as long as this many tiles (the last
 // stores, a page lookup and the first tile's loads, one after the other, where the GPU streams:
-// 16 sequences of 8 to 32 drafted tokens over 128 to 4096 keys, 32/8 heads, D = 128: 45.2 us
-// without, 43.6 with 4, 44.7 with 7; 12 of 512 to 16384 keys, 16 heads, D = 64: 85, 79, 78).
+// 16 sequences of 8 to 32 drafted tokens over 128 to 4096 keys, 32/8 heads, D = 128: 47.5 us
+// without, 45.2 with 4, 45.9 with 7; 12 of 512 to 16384 keys, 16 heads, D = 64: 89, 80, 79;
+// one of 16 over 700: 16.3, 15.0, 16.1).
 constexpr int kUnitCost = 4;
 
 struct TreeKParams {
@@ -737,12 +738,12 @@ hipError_t launch_typed(const TreeArgs& a, hipStream_t st) {
 }  // namespace
 
 // Rows of a workgroup: the fewest that hold a sequence's max_q * g rows of a kv head,
-// so that the others' matrix work is not done for nothing, from 64 up to 256 (4 sequences
-// of 64 drafted tokens, 64/8 heads, 32768 to 98304 keys: 570 us with 256 rows, 790 with
-// 128, which read the cache twice as often). 32 rows against 128-key tiles, one workgroup
-// a CU, are 1% faster over long streams (64 sequences of 1024 to 16384 keys, 4 tokens,
-// 32/8 heads: 388 us against 392) and slower over all others, and all of D = 64 (one of
-// 500 17.5 against 14.3; 16 of 128 to 4096 35.6 against 30.8): there are none.
+// so that the others' matrix work is not done for nothing, from 64 up to 256. D = 128, us:
+// 16 rows (16 sequences of 4 drafted tokens over 128 to 4096 keys, 32/8 heads) 35.4 with 64, 37.3
+// with 128; 128 rows (8 of 32 over 16384 to 32768) 188 with 128, 290 with 256; 512 rows (4
+// of 64 over 32768 to 98304, 64/8 heads) 678 with 256, 687 with 128, which read the cache
+// twice as often. (32 rows against 128-key tiles, one workgroup a CU, while weights had one part:
+// 64 sequences of 1024 to 16384 keys 388 against 392, one of 500 17.5 against 14.3: there are none.)
 TreePlan make_tree_plan(const Geometry& g, int max_q, int64_t max_kv, int cus) {
     TreePlan plan;
     const int64_t rows = (int64_t)std::max(max_q, 1) * g.g;
