@@ -28,13 +28,14 @@
 //     leave nothing in the caches (the 64 sequences 418 -> 381 us; 119 MB of cache that
 //     nothing else displaced since the last call 45 -> 50, displaced 49 -> 47). Products
 //     and softmax are those of the flash forward (fwd.hip): S^T = K Q^T, O^T += V^T P^T
-//     on 32x32x16 matrix instructions, operands read four ahead (two the same), softmax statistics and sums in fp32.
+//     on 32x32x16 matrix instructions, operands read four ahead (two the same), softmax
+//     statistics and sums in fp32.
 //   * P enters the second product as the sum of two numbers of q's type, itself rounded
 //     and what that left: 16 bits of it in bf16, 22 in fp16, far below the rounding of the
 //     result. (Rounded once, results were off by 2.1-2.3e-3 of their norm in bf16 where
 //     1.7e-3 is their own rounding. Its second part takes half as many products again,
 //     which the streams hide, 377 -> 380 us; few rows 43 -> 45; the long trees, at the matrix
-//     cores' rate, 512 -> 688.) A third part would be below what fp32 scores are off by.
+//     cores' rate, 512 -> 688.)
 //   * Keys before the tree are seen by every row: their tiles have no masks. The
 //     tree's tiles take 32 bits per row and 32 keys, and there nothing of a key that
 //     a row does not see reaches it, infinities and NaN of V included (a product with 0
